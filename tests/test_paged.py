@@ -1,0 +1,498 @@
+"""The paged cache: pages and slots against a list of Python, appended rows and attention against 64 bits, a layer's run of all
+of them, refusals."""
+import math
+
+import pytest
+import torch
+
+import ultraattn_b200 as ua
+from ultraattn_b200.ops import attention as A
+from ultraattn_b200.ops import paged as G
+
+CUDA = pytest.param("cuda", marks=pytest.mark.gpu)
+NAN = float("nan")
+
+
+def _dev(device):
+    if device == "cuda" and not torch.cuda.is_available():
+        pytest.skip("needs a CUDA GPU")
+    return torch.device(device)
+
+
+def _i32(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+# ------------------------------------------------------------------------------------------------
+# pages
+# ------------------------------------------------------------------------------------------------
+def _model(context, new, rows, free, page):
+    """What a step's bookkeeping is, in lists: (rows of pages, free list, cu, pos, slots)."""
+    free, rows = list(free), [list(r) for r in rows]
+    cu, pos, slots = [0], [], []
+    for c, k, row in zip(context, new, rows):
+        while len(row) < -(-c // page):
+            row.append(free.pop())
+        for p in range(c - k, c):
+            pos.append(p)
+            slots.append(row[p // page] * page + p % page if p >= 0 else -1)
+        cu.append(cu[-1] + k)
+    return rows, free, cu, pos, slots
+
+
+def _pool(context, new, page, spare=3, seed=0):
+    """(rows of pages that the requests hold before the step, free list)"""
+    g = torch.Generator().manual_seed(seed)
+    up = lambda x: -(-max(x, 0) // page)
+    order = torch.randperm(sum(up(c) for c in context) + spare, generator=g).tolist()
+    rows = []
+    for c, k in zip(context, new):
+        n = up(c - k)
+        rows.append(order[:n])
+        order = order[n:]
+    return rows, order
+
+
+LENGTHS = {
+    "one": ([1], [1]),
+    "page ends": ([16, 17, 32, 33, 1, 15], [1, 1, 1, 1, 1, 1]),
+    "nothing new": ([5, 0, 40], [0, 0, 0]),
+    "mixed": ([100, 7, 3, 64, 65, 200], [100, 1, 0, 64, 1, 33]),
+    "more new than context": ([2, 30], [5, 30]),
+    "no request": ([], []),
+    "many requests": ([(i * 37) % 211 + 1 for i in range(1500)], [1 if i % 3 else min(9, (i * 37) % 211 + 1) for i in range(1500)]),
+    "many tokens": ([9000, 50, 4000], [9000, 1, 3500]),
+}
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+@pytest.mark.parametrize("page", [1, 16, 64, 256])
+@pytest.mark.parametrize("name", LENGTHS)
+def test_assign_pages(device, page, name):
+    dev = _dev(device)
+    context, new = LENGTHS[name]
+    rows, free = _pool(context, new, page)
+    width = max([-(-c // page) for c in context] + [0]) + 2
+    table = _i32([r + [-7] * (width - len(r)) for r in rows], dev).view(len(rows), width)
+    want_rows, want_free, cu, pos, slots = _model(context, new, rows, free, page)
+    tokens = len(pos) + 3
+    stack, count = _i32(free + [-1, -1], dev), _i32([len(free)], dev)
+    step = ua.paged.assign_pages(_i32(context, dev), _i32(new, dev), table, stack, count, page_size=page, tokens=tokens)
+    assert step.cu_new.tolist() == cu and step.pos.tolist() == pos + [0] * 3 and step.slots.tolist() == slots + [-1] * 3
+    assert table.tolist() == [r + [-7] * (width - len(r)) for r in want_rows]
+    assert step.free_count.tolist() == [len(want_free)] and count.tolist() == [len(free)]
+    assert stack.tolist() == free + [-1, -1]
+    again = ua.paged.assign_pages(_i32(context, dev), _i32(new, dev), table, stack, count, page_size=page, tokens=tokens, count_out=count)
+    assert again.free_count is count and count.tolist() == [len(want_free)] and again.slots.tolist() == step.slots.tolist()
+    if dev.type == "cuda":
+        A.check_status(dev)
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_release_pages(device):
+    dev = _dev(device)
+    context = [33, 16, 0, 17, 1, 1000]
+    ended = [True, False, True, True, False, True]
+    rows, free = _pool(context, [0] * 6, 16)
+    width = 70
+    table = _i32([r + [-7] * (width - len(r)) for r in rows], dev)
+    before = table.clone()
+    back = [p for r, e in zip(rows, ended) if e for p in r]
+    stack, count = _i32(free + [-1] * len(back), dev), _i32([len(free)], dev)
+    left = ua.paged.release_pages(torch.tensor(ended, device=dev), _i32(context, dev), table, stack, count, page_size=16)
+    assert stack.tolist() == free + back and left.tolist() == [len(free) + len(back)] and count.tolist() == [len(free)]
+    assert torch.equal(table, before)
+    # the last page given back is the next one taken
+    step = ua.paged.assign_pages(_i32([1], dev), _i32([1], dev), torch.full((1, 1), -1, dtype=torch.int32, device=dev), stack, left,
+                                 page_size=16, tokens=1)
+    assert step.slots.tolist() == [back[-1] * 16]
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+@pytest.mark.parametrize("why", ["pool", "table", "tokens", "negative", "negative new", "stack"])
+def test_impossible_steps(device, why):
+    """Nothing is assigned, and the error is reported; the call behind it is served again."""
+    dev = _dev(device)
+    context, new, tokens, count = [40, 20], [1, 20], 30, 5
+    if why == "pool":
+        count = 1
+    elif why == "table":
+        context = [40, 50]
+    elif why == "tokens":
+        tokens = 20
+    elif why == "negative":
+        context = [40, -1]
+    elif why == "negative new":
+        new = [1, -3]
+    elif why == "stack":
+        count = 99
+    table = _i32([[9, 8, -7], [-7, -7, -7]], dev)
+    stack, n = _i32([1, 2, 3, 4, 5], dev), _i32([count], dev)
+    args = (table, stack, n)
+
+    def call():
+        return ua.paged.assign_pages(_i32(context, dev), _i32(new, dev), *args, page_size=16, tokens=tokens, count_out=n)
+
+    if dev.type == "cpu":
+        with pytest.raises(RuntimeError):
+            call()
+    else:
+        step = call()
+        assert step.slots.tolist() == [-1] * tokens and step.cu_new.tolist() == [0, 0, 0]
+        with pytest.raises(RuntimeError, match="code=3"):
+            A.check_status(dev)
+    assert table.tolist() == [[9, 8, -7], [-7, -7, -7]] and n.tolist() == [count]
+    n.fill_(5)
+    step = ua.paged.assign_pages(_i32([40, 20], dev), _i32([1, 20], dev), *args, page_size=16, tokens=30)
+    assert table.tolist() == [[9, 8, -7], [5, 4, -7]] and step.free_count.tolist() == [3]      # (39 tokens have had three pages)
+    if dev.type == "cuda":
+        A.check_status(dev)
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_pages_given_back_twice(device):
+    dev = _dev(device)
+    table, stack, n = _i32([[0, 1]], dev), _i32([1, 2, 3], dev), _i32([2], dev)
+    call = lambda: ua.paged.release_pages(torch.tensor([True], device=dev), _i32([20], dev), table, stack, n, page_size=16, count_out=n)
+    if dev.type == "cpu":
+        with pytest.raises(RuntimeError):
+            call()
+    else:
+        call()
+        with pytest.raises(RuntimeError, match="code=3"):
+            A.check_status(dev)
+    assert stack.tolist() == [1, 2, 3] and n.tolist() == [2]
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_page_refusals(device):
+    dev = _dev(device)
+    c, t, f, n = _i32([3, 4], dev), _i32([[0], [1]], dev), _i32([2, 3], dev), _i32([2], dev)
+    ok = dict(page_size=16, tokens=2)
+    bad = [
+        lambda: ua.paged.assign_pages(c, c, t, f, n, page_size=24, tokens=2),
+        lambda: ua.paged.assign_pages(c, c, t, f, n, page_size=0, tokens=2),
+        lambda: ua.paged.assign_pages(c, c, t, f, n, page_size=16, tokens=-1),
+        lambda: ua.paged.assign_pages(c.long(), c, t, f, n, **ok),
+        lambda: ua.paged.assign_pages(c[:1], c, t, f, n, **ok),
+        lambda: ua.paged.assign_pages(c, c, t.t(), f, n, **ok),
+        lambda: ua.paged.assign_pages(c, c, t, f, f, **ok),
+        lambda: ua.paged.assign_pages(c, c, t, f, n, count_out=f, **ok),
+        lambda: ua.paged.release_pages(c, c, t, f, n, page_size=16),
+        lambda: ua.paged.release_pages(torch.tensor([True], device=dev), c, t, f, n, page_size=16),
+        lambda: ua.paged.assign_pages(*(_i32([1] * (G.MAX_REQUESTS + 1), dev),) * 2, _i32([[0]] * (G.MAX_REQUESTS + 1), dev), f, n, **ok),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")
+
+
+# ------------------------------------------------------------------------------------------------
+# append
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,rot,inter,layout", [(128, 128, False, "tokens first"), (128, 96, True, "heads first"), (128, 0, False, "tokens first"),
+                                                  (80, 40, False, "heads first"), (66, 66, True, "tokens first")])
+def test_rotary_append(device, dtype, dim, rot, inter, layout):
+    dev = _dev(device)
+    g = torch.Generator().manual_seed(dim + rot)
+    T, H, Hk, page, pages = 41, 6, 2, 16, 9
+    qkv = torch.randn(T, H + 2 * Hk, dim, generator=g).to(dtype).to(dev)
+    q, k, v = qkv.split([H, Hk, Hk], 1)
+    slots = torch.randperm(pages * page, generator=g)[:T].to(torch.int32)
+    slots[[3, 17]] = -1
+    slots = slots.to(dev)
+    pos = torch.randint(0, 500_000, (T,), generator=g).to(dev)
+    if layout == "tokens first":
+        kc, vc = (torch.randn(pages, page, Hk, dim, generator=g).to(dtype).to(dev) for _ in range(2))
+    else:
+        kc, vc = (torch.randn(pages, Hk, page, dim, generator=g).to(dtype).to(dev).transpose(1, 2) for _ in range(2))
+    want_k, want_v = kc.clone(), vc.clone()
+    f = ua.rotary_frequencies(rot, device=dev)[0] if rot else None
+    turn = (lambda x: ua.ops.rotary.rotate((x,), pos, f, interleaved=inter)[0]) if rot else (lambda x: x)
+    qkv0 = qkv.clone()
+    for t in range(T):
+        s = int(slots[t])
+        if s >= 0:
+            want_k[s // page, s % page], want_v[s // page, s % page] = turn(k)[t], v[t]
+    out = ua.paged.rotary_append(q, k, v, pos, slots, kc, vc, f, interleaved=inter)
+    assert torch.equal(out, turn(q)) and torch.equal(kc, want_k) and torch.equal(vc, want_v) and torch.equal(qkv, qkv0)
+    want_q = turn(q).clone()
+    assert ua.paged.rotary_append(q, k, v, pos, slots, kc, vc, f, interleaved=inter, q_out=q) is q
+    assert torch.equal(q, want_q) and torch.equal(qkv[:, H:], qkv0[:, H:])
+    if dev.type == "cuda":
+        A.check_status(dev)
+        assert ua.paged.rotary_append(q[:0], k[:0], v[:0], pos[:0], slots[:0], kc, vc, f).shape == (0, H, dim)
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_append_refusals(device):
+    dev = _dev(device)
+    q, k = torch.randn(3, 4, 64, device=dev), torch.randn(3, 2, 64, device=dev)
+    c, s, p = torch.zeros(2, 16, 2, 64, device=dev), _i32([0, 1, 32], dev), _i32([0, 1, 2], dev)
+    f = ua.rotary_frequencies(64, device=dev)[0]
+    bad = [
+        lambda: ua.paged.rotary_append(q, k, k[:2], p, s, c, c, f),
+        lambda: ua.paged.rotary_append(q, k, k, p, s[:2], c, c, f),
+        lambda: ua.paged.rotary_append(q, k, k, p, s.long(), c, c, f),
+        lambda: ua.paged.rotary_append(q, k, k, p[:2], s, c, c, f),
+        lambda: ua.paged.rotary_append(q, k, k, p, s, c[:, :, :1], c[:, :, :1], f),
+        lambda: ua.paged.rotary_append(q, k, k, p, s, c, c[:1], f),
+        lambda: ua.paged.rotary_append(q, k, k, p, s, c[:, :12], c[:, :12], f),
+        lambda: ua.paged.rotary_append(q.half(), k, k, p, s, c, c, f),
+        lambda: ua.paged.rotary_append(q, k, k, p, s, c, c, f, q_out=q[:2]),
+        lambda: ua.paged.rotary_append(q[0], k, k, p, s, c, c, f),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")
+    # a slot behind the cache: reported, and not written
+    if dev.type == "cpu":
+        with pytest.raises(RuntimeError):
+            ua.paged.rotary_append(q, k, k, p, s, c, c, f)
+    else:
+        ua.paged.rotary_append(q, k, k, p, s, c, torch.zeros_like(c), f)
+        with pytest.raises(RuntimeError, match="code=3"):
+            A.check_status(dev)
+
+
+# ------------------------------------------------------------------------------------------------
+# attention
+# ------------------------------------------------------------------------------------------------
+def _exact(q, keys, values, context, new, scale, left, sink):
+    """(o, lse, sum p |v|) of one request, fp64: q [new, H, D], keys / values [context, Hk, D]."""
+    q, keys, values = (x.double() for x in (q, keys, values))
+    group = q.shape[1] // max(1, keys.shape[1])
+    k, v = (x.repeat_interleave(group, 1) for x in (keys, values))
+    s = torch.einsum("qhd,khd->hqk", q, k) * scale
+    p = torch.arange(context - new, context, device=q.device)[:, None]
+    j = torch.arange(context, device=q.device)
+    seen = j <= p
+    if left >= 0:
+        seen &= (j >= p - left) | (j < sink)
+    s = s.masked_fill(~seen, -math.inf)
+    z = torch.logsumexp(s, -1) if context else s.new_full(s.shape[:2], -math.inf)
+    w = torch.where(seen, torch.exp(s - torch.where(z.isfinite(), z, 0.0)[..., None]), 0.0)
+    return torch.einsum("hqk,khd->qhd", w, v), z, torch.einsum("hqk,khd->qhd", w, v.abs())
+
+
+def _close(o, lse, want_o, want_lse, weight):
+    """o: half a step of bf16 for the result, half a step of each probability (bf16 operands of P V) times sum p |v|, and 2^-11 of
+    that for the rest: fp32 sums over 128 products move a score of at most 40 by 40 * 128 * 2^-24 < 2^-11. lse: that score
+    error and an fp32 rounding."""
+    half = 2.0 ** -8
+    off = (o.double() - want_o).abs()
+    bound = half * want_o.abs() + (half + 2.0 ** -11) * weight + 1e-30
+    assert (off <= bound).all(), f"o is off by {off.max():.3g}, {(off / bound).max():.3g} of what is allowed"
+    dead = want_lse == -math.inf
+    assert torch.equal(lse == -math.inf, dead)
+    d = (lse.double() - want_lse)[~dead].abs()
+    assert (d <= 2.0 ** -11 + 2.0 ** -22 * want_lse[~dead].abs()).all(), f"lse is off by {d.max():.3g}"
+
+
+def _problem(dev, context, new, H, Hk, page, dtype=torch.bfloat16, layout="tokens first", seed=0, pad=0, scale_q=1.0, D=128, extra=2):
+    """A cache whose every place that no request has written holds NaN, and what its requests have written."""
+    g = torch.Generator().manual_seed(seed + sum(context) + 7 * H + page)
+    n_pages = [-(-c // page) for c in context]
+    total, width = sum(n_pages) + extra, max(n_pages + [0]) + 1
+    order = torch.randperm(total, generator=g).tolist()
+    table, at = [], 0
+    for n in n_pages:
+        table.append(order[at:at + n] + [-1] * (width - n))         # (entries behind the last page name none)
+        at += n
+    shape = (total, page, Hk, D) if layout == "tokens first" else (total, Hk, page, D)
+    kc, vc = (torch.full(shape, NAN, dtype=dtype, device=dev) for _ in range(2))
+    if layout != "tokens first":
+        kc, vc = kc.transpose(1, 2), vc.transpose(1, 2)
+    keys, values = [], []
+    for c, row in zip(context, table):
+        k, v = (torch.randn(c, Hk, D, generator=g).to(dtype).to(dev) for _ in range(2))
+        j = torch.arange(c)
+        idx = torch.tensor(row, device=dev)[(j // page).to(dev)]
+        kc[idx, (j % page).to(dev)], vc[idx, (j % page).to(dev)] = k, v
+        keys.append(k), values.append(v)
+    T = sum(new)
+    q = (torch.randn(T + pad, H, D, generator=g) * scale_q).to(dtype).to(dev)
+    cu = [0]
+    for k in new:
+        cu.append(cu[-1] + k)
+    return q, kc, vc, _i32(table, dev).view(len(context), width), _i32(context, dev), _i32(cu, dev), keys, values
+
+
+def _check(dev, context, new, H, Hk, page, left=-1, sink=0, most_new=None, softmax_scale=None, **more):
+    q, kc, vc, table, ctx, cu, keys, values = _problem(dev, context, new, H, Hk, page, **more)
+    o, lse = ua.paged_attention(q, kc, vc, table, ctx, cu, most_new=most_new, window_size=(left, 0), sink_tokens=sink,
+                                softmax_scale=softmax_scale)
+    a = 0
+    for c, k, kk, vv in zip(context, new, keys, values):
+        want = _exact(q[a:a + k], kk, vv, c, k, 128 ** -0.5 if softmax_scale is None else softmax_scale, left, sink)
+        _close(o[a:a + k], lse[:, a:a + k], *want)
+        a += k
+    if dev.type == "cuda":
+        A.check_status(dev)
+        o2, lse2 = ua.paged_attention(q, kc, vc, table, ctx, cu, most_new=most_new, window_size=(left, 0), sink_tokens=sink,
+                                      softmax_scale=softmax_scale)
+        assert torch.equal(o[:a], o2[:a]) and torch.equal(lse[:, :a], lse2[:, :a])          # no sum depends on timing
+    return o, lse
+
+
+# (context, new) of the requests
+BATCHES = {
+    "one key": ([1], [1]),
+    "decode short": ([2, 15, 16, 17, 127, 128, 129, 130], [1] * 8),
+    "decode long": ([3001, 5, 2048, 777], [1] * 4),
+    "decode one long": ([9001], [1]),
+    "prompts": ([5, 128, 129, 300], [5, 128, 129, 300]),
+    "chunks": ([400, 1000, 513], [3, 130, 257]),
+    "mixed": ([900, 1, 640, 64, 333, 2000], [1, 1, 300, 0, 333, 1]),
+    "more new than context": ([2, 40, 0], [5, 40, 3]),
+    "nothing new": ([50, 70], [0, 0]),
+    "chunk behind a long context": ([5000], [200]),
+}
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+@pytest.mark.parametrize("name", BATCHES)
+@pytest.mark.parametrize("heads,kv,page", [(8, 2, 16), (4, 4, 64), (7, 1, 128), (6, 2, 32), (16, 1, 256)])
+def test_attention(device, name, heads, kv, page):
+    _check(_dev(device), *BATCHES[name], heads, kv, page)
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+@pytest.mark.parametrize("name", BATCHES)
+@pytest.mark.parametrize("left,sink,page", [(0, 0, 16), (63, 4, 16), (127, 0, 64), (128, 130, 128), (500, 1, 256), (10_000, 4, 32)])
+def test_attention_window(device, name, left, sink, page):
+    _check(_dev(device), *BATCHES[name], 8, 2, page, left, sink)
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_attention_ignores_pages_outside_the_window(device):
+    """Pages that no query sees any more may be given back: their entries name no page, or one that holds anything."""
+    dev = _dev(device)
+    context, new, left, page = [1000, 700], [1, 90], 100, 16
+    q, kc, vc, table, ctx, cu, keys, values = _problem(dev, context, new, 8, 2, page)
+    o, lse = ua.paged_attention(q, kc, vc, table, ctx, cu, window_size=(left, 0))
+    for r, (c, k) in enumerate(zip(context, new)):
+        first = (c - k - left) // page                  # the page of the first key that is seen
+        table[r, :first] = _i32([-1, 1 << 30], dev)[torch.arange(first, device=dev) % 2]
+        j = (c - k - left) % page
+        kc[table[r, first].long(), :j], vc[table[r, first].long(), :j] = NAN, float("inf")
+    o2, lse2 = ua.paged_attention(q, kc, vc, table, ctx, cu, window_size=(left, 0))
+    assert torch.equal(o, o2) and torch.equal(lse, lse2) and o.isfinite().all()
+    if dev.type == "cuda":
+        A.check_status(dev)
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_attention_layouts_and_padding(device):
+    """Heads before tokens in a page, queries that are views, more rows than tokens (left alone), a scale, own outputs."""
+    dev = _dev(device)
+    context, new = [300, 77, 1030], [1, 20, 1]
+    for layout in ("tokens first", "heads first"):
+        _check(dev, context, new, 8, 2, 32, layout=layout, softmax_scale=0.03)
+        _check(dev, context, new, 8, 2, 32, layout=layout, most_new=20)
+    q, kc, vc, table, ctx, cu, _, _ = _problem(dev, context, new, 8, 2, 32, pad=13)
+    want_o, want_lse = ua.paged_attention(q, kc, vc, table, ctx, cu)
+    packed = torch.randn(q.shape[0], 8 * 128 + 40, device=dev).to(torch.bfloat16)
+    view = packed[:, 8:8 + 1024].unflatten(1, (8, 128))
+    view.copy_(q)
+    o = torch.full((q.shape[0], 9, 136), 7.0, dtype=torch.bfloat16, device=dev)[:, 1:, 8:]
+    lse = torch.full((8, q.shape[0] + 5), 7.0, device=dev)[:, 3:-2]
+    r = ua.paged_attention(view, kc, vc, table, ctx, cu, out=(o, lse))
+    assert r[0] is o and r[1] is lse
+    assert torch.equal(o[:22], want_o[:22]) and torch.equal(lse[:, :22], want_lse[:, :22])
+    assert (o[22:] == 7).all() and (lse[:, 22:] == 7).all()
+    odd = torch.empty(q.shape[0] * 8 * 128 + 1, dtype=torch.bfloat16, device=dev)[1:].view(q.shape)
+    odd.copy_(q)
+    assert torch.equal(ua.paged_attention(odd, kc, vc, table, ctx, cu)[0][:22], want_o[:22])
+    heads_first = q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(ua.paged_attention(heads_first, kc, vc, table, ctx, cu)[0][:22], want_o[:22])
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_attention_large_scores(device):
+    """Scores far apart, of which one key takes all the weight: the running maximum moves."""
+    _check(_dev(device), [700, 260], [1, 260], 8, 2, 64, scale_q=4.0)
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_attention_shared_pages(device):
+    """Two requests that name the same pages for a common beginning."""
+    dev = _dev(device)
+    q, kc, vc, table, ctx, cu, keys, values = _problem(dev, [150, 150], [1, 1], 4, 2, 16)
+    table[1, :8] = table[0, :8]
+    o, lse = ua.paged_attention(q, kc, vc, table, ctx, cu)
+    for r in range(2):
+        kk, vv = (torch.cat([x[0][:128], x[r][128:]]) for x in (keys, values))
+        _close(o[r:r + 1], lse[:, r:r + 1], *_exact(q[r:r + 1], kk, vv, 150, 1, 128 ** -0.5, -1, 0))
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_attention_bad_pages(device):
+    """A page that the cache does not have, where a query needs it: reported; the other requests come out as they are."""
+    dev = _dev(device)
+    q, kc, vc, table, ctx, cu, keys, values = _problem(dev, [100, 200, 50], [1, 1, 20], 4, 2, 16)
+    want, _ = ua.paged_attention(q, kc, vc, table, ctx, cu)
+    for entry in (-1, kc.shape[0]):
+        t = table.clone()
+        t[1, 3] = entry
+        if dev.type == "cpu":
+            with pytest.raises(RuntimeError):
+                ua.paged_attention(q, kc, vc, t, ctx, cu)
+            continue
+        o, _ = ua.paged_attention(q, kc, vc, t, ctx, cu)
+        torch.cuda.synchronize()
+        assert torch.equal(o[0], want[0]) and torch.equal(o[2:], want[2:])
+        with pytest.raises(RuntimeError, match="code=3"):
+            A.check_status(dev)
+    short = table[:, :-4].contiguous()              # a table without the columns of the longest request
+    if dev.type == "cpu":
+        with pytest.raises(RuntimeError):
+            ua.paged_attention(q, kc, vc, short, ctx, cu)
+    else:
+        o, _ = ua.paged_attention(q, kc, vc, short, ctx, cu)
+        assert torch.equal(o[0], want[0]) and torch.equal(o[2:], want[2:])
+        with pytest.raises(RuntimeError, match="code=3"):
+            A.check_status(dev)
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_attention_refusals(device):
+    dev = _dev(device)
+    q, kc, vc, table, ctx, cu, _, _ = _problem(dev, [100, 20], [1, 3], 4, 2, 16)
+    f = ua.paged_attention
+    bad = [
+        lambda: f(q[:, :3], kc, vc, table, ctx, cu),
+        lambda: f(q, kc, vc[:-1], table, ctx, cu),
+        lambda: f(q, kc, vc, table.long(), ctx, cu),
+        lambda: f(q, kc, vc, table, ctx[:1], cu),
+        lambda: f(q, kc, vc, table, ctx, cu[:-1]),
+        lambda: f(q, kc, vc, table.t().contiguous().t(), ctx, cu),
+        lambda: f(q[..., :64], kc, vc, table, ctx, cu),
+        lambda: f(q, kc[:, :12], vc[:, :12], table, ctx, cu),
+        lambda: f(q, kc, vc, table, ctx, cu, window_size=(5, 3)),
+        lambda: f(q, kc, vc, table, ctx, cu, sink_tokens=3),
+        lambda: f(q, kc, vc, table, ctx, cu, sink_tokens=-1, window_size=(5, 0)),
+        lambda: f(q, kc, vc, table, ctx, cu, most_new=-1),
+        lambda: f(q, kc, vc, table, ctx, cu, out=(q[:2], torch.empty(4, 4, device=dev))),
+        lambda: f(q, kc, vc, table, ctx, cu, out=(torch.empty_like(q), torch.empty(4, 4, device=dev).half())),
+        lambda: f(q.float(), kc, vc, table, ctx, cu),
+        lambda: f(q[0], kc, vc, table, ctx, cu),
+    ]
+    if dev.type == "cuda":
+        bad += [
+            lambda: f(q.half(), kc.half(), vc.half(), table, ctx, cu),
+            lambda: f(q[..., :64], kc[..., :64], vc[..., :64], table, ctx, cu),
+            lambda: f(q, kc[:, :8], vc[:, :8], table, ctx, cu),
+            lambda: f(q, kc.cpu(), vc.cpu(), table, ctx, cu),
+            lambda: f(q, kc, vc, table.cpu(), ctx, cu),
+        ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")
+    empty = f(q[:0], kc, vc, table[:0], ctx[:0], cu[:1])
+    assert empty[0].shape == (0, 4, 128) and empty[1].shape == (4, 0)

@@ -1,0 +1,208 @@
+"""The general rotary embedding: frequencies, restatement and kernel against complex products in 64 bits, gradients against
+differences, refusals."""
+import math
+
+import pytest
+import torch
+
+import ultraattn_b200 as ua
+from ultraattn_b200.ops import rotary as R
+
+CUDA = pytest.param("cuda", marks=pytest.mark.gpu)
+
+
+def _dev(device):
+    if device == "cuda" and not torch.cuda.is_available():
+        pytest.skip("needs a CUDA GPU")
+    return torch.device(device)
+
+
+def _exact(x, pos, inv_freq, magnitude=1.0, interleaved=False, inverse=False):
+    """Pairs as complex numbers times magnitude * exp(+- i pos f), fp64."""
+    x, n = x.double().cpu(), inv_freq.numel()
+    z = torch.complex(x[..., 0:2 * n:2], x[..., 1:2 * n:2]) if interleaved else torch.complex(x[..., :n], x[..., n:2 * n])
+    ang = pos.cpu().double()[..., None] * inv_freq.cpu() * (-1 if inverse else 1)
+    z = z * torch.polar(torch.full_like(ang, magnitude), ang)[..., None, :]
+    y = x.clone()
+    if interleaved:
+        y[..., 0:2 * n:2], y[..., 1:2 * n:2] = z.real, z.imag
+    else:
+        y[..., :n], y[..., n:2 * n] = z.real, z.imag
+    return y
+
+
+def _tolerance(x, y, n, magnitude, interleaved):
+    """Half a step of the type, and the fp32 arithmetic in front of it: sine and cosine to 2 units in the last place, their argument
+    and their product with the magnitude to half a one, product and sum of the rotation to half a one each, every one at
+    most 2^-24 of |a| + |b|: 6 together, 8 allowed."""
+    x = x.double().cpu().abs()
+    s = torch.zeros_like(x)
+    if interleaved:
+        t = x[..., 0:2 * n:2] + x[..., 1:2 * n:2]
+        s[..., 0:2 * n:2] = s[..., 1:2 * n:2] = t
+    else:
+        t = x[..., :n] + x[..., n:2 * n]
+        s[..., :n] = s[..., n:2 * n] = t
+    return y, s * magnitude * 8 * 2.0 ** -24
+
+
+def _assert_close(got, x, want, n, magnitude, interleaved):
+    y, arith = _tolerance(x, want, n, magnitude, interleaved)
+    bound = torch.finfo(got.dtype).eps / 2 * (y.abs() + arith) + arith + torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
+    off = (got.double().cpu() - y).abs()
+    assert (off <= bound).all(), f"off by {off.max():.3g}, {(off / bound.clamp(min=1e-300)).max():.3g} of what is allowed"
+
+
+# ------------------------------------------------------------------------------------------------
+def test_frequencies_without_scaling():
+    f, m = ua.rotary_frequencies(128)
+    assert m == 1.0 and f.dtype == torch.float64
+    for i in (0, 1, 63):
+        assert f[i] == pytest.approx(10000.0 ** (-2 * i / 128), rel=1e-15)
+
+
+def test_frequencies_scaled():
+    plain, _ = ua.rotary_frequencies(64, base=500.0)
+    lin, m = ua.rotary_frequencies(64, base=500.0, scaling="linear", factor=4.0)
+    assert m == 1.0 and torch.equal(lin, plain / 4)
+    ntk, _ = ua.rotary_frequencies(64, base=500.0, scaling="ntk", factor=4.0)
+    assert ntk[0] == 1.0 and ntk[-1] == pytest.approx(float(plain[-1]) / 4, rel=1e-12)
+    plain, _ = ua.rotary_frequencies(128)
+    turns = 4096 * plain / (2 * math.pi)
+    for kind, high, m_want in (("yarn", 32.0, 0.1 * math.log(8.0) + 1), ("bands", 4.0, 1.0)):
+        f, m = ua.rotary_frequencies(128, scaling=kind, factor=8.0, original_context=4096)
+        assert m == pytest.approx(m_want)
+        assert torch.equal(f[turns > high * 1.5], plain[turns > high * 1.5])         # fast pairs keep their angle
+        assert torch.allclose(f[turns < 0.6], plain[turns < 0.6] / 8, rtol=1e-15)    # slow ones are stretched
+        assert ((f <= plain) & (f >= plain / 8 * (1 - 1e-15))).all() and (f.diff() < 0).all()
+        same, m = ua.rotary_frequencies(128, scaling=kind, factor=1.0, original_context=4096)
+        assert m == 1.0 and torch.allclose(same, plain, rtol=1e-15)
+
+
+@pytest.mark.parametrize("bad", [dict(dim=7), dict(dim=0), dict(dim=64, factor=0.0), dict(dim=64, scaling="cubic"),
+                                 dict(dim=2, scaling="ntk", factor=2.0), dict(dim=64, base=-1.0)])
+def test_frequencies_refused(bad):
+    with pytest.raises(ValueError):
+        ua.rotary_frequencies(**bad)
+
+
+# (batch or None, tokens, heads, kv heads, dim, rotated, interleaved)
+SHAPES = [
+    (None, 1, 1, 1, 128, 128, False),
+    (None, 1, 4, 2, 128, 128, True),
+    (None, 300, 32, 8, 128, 128, False),
+    (2, 129, 7, 1, 128, 96, True),
+    (3, 65, 5, 5, 128, 64, False),
+    (None, 77, 3, 2, 80, 80, False),       # 40 pairs: whole vectors
+    (None, 77, 3, 2, 80, 24, False),       # 12 pairs: none of 8
+    (None, 33, 2, 1, 66, 66, True),        # rows that start on no 16 bytes
+    (1, 19, 2, 2, 6, 4, False),
+    (1, 19, 2, 2, 7, 2, True),
+    (None, 5, 1, 1, 512, 512, False),      # the most pairs
+    (2, 9, 3, 1, 64, 64, True),
+]
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward_and_backward(device, dtype, shape):
+    dev = _dev(device)
+    b, s, h, hk, d, rot, inter = shape
+    g = torch.Generator().manual_seed(sum(x or 0 for x in shape))
+    lead = (s,) if b is None else (b, s)
+    q, k, dq, dk = (torch.randn(*lead, n, d, generator=g).to(dtype).to(dev) for n in (h, hk, h, hk))
+    pos = torch.randint(0, 1_000_000, lead, generator=g).to(torch.int32).to(dev)
+    f, m = ua.rotary_frequencies(rot, scaling="yarn" if rot > 2 else None, factor=4.0, device=dev)
+    q.requires_grad_(), k.requires_grad_()
+    q2, k2 = ua.rotary(q, k, pos, f, interleaved=inter, magnitude=m)
+    gq, gk = torch.autograd.grad((q2, k2), (q, k), (dq, dk))
+    for x, y in ((q, q2), (k, k2)):
+        _assert_close(y.detach(), x.detach(), _exact(x.detach(), pos, f, m, inter), rot // 2, m, inter)
+    for x, y in ((dq, gq), (dk, gk)):
+        _assert_close(y, x, _exact(x, pos, f, m, inter, inverse=True), rot // 2, m, inter)
+
+
+def test_gradient_against_differences():
+    g = torch.Generator().manual_seed(5)
+    q, k = (torch.randn(4, n, 12, generator=g, dtype=torch.float64).requires_grad_() for n in (3, 1))
+    pos = torch.tensor([0, 1, 777, 123456])
+    for inter in (False, True):
+        f, m = ua.rotary_frequencies(8, scaling="yarn", factor=2.0)
+        assert torch.autograd.gradcheck(lambda a, b: ua.rotary(a, b, pos, f, interleaved=inter, magnitude=m), (q, k))
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_positions_of_any_size(device):
+    """64-bit positions, negative ones, and broadcast ones; the angle is that of 64 bits (whose own products p f are exact enough up
+    to 2^31: an error of 2^31 2^-53)."""
+    dev = _dev(device)
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(6, 2, 128, generator=g).to(dev)
+    f, _ = ua.rotary_frequencies(128, device=dev)
+    pos = torch.tensor([0, 1, -5, 524_287, 2 ** 24 + 1, 2 ** 31 - 1], device=dev)
+    want = _exact(x, pos, f)
+    for p in (pos, pos.to(torch.int32)):
+        (y,) = R.rotate((x,), p, f)
+        _assert_close(y, x, want, 64, 1.0, False)
+    xb = torch.randn(3, 6, 2, 128, generator=g).to(dev)
+    (y,) = R.rotate((xb,), pos.expand(3, 6), f)
+    _assert_close(y, xb, _exact(xb, pos.expand(3, 6), f), 64, 1.0, False)
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_views_and_out(device):
+    """Parts of a packed projection, rows that start on no 16 bytes, heads before tokens, in place, the element axis strided."""
+    dev = _dev(device)
+    g = torch.Generator().manual_seed(4)
+    f, _ = ua.rotary_frequencies(128, device=dev)
+    pos = torch.arange(50, device=dev) * 31
+    packed = torch.randn(50, 6 * 128 + 1, generator=g).to(torch.bfloat16).to(dev)
+    views = {
+        "packed": packed[:, :768].unflatten(1, (6, 128))[:, :4],
+        "odd start": packed[:, 1:].unflatten(1, (6, 128)),
+        "heads first": torch.randn(3, 50, 128, generator=g).to(torch.bfloat16).to(dev).transpose(0, 1),
+        "elements strided": torch.randn(50, 128, 3, generator=g).to(torch.bfloat16).to(dev).transpose(1, 2),
+        "every second token": torch.randn(100, 2, 128, generator=g).to(torch.bfloat16).to(dev)[::2],
+        "one head, odd stride": torch.randn(50, 1, 131, generator=g).to(torch.bfloat16).to(dev)[..., :128],
+    }
+    for name, x in views.items():
+        want = _exact(x, pos, f)
+        (y,) = R.rotate((x,), pos, f)
+        assert y.is_contiguous(), name
+        _assert_close(y, x, want, 64, 1.0, False)
+        if x.stride(-1) == 1:
+            before = packed.clone()
+            z = x.clone() if name != "packed" else x
+            src = z.clone()
+            R.rotate((z,), pos, f, out=(z,))
+            _assert_close(z, src, want, 64, 1.0, False)
+            if name == "packed":            # its neighbours stay
+                assert torch.equal(packed[:, 512:], before[:, 512:])
+    for shape in ((0, 3, 128), (4, 0, 128)):
+        e = torch.empty(*shape, device=dev, dtype=torch.bfloat16)
+        assert R.rotate((e,), pos[:shape[0]], f)[0].shape == e.shape
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_refusals(device):
+    dev = _dev(device)
+    x, f, pos = torch.randn(5, 2, 64, device=dev), ua.rotary_frequencies(64, device=dev)[0], torch.arange(5, device=dev)
+    bad = [
+        lambda: ua.rotary(x, x, pos, f.float()),                                        # angles in fp32
+        lambda: ua.rotary(x, x, pos[:4], f),                                            # a position short
+        lambda: ua.rotary(x, x, pos.float(), f),
+        lambda: ua.rotary(x, x[:4], pos, f),                                            # fewer keys than queries
+        lambda: ua.rotary(x, x, pos, ua.rotary_frequencies(66, device=dev)[0]),        # more pairs than a head has
+        lambda: R.rotate((x,), pos, f, out=(x[:4],)),
+        lambda: R.rotate((x, x, x, x), pos, f),
+        lambda: R.rotate((x[0],), pos[0], f),
+    ]
+    if dev.type == "cuda":
+        bad += [lambda: ua.rotary(x.double(), x.double(), pos, f), lambda: ua.rotary(x, x, pos.cpu(), f),
+                lambda: ua.rotary(x, x.half(), pos, f), lambda: ua.rotary(x, x, pos, f.cpu()),
+                lambda: R.rotate((torch.randn(5, 2, 1024, device=dev),), pos, ua.rotary_frequencies(1024, device=dev)[0])]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")

@@ -8,6 +8,9 @@ points), ``models`` (Llama-style model built on the kernels).
 """
 from . import patterns  # noqa: F401
 from .api import attention, prefix_lm_attention, varlen_attention  # noqa: F401
+from .ops import paged  # noqa: F401
+from .ops.paged import paged_attention  # noqa: F401
+from .ops.rotary import rotary, rotary_frequencies  # noqa: F401
 from .ops.window import sliding_window_attention  # noqa: F401
 
 __version__ = "0.1.0"

@@ -6,6 +6,7 @@ another implementation on a GPU machine.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_long, c_void_p
@@ -73,6 +74,10 @@ def _declare(lib):
         "ua_add_rmsnorm_fwd": [vp, vp, vp, vp, vp, vp, i, i, f, vp],
         "ua_rmsnorm_bwd_res": [vp, vp, vp, vp, vp, vp, vp, i, i, vp],
         "ua_rope": [vp, vp, vp, vp, vp, l, i, l, l, i, vp],
+        "ua_rotary": [c_char_p, f, vp, vp],                          # packed blocks: see ops/rotary.py, ops/paged.py
+        "ua_attn_paged": [c_char_p, f, vp, vp],
+        "ua_assign_pages": [vp, vp, i, vp, l, i, vp, i, vp, vp, i, i, vp, vp, vp, vp, vp],
+        "ua_release_pages": [vp, vp, i, vp, l, i, vp, i, vp, vp, i, vp, vp],
         "ua_swiglu_fwd": [vp, vp, l, i, vp],
         "ua_swiglu_bwd": [vp, vp, vp, l, i, vp],
         "ua_adam": [vp, vp, vp, vp, vp, l, f, f, f, f, f, i, f, vp],
@@ -144,6 +149,15 @@ def stream_of(t) -> int:
     builds a Stream object first, several microseconds a call.)"""
     import torch
     return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(t):
+    """The tensor's device as the current one, for a launch on its stream (nothing to do in a program that keeps to one)."""
+    import torch
+    return _HERE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def check(rc: int, what: str, launches: int = 1) -> None:

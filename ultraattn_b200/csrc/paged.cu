@@ -1,0 +1,265 @@
+// Bookkeeping of a paged key/value cache on the GPU: which pages a step's requests get, where its tokens go.
+//
+// A request of c tokens holds the first ceil(c / P) entries of its row of the block table. Of the c tokens after a step n are new, so
+//   before = ceil(max(c - n, 0) / P),  after = ceil(c / P),  fresh = after - before,
+// and with F the exclusive sum of `fresh` over the requests, request r's j-th fresh page is free[count - 1 - F_r - j]: the free list is a
+// stack, taken from its top in request order. Token i of request r stands at position p = c - n + i, in the slot
+// table[r][p / P] P + p % P.
+//
+// Integers and latency only (a step of 64 requests moves 2 KB): one launch, every block finds the sums for itself, and the blocks of
+// one cluster share the tokens. Nothing is written before all of them have read the counts (a cluster barrier), so that the
+// count may be updated in place.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "host_common.cuh"
+#include "ptx.cuh"
+
+namespace ua {
+
+constexpr int PAGES_THREADS = 1024;
+constexpr int PAGES_CLUSTER = 8;
+constexpr int PAGES_MAX_REQUESTS = 8192;
+
+struct PagesParams {
+  const int* context;        // [requests] tokens of a request, the new ones among them
+  const int* fresh_tokens;   // [requests] its new tokens
+  const unsigned char* ended;  // release: [requests]
+  int requests;
+  int* table;                // [requests, columns]
+  long table_stride;
+  int columns;
+  int* free_pages;
+  int pool;                  // capacity of the free list
+  const int* count_in;
+  int* count_out;
+  int page_shift;
+  int tokens;                // capacity of pos and slots
+  int* cu;
+  int* pos;
+  int* slots;
+  int* status;
+};
+
+__device__ __forceinline__ void report_pages(const PagesParams& p, int where, int extra) {
+  if (atomicCAS(p.status, 0, UA_ERR_BAD_ARG) == 0) {
+    p.status[1] = where;
+    p.status[2] = 0;
+    p.status[3] = extra;
+  }
+}
+
+// Exclusive sums over the block of two counts per thread; totals in `sum_a`, `sum_b`.
+__device__ __forceinline__ void block_scan(long& a, long& b, long& sum_a, long& sum_b, long (*warp_sums)[2]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const long a0 = a, b0 = b;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long x = __shfl_up_sync(0xFFFFFFFFu, a, d), y = __shfl_up_sync(0xFFFFFFFFu, b, d);
+    if (lane >= d) {
+      a += x;
+      b += y;
+    }
+  }
+  if (lane == 31) {
+    warp_sums[warp][0] = a;
+    warp_sums[warp][1] = b;
+  }
+  __syncthreads();
+  long before_a = 0, before_b = 0;
+  sum_a = sum_b = 0;
+  for (int w = 0; w < warps; ++w) {
+    const long x = warp_sums[w][0], y = warp_sums[w][1];
+    if (w < warp) {
+      before_a += x;
+      before_b += y;
+    }
+    sum_a += x;
+    sum_b += y;
+  }
+  a += before_a - a0;
+  b += before_b - b0;
+}
+
+// largest r with first[r] <= x (first[0] = 0, non-decreasing): the request that item x belongs to
+__device__ __forceinline__ int request_of(const int* first, int requests, int x) {
+  int lo = 0, hi = requests;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int pages_of(int tokens, int shift) {
+  return tokens <= 0 ? 0 : ((tokens - 1) >> shift) + 1;
+}
+
+__global__ void __launch_bounds__(PAGES_THREADS) assign_pages_kernel(const __grid_constant__ PagesParams p) {
+  extern __shared__ int smem[];
+  __shared__ long warp_sums[32][2];
+  int* cu = smem;                              // [requests + 1] first new token
+  int* first = cu + p.requests + 1;            // [requests + 1] first fresh page
+  int* ctx = first + p.requests + 1;           // [requests]
+  grid_wait();
+  grid_trigger();
+  const int n = p.requests, sh = p.page_shift;
+  const int per = (n + blockDim.x - 1) / blockDim.x;
+  const int r0 = min(n, static_cast<int>(threadIdx.x) * per), r1 = min(n, r0 + per);
+  const int count = *p.count_in;
+  long new_tokens = 0, new_pages = 0;
+  bool bad = false;
+  for (int r = r0; r < r1; ++r) {
+    const int c = p.context[r], k = p.fresh_tokens[r];
+    ctx[r] = c;
+    bad |= c < 0 || k < 0 || pages_of(c, sh) > p.columns;
+    const long past = static_cast<long>(c) - k;
+    new_tokens += max(k, 0);
+    new_pages += pages_of(c, sh) - pages_of(past > 0 ? static_cast<int>(past) : 0, sh);
+  }
+  long a = new_tokens, b = new_pages, all_tokens, all_pages;
+  block_scan(a, b, all_tokens, all_pages, warp_sums);
+  bad = __syncthreads_or(bad) || all_tokens > p.tokens || all_pages > count || count > p.pool;
+  if (!bad) {
+    for (int r = r0; r < r1; ++r) {
+      const int c = ctx[r], k = p.fresh_tokens[r];
+      cu[r] = static_cast<int>(a);
+      first[r] = static_cast<int>(b);
+      a += k;
+      b += pages_of(c, sh) - pages_of(c > k ? c - k : 0, sh);
+    }
+  }
+  if (threadIdx.x == 0) {
+    cu[n] = bad ? 0 : static_cast<int>(all_tokens);
+    first[n] = bad ? 0 : static_cast<int>(all_pages);
+  }
+  __syncthreads();
+  cluster_sync_all();                          // every block has read the count and the lengths
+  const int i0 = blockIdx.x * blockDim.x + threadIdx.x, step = gridDim.x * blockDim.x;
+  if (bad) {
+    if (i0 == 0) {
+      report_pages(p, all_pages > count ? 511 : all_tokens > p.tokens ? 512 : 510, static_cast<int>(min(all_pages, 0x7FFFFFFFl)));
+      *p.count_out = count;
+    }
+    for (int i = i0; i <= n; i += step) p.cu[i] = 0;
+    for (int t = i0; t < p.tokens; t += step) {
+      p.pos[t] = 0;
+      p.slots[t] = -1;
+    }
+    return;
+  }
+  if (i0 == 0) *p.count_out = count - first[n];
+  for (int i = i0; i <= n; i += step) p.cu[i] = cu[i];
+  for (int j = i0; j < first[n]; j += step) {
+    const int r = request_of(first, n, j);
+    const int past = ctx[r] - (cu[r + 1] - cu[r]);
+    p.table[r * p.table_stride + pages_of(past, sh) + (j - first[r])] = p.free_pages[count - 1 - j];
+  }
+  for (int t = i0; t < p.tokens; t += step) {
+    int at = 0, slot = -1;
+    if (t < cu[n]) {
+      const int r = request_of(cu, n, t);
+      const int past = ctx[r] - (cu[r + 1] - cu[r]);
+      at = past + (t - cu[r]);
+      if (at >= 0) {
+        const int col = at >> sh, held = pages_of(past, sh);
+        const int page = col >= held ? p.free_pages[count - 1 - (first[r] + col - held)] : p.table[r * p.table_stride + col];
+        if (page >= 0) slot = (page << sh) + (at & ((1 << sh) - 1));
+      }
+    }
+    p.pos[t] = at;
+    p.slots[t] = slot;
+  }
+}
+
+// The pages of ended requests go back onto the stack, in request order.
+__global__ void __launch_bounds__(PAGES_THREADS) release_pages_kernel(const __grid_constant__ PagesParams p) {
+  extern __shared__ int smem[];
+  __shared__ long warp_sums[32][2];
+  int* first = smem;                           // [requests + 1]
+  grid_wait();
+  grid_trigger();
+  const int n = p.requests, sh = p.page_shift;
+  const int per = (n + blockDim.x - 1) / blockDim.x;
+  const int r0 = min(n, static_cast<int>(threadIdx.x) * per), r1 = min(n, r0 + per);
+  const int count = *p.count_in;
+  auto held = [&](int r) { return p.ended[r] ? pages_of(p.context[r], sh) : 0; };
+  long a = 0, unused = 0, all, all_unused;
+  bool bad = false;
+  for (int r = r0; r < r1; ++r) {
+    const int h = held(r);
+    bad |= h > p.columns;
+    a += h;
+  }
+  block_scan(a, unused, all, all_unused, warp_sums);
+  bad = __syncthreads_or(bad) || count < 0 || all > static_cast<long>(p.pool) - count;
+  if (!bad) {
+    for (int r = r0; r < r1; ++r) {
+      first[r] = static_cast<int>(a);
+      a += held(r);
+    }
+  }
+  if (threadIdx.x == 0) first[n] = bad ? 0 : static_cast<int>(all);
+  __syncthreads();
+  cluster_sync_all();
+  const int i0 = blockIdx.x * blockDim.x + threadIdx.x, step = gridDim.x * blockDim.x;
+  if (i0 == 0) {
+    if (bad) report_pages(p, 513, static_cast<int>(min(all, 0x7FFFFFFFl)));
+    *p.count_out = count + first[n];
+  }
+  for (int j = i0; j < first[n]; j += step) {
+    const int r = request_of(first, n, j);
+    p.free_pages[count + j] = p.table[r * p.table_stride + (j - first[r])];
+  }
+}
+
+// `items`: what the launch has to go through (tokens, pages). One block up to 2048 of them: a cluster costs its barrier.
+static int launch_pages(void (*kernel)(PagesParams), const PagesParams& p, long items, int smem, cudaStream_t stream) {
+  static int smem_set[2][64] = {};
+  const int which = kernel == release_pages_kernel;
+  int dev = 0;
+  UA_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !smem_set[which][dev]) {
+    UA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * PAGES_MAX_REQUESTS + 2) * 4));
+    if (dev < 64) smem_set[which][dev] = 1;
+  }
+  const unsigned blocks = items > 2048 ? PAGES_CLUSTER : 1;
+  const unsigned threads = items > 256 || p.requests > 256 ? PAGES_THREADS : 256;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {blocks, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  UA_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+  return 0;
+}
+
+}  // namespace ua
+
+using namespace ua;
+
+extern "C" int ua_assign_pages(const int* context, const int* fresh, int requests, int* table, long table_stride, int columns,
+                               const int* free_pages, int pool, const int* count_in, int* count_out, int page_shift, int tokens, int* cu,
+                               int* pos, int* slots, int* status, cudaStream_t stream) {
+  if (requests < 0 || requests > PAGES_MAX_REQUESTS) UA_FAIL("ua_assign_pages: %d requests (%d at most)", requests, PAGES_MAX_REQUESTS);
+  PagesParams p{context, fresh, nullptr, requests, table, table_stride, columns, const_cast<int*>(free_pages), pool, count_in, count_out,
+                page_shift, tokens, cu, pos, slots, status};
+  return launch_pages(assign_pages_kernel, p, tokens, (3 * requests + 2) * 4, stream);
+}
+
+extern "C" int ua_release_pages(const unsigned char* ended, const int* context, int requests, const int* table, long table_stride,
+                                int columns, int* free_pages, int pool, const int* count_in, int* count_out, int page_shift, int* status,
+                                cudaStream_t stream) {
+  if (requests < 0 || requests > PAGES_MAX_REQUESTS) UA_FAIL("ua_release_pages: %d requests (%d at most)", requests, PAGES_MAX_REQUESTS);
+  PagesParams p{context, nullptr, ended, requests, const_cast<int*>(table), table_stride, columns, free_pages, pool, count_in, count_out,
+                page_shift, 0, nullptr, nullptr, nullptr, status};
+  return launch_pages(release_pages_kernel, p, static_cast<long>(requests) * columns, (requests + 1) * 4, stream);
+}

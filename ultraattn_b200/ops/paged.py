@@ -1,0 +1,322 @@
+"""A paged key/value cache: pages, slots, the write of new tokens and the attention that reads it.
+
+The cache of a layer is a pair of tensors ``[pages, page_size, kv_heads, 128]``. A request of ``c`` tokens holds ``ceil(c /
+page_size)`` pages, named in order by its row of a block table ``[requests, columns]`` int32. Every length lives on the GPU: a
+step never waits for the host, and can be captured into a CUDA graph and replayed for other lengths.
+
+    step = assign_pages(context, new, table, free, count, page_size=64, tokens=T, count_out=count)
+    for each layer:
+        q = rotary_append(q, k, v, step.pos, step.slots, k_cache, v_cache, inv_freq)
+        o, lse = paged_attention(q, k_cache, v_cache, table, context, step.cu_new)
+    release_pages(ended, context, table, free, count, page_size=64, count_out=count)
+
+``context[r]`` counts the tokens of request r with the ``new[r]`` of this step; the new tokens of all requests lie one after the
+other in the ``T`` rows of q, k and v. Rows behind the last of them (a batch padded to a fixed size) are given no slot, and
+nothing is written for them.
+
+What the GPU finds to be impossible (no free page left, a table too narrow, a page that the cache does not have) is reported
+like a kernel's other errors, by :func:`ultraattn_b200.ops.attention.check_status`; nothing outside the tensors is touched.
+CPU tensors run PyTorch restatements, the oracles of the kernel tests, which raise at once.
+"""
+from __future__ import annotations
+
+import math
+import struct
+from typing import NamedTuple
+
+import torch
+
+from .. import _lib
+from . import rotary as R
+from .attention import KERNEL_HEAD_DIM, status_buffer
+
+MAX_REQUESTS = 8192
+_ATTN = struct.Struct("30q")          # struct UaPagedAttn of csrc/paged_args.h
+
+
+class PagedStep(NamedTuple):
+    """What :func:`assign_pages` finds for the tokens of a step, all int32."""
+    cu_new: torch.Tensor         # [requests + 1] first new token of every request, and their number
+    pos: torch.Tensor            # [tokens] position of every new token (0 behind the last)
+    slots: torch.Tensor          # [tokens] page * page_size + offset (-1: none)
+    free_count: torch.Tensor     # [1] free pages left
+
+
+def _shift(page_size: int) -> int:
+    if page_size < 1 or page_size & (page_size - 1):
+        raise ValueError(f"the page size must be a power of two, not {page_size}")
+    return page_size.bit_length() - 1
+
+
+def _int32(device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or t.device != device:
+            raise ValueError(f"{name} must be int32 on {device}, not {t.dtype} on {t.device}")
+
+
+def _check_pool(lengths, table, free_pages, free_count, count_out) -> None:
+    dev = table.device
+    _int32(dev, block_table=table, free_pages=free_pages, free_count=free_count, **lengths)
+    n = table.shape[0]
+    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("the block table is [requests, columns] with the columns side by side")
+    for name, t in lengths.items():
+        if t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+            raise ValueError(f"{name} must hold one number for each of the {n} rows of the block table")
+    if n > MAX_REQUESTS:
+        raise ValueError(f"at most {MAX_REQUESTS} requests, not {n}")
+    if free_pages.dim() != 1 or not free_pages.is_contiguous() or free_count.numel() != 1:
+        raise ValueError("free_pages is a vector and free_count a single number")
+    if count_out is not None:
+        _int32(dev, count_out=count_out)
+        if count_out.numel() != 1:
+            raise ValueError("count_out is a single number")
+
+
+def assign_pages(context_lens, new_lens, block_table, free_pages, free_count, *, page_size: int, tokens: int,
+                 count_out=None) -> PagedStep:
+    """Pages for the new tokens of a step, and where each of them goes.
+
+    ``context_lens``, ``new_lens`` ``[requests]``: tokens of every request with the new ones, and the new ones. The first
+    ``ceil((context - new) / page_size)`` entries of a request's row in ``block_table`` are its pages so far; the entries up to
+    ``ceil(context / page_size)`` are written here, with pages from the top of the stack ``free_pages[:free_count]``, in the order of
+    the requests. ``tokens``: rows of the result, at least the sum of ``new_lens``.
+    ``free_count`` itself is not changed unless it is given as ``count_out`` too; else the pages left are in the result
+    alone. All int32. A new token in front of position 0 (``new > context``) gets no slot. If the pages do not suffice, or a row of
+    the table, or ``tokens``, nothing is assigned: every slot is -1, ``cu_new`` is 0 (and the error reported, see above)."""
+    sh = _shift(page_size)
+    _check_pool(dict(context_lens=context_lens, new_lens=new_lens), block_table, free_pages, free_count, count_out)
+    if tokens < 0:
+        raise ValueError("tokens must not be negative")
+    dev, n = block_table.device, block_table.shape[0]
+    if not block_table.is_cuda:
+        return _assign_reference(context_lens, new_lens, block_table, free_pages, free_count, page_size, tokens, count_out)
+    buf = torch.empty(n + 1 + 2 * tokens + 1, dtype=torch.int32, device=dev)
+    cu, pos, slots, left = buf.split([n + 1, tokens, tokens, 1])
+    left = left if count_out is None else count_out
+    with _lib.on_device(block_table):
+        rc = _lib.load().ua_assign_pages(context_lens.data_ptr(), new_lens.data_ptr(), n, block_table.data_ptr(), block_table.stride(0),
+                                         block_table.shape[1], free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(),
+                                         left.data_ptr(), sh, tokens, cu.data_ptr(), pos.data_ptr(), slots.data_ptr(),
+                                         status_buffer(dev).data_ptr(), _lib.stream_of(block_table))
+    _lib.check(rc, "ua_assign_pages")
+    return PagedStep(cu, pos, slots, left)
+
+
+def _assign_reference(context, new, table, free, count_in, page_size, tokens, count_out) -> PagedStep:
+    up = lambda x: -(-max(x, 0) // page_size)
+    ctx, fresh, count = context.tolist(), new.tolist(), int(count_in)
+    need = sum(up(c) - up(c - k) for c, k in zip(ctx, fresh))
+    if any(c < 0 or k < 0 or up(c) > table.shape[1] for c, k in zip(ctx, fresh)):
+        raise RuntimeError("a length is negative or needs more pages than the block table has columns")
+    if sum(fresh) > tokens or need > count or count > free.shape[0]:
+        raise RuntimeError(f"{need} pages for {sum(fresh)} tokens asked for, {count} pages and {tokens} tokens there")
+    pos, slots, cu = [], [], [0]
+    for r, (c, k) in enumerate(zip(ctx, fresh)):
+        for j in range(up(c - k), up(c)):
+            count -= 1
+            table[r, j] = free[count]
+        at = list(range(c - k, c))
+        pos += at
+        slots += [int(table[r, p // page_size]) * page_size + p % page_size if p >= 0 and table[r, p // page_size] >= 0 else -1
+                  for p in at]
+        cu.append(cu[-1] + k)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)
+    left = i32([count])
+    if count_out is not None:
+        count_out.fill_(count)
+        left = count_out
+    pad = tokens - len(pos)
+    return PagedStep(i32(cu), i32(pos + [0] * pad), i32(slots + [-1] * pad), left)
+
+
+def release_pages(ended, context_lens, block_table, free_pages, free_count, *, page_size: int, count_out=None) -> torch.Tensor:
+    """The pages of the requests for which ``ended`` (``[requests]`` bool) is set, ``ceil(context_lens / page_size)`` of each, go back
+    onto the stack ``free_pages``, in the order of the requests; the table itself is left as it is. Returns the number
+    of free pages, in ``count_out`` if given (``free_count`` itself may be). If the stack has no room for them (a page given
+    back twice), nothing changes and the error is reported."""
+    sh = _shift(page_size)
+    _check_pool(dict(context_lens=context_lens), block_table, free_pages, free_count, count_out)
+    n = block_table.shape[0]
+    if ended.dtype != torch.bool or ended.shape != (n,) or not ended.is_contiguous() or ended.device != block_table.device:
+        raise ValueError(f"ended must hold one truth value for each of the {n} rows of the block table, on its device")
+    if not block_table.is_cuda:
+        pages = [int(block_table[r, j]) for r in range(n) if ended[r] for j in range(-(-int(context_lens[r]) // page_size))]
+        count = int(free_count)
+        if count + len(pages) > free_pages.shape[0]:
+            raise RuntimeError(f"{len(pages)} pages given back to a stack of {free_pages.shape[0]} with {count} on it")
+        free_pages[count:count + len(pages)] = torch.tensor(pages, dtype=torch.int32)
+        out = count_out if count_out is not None else torch.empty_like(free_count)
+        return out.fill_(count + len(pages))
+    out = count_out if count_out is not None else torch.empty_like(free_count)
+    with _lib.on_device(block_table):
+        rc = _lib.load().ua_release_pages(ended.data_ptr(), context_lens.data_ptr(), n, block_table.data_ptr(), block_table.stride(0),
+                                          block_table.shape[1], free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(),
+                                          out.data_ptr(), sh, status_buffer(block_table.device).data_ptr(), _lib.stream_of(block_table))
+    _lib.check(rc, "ua_release_pages")
+    return out
+
+
+def _check_cache(k_cache, v_cache) -> int:
+    """The shift of a cache's page size."""
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype or k_cache.device != v_cache.device:
+        raise ValueError("k_cache and v_cache are [pages, page_size, kv_heads, dim], alike")
+    if any(c.shape[-1] > 1 and c.stride(-1) != 1 for c in (k_cache, v_cache)):
+        raise ValueError("the elements of a head of the cache must be side by side")
+    return _shift(k_cache.shape[1])
+
+
+def rotary_append(q, k, v, pos, slots, k_cache, v_cache, inv_freq=None, *, interleaved: bool = False, magnitude: float = 1.0,
+                  q_out=None) -> torch.Tensor:
+    """Queries turned by their positions, and keys, turned, and values written into the cache, in one launch.
+
+    ``q [tokens, heads, dim]``, ``k``, ``v [tokens, kv_heads, dim]`` (views of a packed projection are fine), ``pos`` and
+    ``slots`` ``[tokens]`` int32 from :func:`assign_pages`; the caches as in :func:`paged_attention` (any head dim; bf16, fp16 or
+    fp32). A token whose slot is negative is not written to the cache. ``inv_freq``, ``interleaved``, ``magnitude`` as in
+    :func:`ultraattn_b200.rotary`; without ``inv_freq`` nothing is turned. Returns the queries, in ``q_out`` if given (``q``
+    itself: in place). Slots must differ: of two tokens with the same slot either may end up in it."""
+    sh = _check_cache(k_cache, v_cache)
+    T, hk, dim = k.shape if k.dim() == 3 else (-1, -1, -1)
+    if q.dim() != 3 or k.shape != v.shape or q.shape[0] != T or q.shape[2] != dim or tuple(k_cache.shape[2:]) != (hk, dim):
+        raise ValueError("q, k and v are [tokens, heads, dim] with the cache's heads and head dim")
+    if any(t.dtype != k_cache.dtype or t.device != k_cache.device for t in (q, k, v)):
+        raise ValueError("q, k, v and the cache have one type and device")
+    _int32(q.device, slots=slots)
+    if slots.shape != (T,) or (T > 1 and slots.stride(0) != 1):
+        raise ValueError("slots must hold one number for each token")
+    if inv_freq is not None:
+        _check_angles_append(q, pos, inv_freq)
+    if q_out is not None and (q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != q.device or
+                              (dim > 1 and q_out.stride(-1) != 1)):
+        raise ValueError("q_out must match q")
+    n_slots = k_cache.shape[0] << sh
+    if not q.is_cuda:
+        turn = (lambda x: R.rotate_reference(x, pos, inv_freq, interleaved, magnitude)) if inv_freq is not None else (lambda x: x)
+        if T and int(slots.max()) >= n_slots:
+            raise RuntimeError(f"slot {int(slots.max())} of a cache of {n_slots}")
+        there = slots >= 0
+        page, off = slots[there].long() >> sh, slots[there].long() & ((1 << sh) - 1)
+        k_cache[page, off] = turn(k)[there]
+        v_cache[page, off] = v[there]
+        return turn(q).clone() if q_out is None else q_out.copy_(turn(q))
+    R._check_kernel(q, k, v, k_cache, pairs=0 if inv_freq is None else inv_freq.shape[0])
+    q, k, v = (R._with_last(t) for t in (q, k, v))
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+    if T:
+        turned = inv_freq is not None
+        R.launch([R.part(q, out, turned), R.part(k, k_cache, turned, True), R.part(v, v_cache, False, True)], q, pos,
+                 inv_freq.contiguous() if turned else None, interleaved, magnitude, slots=slots, page_shift=sh, n_slots=n_slots)
+    return out
+
+
+def _check_angles_append(q, pos, inv_freq) -> None:
+    R._check_angles(q, pos, inv_freq)
+
+
+def paged_attention_reference(q, k_cache, v_cache, block_table, context_lens, cu_new, softmax_scale=None, window_size=(-1, 0),
+                              sink_tokens: int = 0, out=None):
+    """PyTorch restatement of :func:`paged_attention` (fp32; fp64 for fp64 tensors), request by request."""
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    T, H, D = q.shape
+    page, hk = k_cache.shape[1:3]
+    scale = D ** -0.5 if softmax_scale is None else softmax_scale
+    o, lse = out if out is not None else (torch.zeros_like(q), torch.full((H, T), float("-inf"), dtype=torch.float32, device=q.device))
+    cu, left = cu_new.tolist(), window_size[0]
+    for r, c in enumerate(context_lens.tolist()):
+        a, b = cu[r], cu[r + 1]
+        if b <= a:
+            continue
+        n_pages = -(-c // page)
+        pages = block_table[r, :n_pages].long()
+        if n_pages > block_table.shape[1]:
+            raise RuntimeError(f"request {r}: {n_pages} pages, {block_table.shape[1]} columns in the block table")
+        key = torch.arange(c, device=q.device)
+        p = torch.arange(c - (b - a), c, device=q.device)[:, None]
+        seen = key <= p
+        if left >= 0:
+            seen &= (key >= p - left) | (key < sink_tokens)
+        used = seen.any(0)
+        bad = used & ((pages[key // page] < 0) | (pages[key // page] >= k_cache.shape[0]))
+        if bad.any():
+            raise RuntimeError(f"request {r}: a page that the cache does not have")
+        # (what no query sees, pages given back among them, may hold anything)
+        kk, vv = (torch.where(used[:, None, None], x[pages[key // page].clamp(0, k_cache.shape[0] - 1), key % page], 0).to(wide)
+                  for x in (k_cache, v_cache))
+        kk, vv = (x.repeat_interleave(H // hk, 1) for x in (kk, vv))
+        s = torch.einsum("qhd,khd->hqk", q[a:b].to(wide), kk) * scale
+        s = s.masked_fill(~seen, float("-inf"))
+        z = torch.logsumexp(s, -1) if c else s.new_full((H, b - a), float("-inf"))
+        w = torch.exp(s - torch.where(torch.isfinite(z), z, torch.zeros_like(z))[..., None])
+        o[a:b] = torch.einsum("hqk,khd->qhd", w, vv).to(o.dtype)
+        lse[:, a:b] = z
+    return o, lse
+
+
+def paged_attention(q, k_cache, v_cache, block_table, context_lens, cu_new, *, most_new: int | None = None,
+                    softmax_scale: float | None = None, window_size=(-1, 0), sink_tokens: int = 0, out=None):
+    """``(o, lse)``: causal attention of the new tokens of a ragged batch over a paged cache.
+
+    ``q [tokens, heads, 128]`` bf16: the new tokens of request r are the rows ``cu_new[r] .. cu_new[r + 1]``, the last
+    of its ``context_lens[r]`` tokens, whose keys and values lie in the pages that row r of ``block_table`` names. Query i of n
+    sees the keys up to its own position ``p = context - n + i``; with ``window_size = (left, 0)`` those from ``p - left`` on, and
+    the first ``sink_tokens``. ``k_cache``, ``v_cache`` ``[pages, page_size, kv_heads, 128]`` bf16 with any strides that are multiples of
+    8 elements; ``heads`` a multiple of ``kv_heads``. Every length from one token on runs in the same call: decoding requests,
+    chunks of prompts and whole prompts. ``most_new``: a bound for the new tokens of a request that the host knows
+    (default: ``tokens``).
+
+    ``o [tokens, heads, 128]`` bf16 and ``lse [heads, tokens]`` fp32, in ``out = (o, lse)`` if given; rows behind the
+    last request are not written. A query that sees no key (``context < n``) gives 0 and -inf. What the cache holds in places that no
+    query of a request sees (behind its last token, in pages before its window) does not matter, NaN included. Forward only."""
+    if q.dim() != 3 or k_cache.dim() != 4 or q.shape[2] != k_cache.shape[3]:
+        raise ValueError("q is [tokens, heads, dim], the caches [pages, page_size, kv_heads, dim]")
+    sh = _check_cache(k_cache, v_cache)
+    T, H, D = q.shape
+    pages, page_size, hk = k_cache.shape[:3]
+    n = block_table.shape[0]
+    _int32(q.device, block_table=block_table, context_lens=context_lens, cu_new=cu_new)
+    if block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("the block table is [requests, columns] with the columns side by side")
+    if context_lens.shape != (n,) or cu_new.shape != (n + 1,) or (n > 1 and context_lens.stride(0) != 1) or (n and cu_new.stride(0) != 1):
+        raise ValueError(f"context_lens and cu_new hold {n} and {n + 1} numbers for {n} rows of the block table")
+    if hk == 0 or H % hk != 0:
+        raise ValueError(f"{H} query heads do not divide into {hk} key/value heads")
+    if q.dtype != k_cache.dtype or q.device != k_cache.device:
+        raise ValueError("q and the cache have one type and device")
+    left, right = (int(x) for x in window_size)
+    if right not in (0, -1):
+        raise ValueError("new tokens see no later ones: window_size is (left, 0)")
+    if sink_tokens < 0 or (sink_tokens and left < 0):
+        raise ValueError("sink_tokens goes with a window")
+    if out is not None:
+        o, lse = out
+        if o.shape != q.shape or o.dtype != q.dtype or lse.shape != (H, T) or lse.dtype != torch.float32 or o.device != q.device or lse.device != q.device:
+            raise ValueError("out is (o like q, lse [heads, tokens] fp32)")
+    most_new = T if most_new is None else min(int(most_new), T)
+    if most_new < 0:
+        raise ValueError("most_new must not be negative")
+    if not q.is_cuda:
+        return paged_attention_reference(q, k_cache, v_cache, block_table, context_lens, cu_new, softmax_scale, (left, 0), sink_tokens, out)
+    if D != KERNEL_HEAD_DIM or q.dtype != torch.bfloat16:
+        raise ValueError(f"the kernel takes bf16 heads of {KERNEL_HEAD_DIM} elements, not {q.dtype} of {D}")
+    if page_size < 16:
+        raise ValueError(f"the kernel reads pages of 16 tokens or more, not {page_size}")
+    if n > MAX_REQUESTS:
+        raise ValueError(f"at most {MAX_REQUESTS} requests, not {n}")
+    q = q if q.stride(2) == 1 and q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0 and q.data_ptr() % 16 == 0 else q.clone(
+        memory_format=torch.contiguous_format)
+    for c in (k_cache, v_cache):
+        if any(s % 8 for s in c.stride()[:3]) or c.data_ptr() % 16:
+            raise ValueError("the strides of a cache are multiples of 8 elements and it starts on 16 bytes")
+    if out is None:
+        o, lse = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(H, T, dtype=torch.float32, device=q.device)
+    elif o.stride(2) != 1 or o.stride(0) % 8 or o.stride(1) % 8 or o.data_ptr() % 16 or (T > 1 and lse.stride(1) != 1):
+        raise ValueError("the rows of o start on 16 bytes, the tokens of lse lie side by side")
+    scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
+    block = _ATTN.pack(q.data_ptr(), T, H, q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), pages, hk,
+                       *k_cache.stride()[:3], *v_cache.stride()[:3], sh, block_table.data_ptr(), block_table.stride(0),
+                       block_table.shape[1], context_lens.data_ptr(), cu_new.data_ptr(), n, most_new, left, int(sink_tokens),
+                       o.data_ptr(), o.stride(0), o.stride(1), lse.data_ptr(), lse.stride(0))
+    with _lib.on_device(q):
+        rc = _lib.load().ua_attn_paged(block, scale, status_buffer(q.device).data_ptr(), _lib.stream_of(q))
+    _lib.check(rc, "ua_attn_paged")
+    return o, lse

@@ -1,0 +1,198 @@
+"""Rotary position embedding in its general form: both layouts of the pairs, part of the head, frequencies
+scaled for long contexts, any position; forward and backward.
+
+A head's first ``2 * len(inv_freq)`` elements are turned pair by pair: the pair ``f`` at position ``p`` by the angle
+``p * inv_freq[f]``, and scaled by ``magnitude``. Pairs are ``(i, i + half)``, or ``(2 i, 2 i + 1)`` with ``interleaved``; the
+other elements are copied. The kernel finds the angles itself, as fractions of a turn in 64-bit integers: positions
+of any size are exact and there is no table (:func:`ultraattn_b200.ops.elementwise.rope` reads one whose angles are products in
+fp32, 0.03 rad off at position 500k).
+
+:func:`rotary_frequencies` gives ``(inv_freq, magnitude)`` of the usual ways to stretch a context. On CPU tensors the same
+functions run a PyTorch restatement with 64-bit angles, the oracle of the kernel tests.
+"""
+from __future__ import annotations
+
+import math
+import struct
+
+import torch
+
+from .. import _lib
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_MAX_PAIRS = 256
+_ROTARY = struct.Struct("33q16q")      # struct UaRotary of csrc/paged_args.h
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: str | None = None, factor: float = 1.0,
+                       original_context: int = 8192, low: float = 1.0, high: float | None = None, device=None):
+    """``(inv_freq, magnitude)``: the angle per position of each of ``dim / 2`` pairs (fp64, on ``device``) and
+    the factor of the rotated vector.
+
+    ``scaling`` stretches the context that the angles were trained on (``original_context`` tokens) by ``factor``:
+
+    * ``None``       ``base ** (-2 i / dim)``;
+    * ``"linear"``   every angle divided by ``factor`` (position interpolation);
+    * ``"ntk"``      the base times ``factor ** (dim / (dim - 2))``: the slowest pair is stretched by ``factor``, the
+      fastest not at all;
+    * ``"yarn"``     pairs that turn more than ``high`` (32) times within the original context keep their angle, those that
+      turn less than ``low`` (1) times are divided, a linear ramp over the pair's index in between; magnitude
+      ``0.1 ln(factor) + 1``;
+    * ``"bands"``    the same by the number of turns itself, with ``high`` = 4 and magnitude 1.
+    """
+    if dim < 2 or dim % 2 != 0:
+        raise ValueError(f"the rotated part of a head has an even number of elements, not {dim}")
+    if factor <= 0 or base <= 0 or original_context <= 0:
+        raise ValueError("base, factor and original_context must be positive")
+    i = torch.arange(0, dim, 2, dtype=torch.float64)
+    f = base ** (-i / dim)
+    magnitude = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "ntk":
+        if dim < 4:
+            raise ValueError("scaling='ntk' needs at least two pairs")
+        f = (base * factor ** (dim / (dim - 2))) ** (-i / dim)
+    elif scaling == "yarn":
+        high = 32.0 if high is None else high
+        pair_at = lambda turns: dim * math.log(original_context / (turns * 2 * math.pi)) / (2 * math.log(base))
+        first, last = max(math.floor(pair_at(high)), 0), min(math.ceil(pair_at(low)), dim - 1)
+        ramp = ((i / 2 - first) / max(last - first, 1e-3)).clamp(0, 1)
+        f = f / factor * ramp + f * (1 - ramp)
+        magnitude = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    elif scaling == "bands":
+        high = 4.0 if high is None else high
+        keep = ((original_context * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        f = f * keep + f / factor * (1 - keep)
+    elif scaling is not None:
+        raise ValueError(f"unknown scaling {scaling!r}: None, 'linear', 'ntk', 'yarn' or 'bands'")
+    return f.to(device) if device is not None else f, magnitude
+
+
+def rotate_reference(x, pos, inv_freq, interleaved=False, magnitude=1.0, inverse=False):
+    """``x [..., heads, dim]`` at ``pos [...]``: angles in 64 bits, the rotation in 32 (64 for fp64 tensors)."""
+    ang = pos.double()[..., None] * inv_freq.double()
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    cos, sin = (t.to(wide)[..., None, :] for t in (ang.cos() * magnitude, ang.sin() * (-magnitude if inverse else magnitude)))
+    half, xf = inv_freq.shape[0], x.to(wide)
+    a, b = (xf[..., 0:2 * half:2], xf[..., 1:2 * half:2]) if interleaved else (xf[..., :half], xf[..., half:2 * half])
+    ra, rb = a * cos - b * sin, b * cos + a * sin
+    turned = torch.stack([ra, rb], -1).flatten(-2) if interleaved else torch.cat([ra, rb], -1)
+    return torch.cat([turned, xf[..., 2 * half:]], -1).to(x.dtype)
+
+
+def _check_angles(x, pos, inv_freq):
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1:
+        raise ValueError("inv_freq must be a vector of fp64 angles (rotary_frequencies)")
+    if 2 * inv_freq.shape[0] > x.shape[-1]:
+        raise ValueError(f"{inv_freq.shape[0]} pairs do not fit heads of {x.shape[-1]} elements")
+    if pos.dtype not in (torch.int32, torch.int64):
+        raise ValueError("positions must be int32 or int64")
+    if tuple(pos.shape) != tuple(x.shape[:-2]):
+        raise ValueError(f"positions {tuple(pos.shape)} for tokens {tuple(x.shape[:-2])}")
+    if pos.device != x.device or inv_freq.device != x.device:
+        raise ValueError("positions and inv_freq must be on the tensors' device")
+
+
+def _check_kernel(*tensors, pairs: int):
+    t0 = tensors[0]
+    if t0.dtype not in _DTYPES:
+        raise ValueError(f"the rotary kernel takes bf16, fp16 and fp32, not {t0.dtype}")
+    for t in tensors:
+        if t.dtype != t0.dtype or t.device != t0.device or t.shape[-1] != t0.shape[-1]:
+            raise ValueError("all tensors of a rotary call have one type, head dim and device")
+    if pairs > _MAX_PAIRS:
+        raise ValueError(f"at most {_MAX_PAIRS} pairs of a head are rotated, not {pairs}")
+
+
+def _with_last(t):
+    """``t`` with consecutive elements of a head side by side."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _bshd(t):
+    """(batch, token, head) strides of ``[tokens, heads, dim]`` or ``[batch, tokens, heads, dim]``."""
+    st = t.stride()
+    return (0, *st[:2]) if t.dim() == 3 else st[:3]
+
+
+def part(src, dst, rotate=True, paged=False) -> tuple:
+    """One tensor of a launch (struct UaRotPart)."""
+    d = dst.stride()[:3] if paged else _bshd(dst)
+    return (src.data_ptr(), dst.data_ptr(), src.shape[-2], int(rotate), int(paged), *_bshd(src), *d)
+
+
+def launch(parts, like, pos, inv_freq, interleaved, magnitude, inverse=False, slots=None, page_shift=0, n_slots=0) -> None:
+    """``ua_rotary`` over the tokens of ``like``."""
+    from .attention import status_buffer
+    batch, tokens = (1, like.shape[0]) if like.dim() == 3 else like.shape[:2]
+    ps = (0, pos.stride(0)) if pos.dim() == 1 else pos.stride()
+    pairs = 0 if inv_freq is None else inv_freq.shape[0]
+    flat = [x for p in parts for x in p] + [0] * (11 * (3 - len(parts)))
+    block = _ROTARY.pack(*flat, len(parts), batch, tokens, pos.data_ptr(), int(pos.dtype == torch.int64), *ps,
+                         0 if slots is None else slots.data_ptr(), page_shift, n_slots,
+                         0 if inv_freq is None else inv_freq.data_ptr(), pairs, like.shape[-1], int(interleaved), int(inverse),
+                         _DTYPES[like.dtype])
+    with _lib.on_device(like):
+        rc = _lib.load().ua_rotary(block, float(magnitude), status_buffer(like.device).data_ptr(), _lib.stream_of(like))
+    _lib.check(rc, "ua_rotary")
+
+
+def rotate(tensors, pos, inv_freq, *, interleaved: bool = False, magnitude: float = 1.0, inverse: bool = False, out=None):
+    """The rotation of each of up to three ``tensors`` (``[tokens, heads, dim]`` with ``pos [tokens]``, or ``[batch, tokens,
+    heads, dim]`` with ``pos [batch, tokens]``) in one launch, without autograd; ``inverse``: its transpose. ``out``: tensors
+    of the same shapes to write (the inputs themselves: in place)."""
+    tensors = tuple(tensors)
+    if not 1 <= len(tensors) <= 3:
+        raise ValueError("one to three tensors are rotated in a call")
+    for t in tensors:
+        if t.dim() not in (3, 4):
+            raise ValueError("tensors to rotate are [tokens, heads, dim] or [batch, tokens, heads, dim]")
+        _check_angles(t, pos, inv_freq)
+    if out is not None:
+        out = tuple(out)
+        if len(out) != len(tensors) or any(o.shape != t.shape or o.dtype != t.dtype or o.device != t.device for o, t in zip(out, tensors)):
+            raise ValueError("out must match the tensors")
+    if not tensors[0].is_cuda:
+        res = tuple(rotate_reference(t, pos, inv_freq, interleaved, magnitude, inverse) for t in tensors)
+        if out is None:
+            return res
+        for o, r in zip(out, res):
+            o.copy_(r)
+        return out
+    _check_kernel(*tensors, pairs=inv_freq.shape[0])
+    src = tuple(_with_last(t) for t in tensors)
+    dst = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors) if out is None else out
+    if any(o.stride(-1) != 1 and o.shape[-1] > 1 for o in dst):
+        raise ValueError("the elements of a head of out must be side by side")
+    if tensors[0].numel() or any(t.numel() for t in tensors):
+        launch([part(s, d) for s, d in zip(src, dst)], tensors[0], pos, inv_freq.contiguous(), interleaved, magnitude, inverse)
+    return dst
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, pos, inv_freq, interleaved, magnitude):
+        ctx.save_for_backward(pos, inv_freq)
+        ctx.form = (interleaved, magnitude)
+        return rotate((q, k), pos, inv_freq, interleaved=interleaved, magnitude=magnitude)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        pos, inv_freq = ctx.saved_tensors
+        interleaved, magnitude = ctx.form
+        dq, dk = rotate((dq, dk), pos, inv_freq, interleaved=interleaved, magnitude=magnitude, inverse=True)
+        return dq, dk, None, None, None, None
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False,
+           magnitude: float = 1.0):
+    """Queries and keys turned by their positions, with autograd: ``(q', k')``.
+
+    ``q [tokens, heads, dim]`` and ``k [tokens, kv_heads, dim]`` (any strides with the elements of a head side by side, views of a
+    packed projection among them) with ``pos [tokens]``, or all of them with a leading batch axis; ``pos`` int32 or int64;
+    ``inv_freq``, ``magnitude`` from :func:`rotary_frequencies`. bf16, fp16 or fp32 on CUDA, any float type on CPU; results and
+    gradients are contiguous and of the inputs' type, computed in fp32."""
+    if q.dim() != k.dim() or q.shape[:-2] != k.shape[:-2]:
+        raise ValueError(f"queries {tuple(q.shape)} and keys {tuple(k.shape)} have different tokens")
+    return _Rotary.apply(q, k, pos, inv_freq, bool(interleaved), float(magnitude))
