@@ -75,7 +75,8 @@ def _declare(lib):
         "ua_rmsnorm_bwd_res": [vp, vp, vp, vp, vp, vp, vp, i, i, vp],
         "ua_rope": [vp, vp, vp, vp, vp, l, i, l, l, i, vp],
         "ua_rotary": [c_char_p, f, vp, vp],                          # packed blocks: see ops/rotary.py, ops/paged.py
-        "ua_attn_paged": [c_char_p, f, vp, vp],
+        "ua_attn_paged": [c_char_p, f, vp, vp, vp],
+        "ua_attn_paged_workspace": [c_char_p],
         "ua_assign_pages": [vp, vp, i, vp, l, i, vp, i, vp, vp, i, i, vp, vp, vp, vp, vp],
         "ua_release_pages": [vp, vp, i, vp, l, i, vp, i, vp, vp, i, vp, vp],
         "ua_swiglu_fwd": [vp, vp, l, i, vp],
@@ -91,6 +92,8 @@ def _declare(lib):
             fn = getattr(lib, name)
             fn.restype = c_int
             fn.argtypes = args
+    if hasattr(lib, "ua_attn_paged_workspace"):
+        lib.ua_attn_paged_workspace.restype = c_long
     return lib
 
 

@@ -1,87 +1,1062 @@
-// Attention of a ragged batch of new tokens over a paged key/value cache.
+// Attention of a ragged batch of new tokens over a paged key/value cache: TMA-fed tcgen05.mma, S / P and O in tensor memory.
 //
 // Query i of request r (n new tokens, c keys in all) stands at position p = c - n + i and sees the keys 0 .. p, with a window those
 // from p - left on and the first `sink`:  o = softmax(scale q K^T) V,  lse = log sum exp(scale q k).
 //
-// The plain kernel: a warp for each query head of a token, four head-dim elements per lane, running maximum and sum.
+// One pass over the keys in tiles of 128 with the running maximum and sum of a row in registers, as in attn_fwd_sm100.cu, whose
+// roles and tensor-memory layouts these are (12 warps: 8 softmax, TMA, two MMA issuers):
+//   FEW    requests of up to 128 rows (decoding, short chunks): both sub-tiles hold the same rows and take the key tiles in turn
+//   !FEW   the others: items of 256 rows, 128 in each sub-tile
+// A row is a query head of a token: row x of an item is token x / G', head x % G' of the group of G heads that shares a key/value head,
+// G' the next power of two (rows of heads behind G are computed and not stored), so that a key is read once for its group.
+//
+// What is different: the work is found on the GPU. The lengths are in device memory, and every CTA (one per SM) sums the requests' key
+// tiles up, takes an equal share of the line of all (request, key/value head, row tile) items and walks it: no table to build, no host,
+// no waiting for the longest request. An item that a border cuts leaves fp32 parts behind, at most two per CTA, which
+// combine_parts merges in the order of the keys. Keys come page by page (a TMA box is a page, or 128 tokens of a larger one).
 #include "host_common.cuh"
 #include "paged_args.h"
 #include "ptx.cuh"
 
 namespace ua {
 
-__device__ __forceinline__ float4 bf16x4(const __nv_bfloat16* p) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
-                     __uint_as_float(u.y & 0xFFFF0000u));
+constexpr int PD = 128;                       // head dim
+constexpr int PT = 128;                       // tile edge
+constexpr int PA_SOFTMAX_WARPS = 8;
+constexpr int PA_TMA_WARP = 8;
+constexpr int PA_QK_WARP = 9;                 // issues S = Q K^T; owns the TMEM allocation
+constexpr int PA_PV_WARP = 10;                // issues O += P V
+constexpr int PA_THREADS = 384;
+constexpr int PA_REGS_LAUNCH = 168, PA_REGS_LOAD = 72, PA_REGS_SOFTMAX = 216;
+static_assert(2 * PA_REGS_SOFTMAX + PA_REGS_LOAD <= 3 * PA_REGS_LAUNCH, "setmaxnreg may only redistribute the launch-time pool");
+constexpr int PA_TILE_BYTES = PT * PD * 2;    // [2 d-halves][128 rows][128 B]
+// What the start and the end of an item cost, in key tiles of its form (a share's border is not put into them).
+template <bool FEW> constexpr int PA_ITEM_TILES = FEW ? 2 : 3;
+constexpr int PA_MIN_SHARE = 3;               // key tiles of a CTA at least, besides
+
+struct PagedParams {
+  CUtensorMap tm_q, tm_k, tm_v;
+  const int* table;
+  long table_stride;
+  int columns;
+  int pages;
+  const int* context;
+  const int* cu_new;
+  int requests;
+  int tokens;
+  int heads, kv_heads, group;
+  int pack_shift;            // log2 of the rows of a token
+  int page_shift;
+  int left, sink;            // left < 0: no window
+  int few_rows;              // requests of up to so many rows belong to the FEW form
+  int other_form;            // the launch is one of two; else it has to take every request
+  float scale_log2;
+  __nv_bfloat16* o;
+  long o_token, o_head;
+  float* lse;
+  long lse_head;
+  float* part_o;             // [2 * CTAs][part_rows][128]
+  float* part_lse;           // [2 * CTAs][part_rows]
+  int* part_desc;            // [CTAs][PA_DESC]
+  int part_rows;
+  int* status;
+};
+// What a CTA left behind: 0: the part of an item that begins here and goes on in the next CTA (1 / 0), its first token, first head and
+// rows (1 - 3); 4: the part of one that began before (0 none, 1 goes on, 2 ends)
+constexpr int PA_DESC = 8;
+
+// A piece of an item: the key tiles that this CTA takes of it.
+struct PagedItem {
+  int exists, total;
+  int q_row;                 // row of q of the request's first new token
+  int tok0, rows;            // first token of the tile in the request, rows of the tile
+  int kv_head;
+  int past;                  // position of the request's first new token
+  int request;
+  int slot;                  // part to write, -1: the result
+  int first[2], end[2];      // key tiles: of the sinks, of the band
+  int lo[2], hi[2];          // keys that some row sees, of each
+};
+
+template <bool FEW>
+struct __align__(1024) PagedSmem {
+  static constexpr int STAGES = FEW ? 3 : 2;
+  uint8_t q[FEW ? 1 : 2][PA_TILE_BYTES];
+  uint8_t k[STAGES][PA_TILE_BYTES];
+  uint8_t v[STAGES][PA_TILE_BYTES];
+  uint8_t o_stage[FEW ? 1 : PA_SOFTMAX_WARPS][FEW ? 16 : 4096];
+  uint64_t q_full;
+  uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
+  uint64_t s_full[2], p_full[2];
+  uint64_t q_empty;
+  uint64_t s_free;           // the scores have been read into registers
+  uint64_t pv_done[2];
+  uint64_t item_full[2], item_empty[2];
+  uint64_t stat_full, merged;
+  PagedItem item[2];
+  float2 stat[FEW ? PT : 1];
+  long sums[12];
+  long start_x;              // where in its request the CTA's share begins
+  int start_r;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(PagedSmem<false>) + 1024 <= 232448 && sizeof(PagedSmem<true>) + 1024 <= 232448, "a CTA may use 227 KB");
+
+__device__ __forceinline__ void paged_error(int* status, int where, int extra) {
+  if (atomicCAS(status, 0, UA_ERR_BAD_ARG) == 0) {
+    status[1] = where;
+    status[2] = static_cast<int>(blockIdx.x);
+    status[3] = extra;
+  }
 }
 
-__global__ void __launch_bounds__(256) attn_paged_plain_kernel(const __grid_constant__ UaPagedAttn a, float scale, int* status) {
+// ---- the line of all items ------------------------------------------------------------------------------------------------
+// Sum over i = 1 .. m of ceil((a + i) / 2^k)
+__device__ __forceinline__ long ceil_sum(long a, long m, int k) {
+  auto upto = [&](long n) {                    // sum of ceil(i / 2^k), i = 1 .. n
+    const long q = n >> k, r = n & ((1l << k) - 1);
+    return ((q * (q + 1) / 2) << k) + r * (q + 1);
+  };
+  return upto(a + m) - upto(a);
+}
+
+// A request as this form sees it.
+template <bool FEW>
+struct PagedRequest {
+  int n, past, q_row, row_tiles;     // row_tiles 0: nothing to do
+  // key tiles of the row tile that begins with token t0: [first, end) of sinks and band, and the keys of each that some row sees
+  __device__ __forceinline__ int tiles(const PagedParams& p, int tile, PagedItem& it) const {
+    const int tpt = (FEW ? PT : 2 * PT) >> p.pack_shift;
+    it.tok0 = tile * tpt;
+    const int toks = min(tpt, n - it.tok0);
+    it.rows = toks << p.pack_shift;
+    const int last = past + it.tok0 + toks - 1;                       // position of the last row; < 0: sees nothing
+    it.lo[0] = it.hi[0] = it.first[0] = it.end[0] = 0;
+    it.hi[1] = max(0, last + 1);
+    it.lo[1] = p.left < 0 ? 0 : max(0, past + it.tok0 - p.left);
+    if (p.left >= 0) {
+      it.hi[0] = max(0, min(p.sink, last - p.left));
+      it.end[0] = (it.hi[0] + PT - 1) / PT;
+    }
+    it.first[1] = it.lo[1] / PT;
+    it.end[1] = (it.hi[1] + PT - 1) / PT;
+    if (it.hi[1] == 0) it.first[1] = it.lo[1] = 0;
+    return it.end[0] + it.end[1] - it.first[1];
+  }
+  // weight of the first m row tiles of a key/value head: their key tiles and PA_ITEM_TILES each (a window: an upper bound that is
+  // the same for all; what a share's border means is settled per item, with its own number of tiles)
+  __device__ __forceinline__ long weight(const PagedParams& p, int m) const {
+    if (FEW) {
+      PagedItem it;
+      return m == 0 ? 0 : PA_ITEM_TILES<FEW> + tiles(p, 0, it);
+    }
+    const int tpt = 2 * PT >> p.pack_shift;
+    long w = static_cast<long>(m) * PA_ITEM_TILES<FEW>;
+    if (p.left >= 0) {
+      const int most = (max(past + n, 0) + PT - 1) / PT;
+      return w + static_cast<long>(m) * min(most, (p.left + tpt) / PT + 2 + (p.sink + PT - 1) / PT);
+    }
+    const int full = min(m, n / tpt);          // tiles whose rows are all there
+    if (full < m) w += (max(past + n, 0) + PT - 1) / PT;
+    if (past < 0) {                            // (more new tokens than the request has)
+      for (int i = 0; i < full; ++i) w += max(0, past + (i + 1) * tpt + PT - 1) / PT;
+    } else if (tpt < PT) {                     // sum of ceil((past + i tpt) / 128): tpt divides 128 ...
+      w += ceil_sum((past + tpt - 1) / tpt, full, p.pack_shift - 1);
+    } else {                                   // ... or is 128 or 256
+      w += static_cast<long>(full) * ((past + PT - 1) / PT) + (tpt / PT) * (static_cast<long>(full) * (full + 1) / 2);
+    }
+    return w;
+  }
+};
+
+template <bool FEW>
+__device__ __forceinline__ PagedRequest<FEW> paged_request(const PagedParams& p, int r, bool report) {
+  PagedRequest<FEW> q;
+  const int first = p.cu_new[r], next = p.cu_new[r + 1];
+  const int c = max(p.context[r], 0);
+  q.q_row = first;
+  q.n = next - first;
+  q.past = c - q.n;
+  const bool bad = first < 0 || next > p.tokens || q.n < 0;
+  const long rows = bad ? 0 : static_cast<long>(q.n) << p.pack_shift;
+  const bool mine = FEW ? rows <= p.few_rows : rows > p.few_rows;
+  if (report && (bad || (!mine && !p.other_form && rows > 0))) paged_error(p.status, bad ? 521 : 522, r);
+  q.row_tiles = bad || !mine ? 0 : static_cast<int>((rows + (FEW ? PT : 2 * PT) - 1) / (FEW ? PT : 2 * PT));
+  return q;
+}
+
+// This CTA's share [x0, x1) of the line, walked item by item.
+template <bool FEW>
+struct PagedWalk {
+  long x0, x1;               // the share
+  long s;                    // where the next item begins
+  int r, head, tile;
+  PagedRequest<FEW> q;
+
+  __device__ __forceinline__ void enter(const PagedParams& p) {
+    while (r < p.requests) {
+      q = paged_request<FEW>(p, r, false);
+      if (q.row_tiles > 0) return;
+      ++r;
+    }
+  }
+  __device__ __forceinline__ void begin(const PagedParams& p, int r0, long in_request, long a, long b) {
+    x0 = a;
+    x1 = b;
+    r = r0;
+    enter(p);
+    const long per_head = q.weight(p, q.row_tiles);
+    head = static_cast<int>(in_request / per_head);
+    const long y = in_request - head * per_head;
+    int lo = 0, hi = q.row_tiles;             // last tile whose items begin at y or before
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (q.weight(p, mid) <= y) lo = mid;
+      else hi = mid;
+    }
+    tile = lo;
+    s = a - y + q.weight(p, lo);
+  }
+  // the next piece of this share; false: there is none. `part`: 0 whole item, 1 its beginning, 2 its middle, 3 its end
+  __device__ __forceinline__ bool next(const PagedParams& p, PagedItem& it, int& part) {
+    while (r < p.requests && s < x1) {
+      const int total = q.tiles(p, tile, it);
+      const long w = q.weight(p, tile + 1) - q.weight(p, tile), e = s + w;
+      const auto cut = [&](long x) -> int {
+        const long t = x - s - PA_ITEM_TILES<FEW>;
+        return x >= e || t > total ? total : t < 0 ? 0 : static_cast<int>(t);
+      };
+      const int t0 = cut(x0), t1 = cut(x1);
+      const bool valid = t1 > t0 || (total == 0 && x0 < e && e <= x1);
+      it.q_row = q.q_row;
+      it.kv_head = head;
+      it.past = q.past;
+      it.request = r;
+      it.total = t1 - t0;
+      part = t0 > 0 ? (t1 < total ? 2 : 3) : (t1 < total ? 1 : 0);
+      // of the sinks' tiles and the band's behind them, those numbered t0 .. t1 - 1
+      const int n0 = it.end[0], f1 = it.first[1];
+      it.first[0] = min(t0, n0);
+      it.end[0] = min(t1, n0);
+      it.first[1] = f1 + max(t0 - n0, 0);
+      it.end[1] = f1 + max(t1 - n0, 0);
+      s = e;
+      if (++tile == q.row_tiles) {
+        tile = 0;
+        if (++head == p.kv_heads) {
+          head = 0;
+          ++r;
+          enter(p);
+        }
+      }
+      if (valid) return true;
+    }
+    return false;
+  }
+};
+
+// ---- outputs ----------------------------------------------------------------------------------------------------------------
+// Where row x of an item goes: token and head; false: nowhere.
+__device__ __forceinline__ bool paged_row(const PagedParams& p, const PagedItem& it, int x, long& tok, int& head) {
+  const int h = x & ((1 << p.pack_shift) - 1);
+  tok = static_cast<long>(it.q_row) + it.tok0 + (x >> p.pack_shift);
+  head = it.kv_head * p.group + h;
+  return x < it.rows && h < p.group;
+}
+
+// 256 rows: this thread's row (l: row sum, m: reference maximum in log2 units; any: its sub-tile has seen a key tile), turned around in
+// shared memory so that a store covers whole 128-byte blocks of rows.
+template <typename Ready>
+__device__ __forceinline__ void paged_epilogue(const PagedParams& p, PagedSmem<false>& s, const PagedItem& it, uint32_t tO, float l, float m, bool any,
+                                               Ready ready) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int w = warp >> 2, quad = warp & 3;
+  const int x = w * PT + quad * 32 + lane;
+  const bool part = it.slot >= 0;
+  float lse = -INFINITY, f = 0.f;
+  if (any && l > 0.f && m > -INFINITY) {
+    lse = (m + log2f(l)) * 0.6931471805599453f;
+    f = 1.0f / l;
+  }
+  long tok;
+  int head;
+  const bool valid = paged_row(p, it, x, tok, head);
+  if (part) {
+    if (x < p.part_rows) p.part_lse[static_cast<long>(it.slot) * p.part_rows + x] = any && l != l ? l : lse;   // (a NaN score: see combine_parts)
+  } else if (valid) {
+    p.lse[head * p.lse_head + tok] = lse;
+  }
+  uint8_t* blk = s.o_stage[warp];
+  const int sub = lane >> 3, ch = lane & 7;
+  const int x0 = w * PT + quad * 32 + sub;
+  uint8_t* dst[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const bool there = paged_row(p, it, x0 + i * 4, tok, head);
+    uint8_t* d = part ? reinterpret_cast<uint8_t*>(p.part_o + (static_cast<long>(it.slot) * p.part_rows + x0 + i * 4) * PD)
+                      : reinterpret_cast<uint8_t*>(p.o + tok * p.o_token + head * p.o_head);
+    dst[i] = there ? d + ch * 16 : nullptr;
+  }
+  ready();
+#pragma unroll 1
+  for (int c = 0; c < (part ? 4 : 2); ++c) {
+    if (part) {
+      uint32_t ov[32];
+      tmem_ld_x32(tO + c * 32, ov);
+      tmem_wait_ld();
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        float g[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] = f == 0.f ? 0.f : __uint_as_float(ov[q * 4 + i]) * f;
+        *reinterpret_cast<float4*>(blk + sw128_offset(lane, q)) = make_float4(g[0], g[1], g[2], g[3]);
+      }
+    } else {
+      uint32_t ov[2][32];
+      tmem_ld_x32(tO + c * 64, ov[0]);
+      tmem_ld_x32(tO + c * 64 + 32, ov[1]);
+      tmem_wait_ld();
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        float g[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = f == 0.f ? 0.f : __uint_as_float(ov[q >> 2][(q & 3) * 8 + i]) * f;
+        *reinterpret_cast<uint4*>(blk + sw128_offset(lane, q)) =
+            make_uint4(pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]), pack_bf16x2(g[4], g[5]), pack_bf16x2(g[6], g[7]));
+      }
+    }
+    __syncwarp();
+    uint4 val[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) val[i] = *reinterpret_cast<const uint4*>(blk + sw128_offset(i * 4 + sub, ch));
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (dst[i] != nullptr) {
+        *reinterpret_cast<uint4*>(dst[i]) = val[i];
+        dst[i] += 128;
+      }
+    __syncwarp();
+  }
+}
+
+// Up to 128 rows, of whose key tiles each sub-tile has seen half: sub-tile 0's warps merge both O from tensor memory.
+__device__ __forceinline__ void paged_few_epilogue(const PagedParams& p, PagedSmem<true>& s, const PagedItem& it, uint32_t tO, float l0, float m0) {
+  const int x = threadIdx.x;
+  const float2 other = s.stat[x];
+  const float m = fmaxf(m0, other.x);
+  const float a0 = fast_exp2(m0 - m), a1 = fast_exp2(other.x - m);
+  const float l = (m0 > -INFINITY || l0 != l0 ? a0 * l0 : 0.f) + (other.x > -INFINITY || other.y != other.y ? a1 * other.y : 0.f);
+  const bool live = l > 0.f && m > -INFINITY, use0 = live && m0 > -INFINITY, use1 = live && other.x > -INFINITY;
+  const float lse = live ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  const float f0 = a0 / l, f1 = a1 / l;
+  const bool part = it.slot >= 0;
+  long tok;
+  int head;
+  const bool valid = paged_row(p, it, x, tok, head);
+  const long prow = static_cast<long>(it.slot) * p.part_rows + x;
+  if (valid) {
+    if (part) p.part_lse[prow] = l != l ? l : lse;
+    else p.lse[head * p.lse_head + tok] = lse;
+  }
+  __nv_bfloat16* optr = p.o + tok * p.o_token + head * p.o_head;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t u[32], v[32];
+    tmem_ld_x32(tO + c * 32, u);
+    tmem_ld_x32(tO + 128 + c * 32, v);
+    tmem_wait_ld();
+    if (!valid) continue;
+    float f[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      f[i] = (use0 ? __uint_as_float(u[i]) * f0 : 0.f) + (use1 ? __uint_as_float(v[i]) * f1 : 0.f);
+    if (part) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        reinterpret_cast<float4*>(p.part_o + prow * PD + c * 32)[q] = make_float4(f[q * 4], f[q * 4 + 1], f[q * 4 + 2], f[q * 4 + 3]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        reinterpret_cast<uint4*>(optr + c * 32)[q] = make_uint4(pack_bf16x2(f[q * 8], f[q * 8 + 1]), pack_bf16x2(f[q * 8 + 2], f[q * 8 + 3]),
+                                                                pack_bf16x2(f[q * 8 + 4], f[q * 8 + 5]), pack_bf16x2(f[q * 8 + 6], f[q * 8 + 7]));
+    }
+  }
+}
+
+// The columns [low, lim) of a tile row's keys that a token at position `pos` sees: of the sinks (e = 0) or of the band.
+__device__ __forceinline__ int paged_low(const PagedParams& p, int e, int pos) { return e == 0 || p.left < 0 ? 0 : max(0, pos - p.left); }
+__device__ __forceinline__ int paged_lim(const PagedParams& p, int e, int pos) { return e == 0 ? min(p.sink, pos - p.left) : pos + 1; }
+
+template <bool FEW>
+__global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_constant__ PagedParams p) {
+  constexpr int STAGES = PagedSmem<FEW>::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  PagedSmem<FEW>& s = *reinterpret_cast<PagedSmem<FEW>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int psh = p.pack_shift;
+  // FEW: warps behind the last row that an item may have are idle
+  const int act_warps = FEW ? (min(PT, p.part_rows) + 31) / 32 : 4;
+
+  if (threadIdx.x == PA_TMA_WARP * 32) {
+    mbar_init(&s.q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], act_warps);
+      mbar_init(&s.pv_done[i], 1);
+      mbar_init(&s.item_full[i], 1);
+      mbar_init(&s.item_empty[i], (FEW ? 1 : 2) + 2 * act_warps);
+    }
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&s.k_full[i], 1);
+      mbar_init(&s.k_empty[i], 1);
+      mbar_init(&s.v_full[i], 1);
+      mbar_init(&s.v_empty[i], 1);
+    }
+    mbar_init(&s.q_empty, 1);
+    mbar_init(&s.s_free, act_warps);
+    mbar_init(&s.stat_full, act_warps);
+    mbar_init(&s.merged, act_warps);
+    s.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == PA_QK_WARP) {
+    tmem_alloc(&s.tmem_base, 512);
+    tmem_relinquish();
+  }
+  grid_wait();
+
+  // ---- the share of this CTA: sums of the requests' weights -------------------------------------------------------------------
+  const int per = (p.requests + PA_THREADS - 1) / PA_THREADS;
+  const int r0 = min(p.requests, static_cast<int>(threadIdx.x) * per), r1 = min(p.requests, r0 + per);
+  long mine = 0;
+  for (int r = r0; r < r1; ++r) {
+    const PagedRequest<FEW> q = paged_request<FEW>(p, r, blockIdx.x == 0);
+    if (q.row_tiles > 0) mine += p.kv_heads * q.weight(p, q.row_tiles);
+  }
+  long before = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long y = __shfl_up_sync(0xFFFFFFFFu, before, d);
+    if (lane >= d) before += y;
+  }
+  if (lane == 31) s.sums[warp] = before;
+  before -= mine;
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = s.tmem_base;
+  long total = 0;
+  for (int i = 0; i < PA_THREADS / 32; ++i) {
+    if (i < warp) before += s.sums[i];
+    total += s.sums[i];
+  }
+  // as many CTAs as have a share worth its start
+  const long most = total / (PA_ITEM_TILES<FEW> + PA_MIN_SHARE);
+  const int ctas = static_cast<int>(most < 1 ? 1 : most < gridDim.x ? most : gridDim.x);
+  const int cta = blockIdx.x;
+  const long x0 = total * cta / ctas, x1 = total * (cta + 1) / ctas;
+  const bool work = total > 0 && cta < ctas;
+  if (work && x0 >= before && x0 < before + mine) {
+    long at = before;
+    for (int r = r0; r < r1; ++r) {
+      const PagedRequest<FEW> q = paged_request<FEW>(p, r, false);
+      const long w = q.row_tiles > 0 ? p.kv_heads * q.weight(p, q.row_tiles) : 0;
+      if (x0 < at + w) {
+        s.start_r = r;
+        s.start_x = x0 - at;
+        break;
+      }
+      at += w;
+    }
+  }
+  __syncthreads();
+
+  WaitCtx wc{&s.abort_flag, p.status, 4000000000ull};
+  auto wait = [&](uint64_t* bar, uint32_t parity, int where) -> bool {
+    if (mbar_wait_quiet(bar, parity, wc)) return true;
+    report_error_call(wc.abort_flag, wc.status, UA_ERR_MBAR_TIMEOUT, where, static_cast<int>(parity));
+    return false;
+  };
+  // Consumers: item n is in its slot, and there is one (false: no more, or a wait gave up). They hand it back by an arrival on item_empty.
+  auto item_there = [&](uint32_t n) -> bool { return wait(&s.item_full[n & 1], (n >> 1) & 1, 420) && s.item[n & 1].exists != 0; };
+
+  if (!work) {
+    if (threadIdx.x < PA_DESC) p.part_desc[cta * PA_DESC + threadIdx.x] = 0;
+    grid_trigger();
+  } else if (warp >= PA_SOFTMAX_WARPS) {
+    reg_dealloc<PA_REGS_LOAD>();
+    if (warp == PA_TMA_WARP) {
+      // =============================== walker and TMA producer =================================
+      // All lanes walk; a lane issues the box of one page and d-half of a tile.
+      PagedWalk<FEW> walk;
+      walk.begin(p, s.start_r, s.start_x, x0, x1);
+      const int box_rows = p.page_shift < 7 ? 1 << p.page_shift : PT;
+      const int boxes = 2 * (PT / box_rows);
+      const int box = lane >> 1, half = lane & 1;
+      const uint32_t box_bytes = static_cast<uint32_t>(box_rows) * 128;
+      int head_part[4] = {0, 0, 0, 0}, cont = 0;
+      uint32_t j = 0, live = 0;
+      bool ok = true;
+      for (uint32_t n = 0; ok; ++n) {
+        PagedItem it;
+        int part = 0;
+        const bool got = walk.next(p, it, part);
+        const uint32_t slot = n & 1;
+        if (n >= 2 && !__all_sync(0xFFFFFFFFu, wait(&s.item_empty[slot], ((n - 2) >> 1) & 1, 403))) break;
+        it.exists = got;
+        it.slot = part == 0 ? -1 : 2 * cta + (part == 1);
+        if (got && part == 1) {
+          head_part[0] = 1;
+          head_part[1] = it.q_row + it.tok0;
+          head_part[2] = it.kv_head * p.group;
+          head_part[3] = it.rows;
+        } else if (got && part > 1) {
+          cont = part == 2 ? 1 : 2;
+        }
+        if (lane == 0) {
+          s.item[slot] = it;
+          mbar_arrive(&s.item_full[slot]);
+        }
+        if (!got) break;
+        if (it.total == 0) continue;
+        // Q: the scores of the item before are complete
+        if (live > 0 && !__all_sync(0xFFFFFFFFu, wait(&s.q_empty, (live - 1) & 1, 402))) break;
+        ++live;
+        if (lane == 0) mbar_arrive_expect_tx(&s.q_full, (FEW ? 1 : 2) * PA_TILE_BYTES);
+        __syncwarp();
+        if (lane < (FEW ? 2 : 4)) {
+          const int w = lane >> 1;
+          tma_load_3d(s.q[w] + half * 16384, &p.tm_q, &s.q_full, half * 64, it.kv_head * p.group, it.q_row + it.tok0 + ((w * PT) >> psh));
+        }
+        const int* row = p.table + it.request * p.table_stride;
+        // this lane's page of tile t: its first key, and the entry (-1: the box is not loaded)
+        auto entry_of = [&](int e, int t) -> int {
+          if (lane >= boxes || t >= it.end[e]) return -1;
+          const int key = t * PT + box * box_rows;
+          if (key >= it.hi[e] || key + box_rows <= it.lo[e]) return -1;
+          const int col = key >> p.page_shift;
+          const int page = col < p.columns ? row[col] : -1;
+          if (page >= 0 && page < p.pages) return page;
+          paged_error(p.status, 520, it.request);
+          return -1;
+        };
+#pragma unroll 1
+        for (int e = 0; e < 2 && ok; ++e) {
+          int page = entry_of(e, it.first[e]);
+#pragma unroll 1
+          for (int t = it.first[e]; t < it.end[e]; ++t, ++j) {
+            const int next_page = entry_of(e, t + 1);
+            const int off = (t * PT + box * box_rows) & ((1 << p.page_shift) - 1);
+            const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, page >= 0)) * box_bytes;
+            const int st = j % STAGES;
+            const uint32_t ph = (j / STAGES) & 1;
+            ok = __all_sync(0xFFFFFFFFu, wait(&s.k_empty[st], ph ^ 1, 400));
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(&s.k_full[st], bytes);
+            __syncwarp();
+            if (page >= 0) tma_load_4d(s.k[st] + half * 16384 + box * box_bytes, &p.tm_k, &s.k_full[st], half * 64, it.kv_head, off, page);
+            ok = __all_sync(0xFFFFFFFFu, wait(&s.v_empty[st], ph ^ 1, 401));
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(&s.v_full[st], bytes);
+            __syncwarp();
+            if (page >= 0) tma_load_4d(s.v[st] + half * 16384 + box * box_bytes, &p.tm_v, &s.v_full[st], half * 64, it.kv_head, off, page);
+            page = next_page;
+          }
+        }
+      }
+      grid_trigger();
+      if (lane == 0) {
+        int* d = p.part_desc + cta * PA_DESC;
+        for (int i = 0; i < 4; ++i) d[i] = head_part[i];
+        d[4] = cont;
+      }
+    } else if (warp == PA_QK_WARP || (!FEW && warp == PA_PV_WARP)) {
+      // =============================== MMA issuers ============================================
+      if (elect_one()) {
+        const uint32_t idesc_s = make_idesc_bf16(128, 128, 0, 0);   // S = Q K^T, both K-major
+        const uint32_t idesc_o = make_idesc_bf16(128, 128, 0, 1);   // O += P V, V is N-major
+        const uint32_t q_desc = desc_lo(smem_u32(s.q[0]), 16), k_desc = desc_lo(smem_u32(s.k[0]), 16);
+        const uint32_t v_desc = desc_lo(smem_u32(s.v[0]), 16384);
+        constexpr uint32_t HI = desc_hi_sw128(1024);
+        constexpr uint32_t TILE16 = PA_TILE_BYTES >> 4;
+        auto issue_s = [&](int w, int st) {
+          const uint32_t qa = q_desc + (FEW ? 0 : w) * TILE16, ka = k_desc + st * TILE16;
+          const uint32_t tS = tmem_base + (FEW ? w * 128 : 0);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+            umma_ss_lo<HI, HI>(tS, qa + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
+          }
+        };
+        auto issue_pv = [&](int w, int st, bool acc) {
+          const uint32_t va = v_desc + st * TILE16;
+          const uint32_t tP = tmem_base + (FEW ? w * 128 : 128 + w * 64), tO = tmem_base + 256 + w * 128;
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) umma_ts_lo<HI>(tO, tP + kk * 8, va + ((kk * 2048) >> 4), idesc_o, (acc || kk > 0) ? 1u : 0u);
+        };
+        auto take_total = [&](uint32_t n) -> int {
+          const int t = s.item[n & 1].total;
+          mbar_arrive(&s.item_empty[n & 1]);
+          return t;
+        };
+        bool ok = true;
+        uint32_t kv = 0, live = 0;
+        if constexpr (FEW) {
+          uint32_t phase = 0;
+          for (uint32_t n = 0; ok && item_there(n); ++n) {
+            const int n_total = take_total(n);
+            if (n_total == 0) continue;
+            if (!wait(&s.q_full, live & 1, 430)) break;
+            auto next_s = [&](int i) -> bool {
+              const uint32_t g = kv + i;
+              if (!wait(&s.k_full[g % STAGES], (g / STAGES) & 1, 431)) return false;
+              tc_fence_after_sync();
+              issue_s(i & 1, g % STAGES);
+              tc_commit(&s.s_full[i & 1]);
+              tc_commit(&s.k_empty[g % STAGES]);
+              if (i + 1 == n_total) tc_commit(&s.q_empty);
+              return true;
+            };
+            ok = next_s(0) && (n_total < 2 || next_s(1));
+            for (int i = 0; i < n_total && ok; ++i) {
+              const int w = i & 1, st = (kv + i) % STAGES;
+              if (!wait(&s.v_full[st], ((kv + i) / STAGES) & 1, 433)) { ok = false; break; }
+              if (!wait(&s.p_full[w], (phase >> w) & 1, 434)) { ok = false; break; }
+              phase ^= 1u << w;
+              tc_fence_after_sync();
+              issue_pv(w, st, i >= 2);
+              tc_commit(&s.pv_done[w]);
+              tc_commit(&s.v_empty[st]);
+              if (i + 2 < n_total) ok = next_s(i + 2);
+            }
+            kv += n_total;
+            ++live;
+          }
+        } else if (warp == PA_QK_WARP) {
+          uint32_t use = 0;
+          auto scores = [&](int w, int st) -> bool {
+            if (use > 0 && !wait(&s.s_free, (use - 1) & 1, 436)) return false;
+            ++use;
+            tc_fence_after_sync();
+            issue_s(w, st);
+            tc_commit(&s.s_full[w]);
+            return true;
+          };
+          for (uint32_t n = 0; ok && item_there(n); ++n) {
+            const int n_total = take_total(n);
+            if (n_total == 0) continue;
+            if (!wait(&s.q_full, live & 1, 430)) break;
+            for (int i = 0; i < n_total && ok; ++i, ++kv) {
+              const int st = kv % STAGES;
+              ok = wait(&s.k_full[st], (kv / STAGES) & 1, 431) && scores(0, st) && scores(1, st);
+              if (ok) tc_commit(&s.k_empty[st]);
+            }
+            if (!ok) break;
+            tc_commit(&s.q_empty);
+            ++live;
+          }
+        } else {
+          auto product = [&](int w, int st, bool acc) -> bool {
+            if (!wait(&s.p_full[w], kv & 1, 434 + w)) return false;
+            tc_fence_after_sync();
+            issue_pv(w, st, acc);
+            tc_commit(&s.pv_done[w]);
+            return true;
+          };
+          for (uint32_t n = 0; ok && item_there(n); ++n) {
+            const int n_total = take_total(n);
+            for (int i = 0; i < n_total && ok; ++i, ++kv) {
+              const int st = kv % STAGES;
+              ok = wait(&s.v_full[st], (kv / STAGES) & 1, 433) && product(0, st, i > 0) && product(1, st, i > 0);
+              if (ok) tc_commit(&s.v_empty[st]);
+            }
+          }
+        }
+      }
+    }
+  } else {
+    reg_alloc<PA_REGS_SOFTMAX>();
+    if ((warp & 3) < act_warps) {
+      // =============================== softmax + epilogue =====================================
+      const int w = warp >> 2, quad = warp & 3;
+      const int r_tile = quad * 32 + lane;
+      const int r_cta = (FEW ? 0 : w * PT) + r_tile;          // row of the item
+      const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+      const uint32_t tS = tmem_base + lane_base + (FEW ? w * 128 : 0);
+      const uint32_t tP = FEW ? tS : tmem_base + lane_base + 128 + w * 64;
+      const uint32_t tO = tmem_base + lane_base + 256 + w * 128;
+      const float NEG_INF = -INFINITY;
+      uint32_t cnt = 0;                        // score tiles of this sub-tile so far
+      uint32_t kv = 0;                         // key tiles of this CTA so far
+      for (uint32_t n = 0; __all_sync(0xFFFFFFFFu, item_there(n)); ++n) {
+        const PagedItem& it = s.item[n & 1];   // (stays in shared memory: the score loop needs the registers)
+        float m_use = NEG_INF, l = 0.f;
+        bool ok = true;
+        uint32_t j = 0;
+#pragma unroll 1
+        for (int e = 0; e < 2 && ok; ++e) {
+          // every row of the warp sees all of the tiles [clear_first, clear_end), no row anything outside [some_first, some_end)
+          int t = it.first[e];
+          const int t_end = it.end[e];
+          int clear_first, clear_end, some_first, some_end;
+          {
+            const int pos = it.past + it.tok0;
+            const int first = pos + ((r_cta - lane) >> psh), last = pos + ((r_cta - lane + 31) >> psh);
+            clear_end = max(0, paged_lim(p, e, first)) >> 7;
+            some_end = (max(0, paged_lim(p, e, last)) + PT - 1) >> 7;
+            some_first = paged_low(p, e, first) >> 7;
+            clear_first = (paged_low(p, e, last) + PT - 1) >> 7;
+            if (r_cta - lane >= it.rows) some_end = 0;
+          }
+#pragma unroll 1
+          for (; t < t_end; ++t, ++j) {
+            if (FEW && (j & 1) != static_cast<uint32_t>(w)) continue;
+            ok = mbar_wait_quiet(&s.s_full[w], cnt & 1, wc);
+            ++cnt;
+            tc_fence_after_sync();
+            // Values that no row of the item sees (behind the last key, before the first of a window, pages that were not loaded)
+            // may be anything, and P = 0 times NaN is one: they become zeros before the tile's P is handed over. (Of two sub-tiles the
+            // first does it: its product is issued before the other's.)
+            const int c0 = t * PT;
+            if ((FEW || w == 0) && (c0 < it.lo[e] || c0 + PT > it.hi[e])) {
+              const uint32_t g = kv + j;
+              const int st = g % STAGES;
+              ok = mbar_wait_quiet(&s.v_full[st], (g / STAGES) & 1, wc) && ok;
+              const int a = max(it.lo[e] - c0, 0), b = min(it.hi[e] - c0, PT);
+              const int dead = a + PT - b;
+              for (int i = threadIdx.x - w * PT; i < dead * 16; i += act_warps * 32) {
+                const int x = i >> 4, r = x < a ? x : b + x - a;
+                *reinterpret_cast<uint4*>(s.v[st] + ((i >> 3) & 1) * 16384 + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async_smem();
+            }
+            if (t < some_first || t >= some_end) {
+              // nothing to see for these 32 rows: P = 0, maximum and sum stay
+              if (!FEW) mbar_arrive_warp(&s.s_free);
+              if (j >= (FEW ? 2u : 1u)) ok = mbar_wait_quiet(&s.pv_done[w], cnt & 1, wc) && ok;
+              ok = __all_sync(0xFFFFFFFFu, ok);
+              if (!ok) break;
+              tc_fence_after_sync();
+              uint32_t zero[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) zero[i] = 0u;
+              tmem_st_x32(tP, zero);
+              tmem_st_x32(tP + 32, zero);
+              tmem_wait_st();
+              tc_fence_before_sync();
+              mbar_arrive_warp(&s.p_full[w]);
+              continue;
+            }
+            float sv[PT];
+            {
+              uint32_t(&raw)[PT] = reinterpret_cast<uint32_t(&)[PT]>(sv);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) tmem_ld_x32(tS + c * 32, reinterpret_cast<uint32_t(&)[32]>(raw[c * 32]));
+              tmem_wait_ld();
+            }
+            if (!FEW) {
+              tc_fence_before_sync();
+              mbar_arrive_warp(&s.s_free);
+            }
+            if (t < clear_first || t >= clear_end) {
+              const int pos = it.past + it.tok0;
+              const int at = pos + (r_cta >> psh), first = pos + ((r_cta - lane) >> psh), last = pos + ((r_cta - lane + 31) >> psh);
+              const int low = paged_low(p, e, at) - c0, lim = paged_lim(p, e, at) - c0;
+              const int clear_lo = paged_low(p, e, last) - c0, clear_hi = paged_lim(p, e, first) - c0;
+#pragma unroll
+              for (int c = 0; c < PT; c += 32) {
+                if (c >= clear_lo && c + 32 <= clear_hi) continue;
+                // bit i: column c + i is seen
+                const int a = min(max(low - c, 0), 32), b = min(max(lim - c, 0), 32);
+                const uint32_t seen = (b > 0 ? 0xFFFFFFFFu >> (32 - b) : 0u) & (a < 32 ? 0xFFFFFFFFu << a : 0u);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) sv[c + i] = (seen >> i) & 1u ? sv[c + i] : NEG_INF;
+              }
+            }
+            float mx8[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mx8[i] = fmaxf(sv[i], sv[8 + i]);
+#pragma unroll
+            for (int i = 16; i < PT; i += 16)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) mx8[k] = fmax3(mx8[k], sv[i + k], sv[i + 8 + k]);
+            float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]));
+            mx = fmax3(mx, mx8[6], mx8[7]) * p.scale_log2;
+            const float m_new = fmaxf(m_use, mx);
+            // P V of the tile before is complete: P may be overwritten, and O rescaled
+            bool need = false;
+            if (j < (FEW ? 2u : 1u)) {
+              m_use = m_new;
+            } else {
+              ok = mbar_wait_quiet(&s.pv_done[w], cnt & 1, wc) && ok;
+              tc_fence_after_sync();
+              // (only when the maximum grew by more than 2^8)
+              need = (m_new - m_use > 8.0f) || (m_use == NEG_INF && m_new > NEG_INF);
+            }
+            if (__any_sync(0xFFFFFFFFu, need || !ok)) {
+              ok = __all_sync(0xFFFFFFFFu, ok);
+              if (!ok) break;
+              const float alpha = need ? fast_exp2(m_use - m_new) : 1.0f;
+              if (need) m_use = m_new;
+              l *= alpha;
+#pragma unroll 1
+              for (int c = 0; c < 8; ++c) {
+                uint32_t ov[16];
+                tmem_ld_x16(tO + c * 16, ov);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+                tmem_st_x16(tO + c * 16, ov);
+              }
+            }
+            const float m_eff = (m_use == NEG_INF) ? 0.f : m_use;
+            const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
+            const uint64_t nm2 = f2_pack(-m_eff, -m_eff);
+            uint64_t ls2[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ls2[k] = f2_pack(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float a, b;
+                f2_unpack(f2_fma(f2_pack(sv[c * 32 + 2 * i], sv[c * 32 + 2 * i + 1]), sc2, nm2), a, b);
+                const float p0 = fast_exp2(a), p1 = fast_exp2(b);
+                ls2[i & 3] = f2_add(ls2[i & 3], f2_pack(p0, p1));
+                pk[i] = pack_bf16x2(p0, p1);           // (bf16: an operand of P V; the sum takes them unrounded)
+              }
+              tmem_st_x16(tP + c * 16, pk);
+            }
+            tmem_wait_st();
+            tc_fence_before_sync();
+            mbar_arrive_warp(&s.p_full[w]);
+            float ls4[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float a, b;
+              f2_unpack(ls2[k], a, b);
+              ls4[k] = a + b;
+            }
+            l += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);
+          }
+        }
+        // ---------------------------------- epilogue --------------------------------------------
+        kv += it.total;
+        const bool any = it.total > (FEW ? w : 0);
+        auto ready = [&]() {
+          if (any && ok) ok = mbar_wait_quiet(&s.pv_done[w], (cnt & 1) ^ 1, wc);
+          tc_fence_after_sync();
+        };
+        if constexpr (FEW) {
+          ready();
+          if (w == 1) {
+            s.stat[r_tile] = make_float2(any ? m_use : NEG_INF, any ? l : 0.f);
+            tc_fence_before_sync();
+            mbar_arrive_warp(&s.stat_full);
+            ok = mbar_wait_quiet(&s.merged, n & 1, wc) && ok;      // (O is free for this sub-tile's next item)
+          } else {
+            ok = mbar_wait_quiet(&s.stat_full, n & 1, wc) && ok;
+            tc_fence_after_sync();
+            paged_few_epilogue(p, s, it, tO, any ? l : 0.f, any ? m_use : NEG_INF);
+            tc_fence_before_sync();
+            mbar_arrive_warp(&s.merged);
+          }
+        } else {
+          paged_epilogue(p, s, it, tO, l, m_use, any, ready);
+          tc_fence_before_sync();
+        }
+        if (!ok) report_error_call(wc.abort_flag, wc.status, UA_ERR_MBAR_TIMEOUT, 440 + w, static_cast<int>(j));
+        __syncwarp();                            // every lane is done reading the item
+        if (lane == 0) mbar_arrive(&s.item_empty[n & 1]);
+        if (!__all_sync(0xFFFFFFFFu, ok)) break;
+      }
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == PA_QK_WARP) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// The parts of a cut item, in the order of its keys: O = sum_i w_i O_i with w_i = exp(lse_i - lse), fp32, one warp per row, 4 elements per
+// lane. Block x: the item that begins in CTA x and goes on behind it, if there is one.
+struct CombineParams {
+  const float* part_o;
+  const float* part_lse;
+  const int* desc;
+  int part_rows, ctas;
+  int pack_shift, group;
+  __nv_bfloat16* o;
+  long o_token, o_head;
+  float* lse;
+  long lse_head;
+};
+constexpr int COMBINE_ROWS = 8;        // rows of a block
+__global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constant__ CombineParams p) {
   grid_wait();
   grid_trigger();
-  const long row = static_cast<long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const long tok = row / a.heads, head = row % a.heads;
-  if (tok >= a.tokens || tok >= a.cu_new[a.requests]) return;
-  int lo = 0, hi = static_cast<int>(a.requests);
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu_new[mid] <= tok) lo = mid;
-    else hi = mid;
+  const int first = blockIdx.x, lane = threadIdx.x & 31;
+  const int* d = p.desc + first * PA_DESC;
+  const int x = blockIdx.y * COMBINE_ROWS + (threadIdx.x >> 5);
+  if (d[0] == 0 || x >= d[3]) return;
+  const int h = x & ((1 << p.pack_shift) - 1);
+  if (h >= p.group) return;
+  // the slots of its parts: 2 first + 1, then 2 (first + 1), 2 (first + 2) .. up to the CTA in which it ends
+  int n = 1;
+  while (first + n < p.ctas && p.desc[(first + n) * PA_DESC + 4] == 1) ++n;
+  ++n;
+  auto slot = [&](int i) -> long { return i == 0 ? 2 * first + 1 : 2 * (first + i); };
+  float mx = -INFINITY;
+  bool bad = false;                    // a NaN score: O = 0 and lse = -inf, as in an item that is not cut
+  for (int i = lane; i < n; i += 32) {
+    const float y = p.part_lse[slot(i) * p.part_rows + x];
+    bad |= y != y;
+    mx = fmaxf(mx, y);
   }
-  const int r = lo, first = a.cu_new[r], n = a.cu_new[r + 1] - first, c = a.context[r];
-  const int pos = c - n + static_cast<int>(tok - first);
-  const long kvh = head / (a.heads / a.kv_heads);
-  const float4 q = bf16x4(static_cast<const __nv_bfloat16*>(a.q) + tok * a.q_token + head * a.q_head + lane * 4);
-  float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int j = 0; j <= pos; ++j) {
-    if (a.left >= 0 && j < pos - a.left && j >= a.sink) j = static_cast<int>(pos - a.left);
-    const long col = j >> a.page_shift, off = j & ((1 << a.page_shift) - 1);
-    const int page = col < a.columns ? a.table[r * a.table_stride + col] : -1;
-    if (page < 0 || page >= a.pages) {
-      if (lane == 0 && atomicCAS(status, 0, UA_ERR_BAD_ARG) == 0) {
-        status[1] = 520;
-        status[2] = r;
-        status[3] = page;
-      }
-      continue;
-    }
-    const float4 k = bf16x4(static_cast<const __nv_bfloat16*>(a.k) + page * a.k_page + off * a.k_token + kvh * a.k_head + lane * 4);
-    float s = q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
-    s *= scale;
-    const float mn = fmaxf(m, s), al = mn == -INFINITY ? 1.f : __expf(m - mn), w = mn == -INFINITY ? 0.f : __expf(s - mn);
-    m = mn;
-    l = l * al + w;
-    const float4 v = bf16x4(static_cast<const __nv_bfloat16*>(a.v) + page * a.v_page + off * a.v_token + kvh * a.v_head + lane * 4);
-    acc.x = acc.x * al + w * v.x;
-    acc.y = acc.y * al + w * v.y;
-    acc.z = acc.z * al + w * v.z;
-    acc.w = acc.w * al + w * v.w;
+  for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, k));
+  if (__any_sync(0xFFFFFFFFu, bad)) mx = -INFINITY;
+  float tot = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (mx > -INFINITY) {
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const long row = slot(i) * p.part_rows + x;
+      const float w = __expf(p.part_lse[row] - mx);
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + row * PD + lane * 4);
+      tot += w;
+      acc.x += w * v.x;
+      acc.y += w * v.y;
+      acc.z += w * v.z;
+      acc.w += w * v.w;
+    }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = tot > 0.f ? 1.f / tot : 0.f;
+  const long tok = d[1] + (x >> p.pack_shift);
+  const int head = d[2] + h;
   uint2 o;
   o.x = pack_bf16x2(acc.x * inv, acc.y * inv);
   o.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.o) + tok * a.o_token + head * a.o_head + lane * 4) = o;
-  if (lane == 0) a.lse[head * a.lse_head + tok] = l > 0.f ? m + __logf(l) : -INFINITY;
+  *reinterpret_cast<uint2*>(p.o + tok * p.o_token + head * p.o_head + lane * 4) = o;
+  if (lane == 0) p.lse[head * p.lse_head + tok] = tot > 0.f ? mx + __logf(tot) : -INFINITY;
 }
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------
+// Which forms a call needs, and the rows of a part of each (0: not launched).
+struct PagedPlan {
+  int pack_shift, few_rows, full_rows, few_limit;
+};
+static PagedPlan plan_paged(const UaPagedAttn* a) {
+  PagedPlan d{};
+  const long group = a->heads / a->kv_heads;
+  while ((1l << d.pack_shift) < group) ++d.pack_shift;
+  const long most = a->most_new << d.pack_shift;
+  if (most <= PT) {
+    d.few_rows = static_cast<int>(most);
+    d.few_limit = d.few_rows;
+  } else {
+    d.full_rows = 2 * PT;
+    if (a->requests > 1) d.few_rows = d.few_limit = PT;
+  }
+  return d;
+}
+static long part_floats(int rows, int ctas) { return rows > 0 ? static_cast<long>(ctas) * (2l * rows * (PD + 1) + PA_DESC) : 0; }
+
+template <bool FEW>
+static int launch_paged(const PagedParams& p, int ctas, cudaStream_t stream) {
+  static int smem_set[64] = {0};
+  const int smem_bytes = sizeof(PagedSmem<FEW>) + 1024;
+  int dev = 0;
+  UA_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !smem_set[dev]) {
+    UA_CUDA(cudaFuncSetAttribute(attn_paged_kernel<FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes));
+    if (dev < 64) smem_set[dev] = 1;
+  }
+  UA_CUDA(launch_kernel(attn_paged_kernel<FEW>, ctas, PA_THREADS, smem_bytes, stream, true, p));
+  return 0;
+}
+
+// strides in elements; an axis of one may have any (the map wants multiples of 16 bytes)
+static uint64_t stride_bytes(long stride, long size) { return size > 1 ? static_cast<uint64_t>(stride) * 2 : PD * 2; }
 
 }  // namespace ua
 
 using namespace ua;
 
-extern "C" int ua_attn_paged(const UaPagedAttn* a, float softmax_scale, int* status, cudaStream_t stream) {
-  if (a->tokens <= 0 || a->requests <= 0) return 0;
+// Floats of workspace that ua_attn_paged needs.
+extern "C" long ua_attn_paged_workspace(const UaPagedAttn* a) {
+  if (a->kv_heads <= 0 || a->heads % a->kv_heads != 0) return 0;
+  const PagedPlan d = plan_paged(a);
+  return part_floats(d.few_rows, sm_count()) + part_floats(d.full_rows, sm_count());
+}
+
+extern "C" int ua_attn_paged(const UaPagedAttn* a, float softmax_scale, float* workspace, int* status, cudaStream_t stream) {
+  if (a->tokens <= 0 || a->requests <= 0 || a->most_new <= 0) return 0;
   if (a->kv_heads <= 0 || a->heads % a->kv_heads != 0)
     UA_FAIL("ua_attn_paged: %ld query heads do not divide into %ld key/value heads", a->heads, a->kv_heads);
+  if (a->heads / a->kv_heads > PT) UA_FAIL("ua_attn_paged: %ld query heads for a key/value head (%d at most)", a->heads / a->kv_heads, PT);
   const uintptr_t bases = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v) |
                           reinterpret_cast<uintptr_t>(a->o);
-  const long strides = a->q_token | a->q_head | a->k_page | a->k_token | a->k_head | a->v_page | a->v_token | a->v_head | a->o_token | a->o_head;
+  const long strides = a->o_token | a->o_head;
   if (bases % 16 != 0 || strides % 8 != 0) UA_FAIL("ua_attn_paged: rows of q, o and the cache must start on 16 bytes");
-  const unsigned grid = static_cast<unsigned>((a->tokens * a->heads + 7) / 8);
-  UA_CUDA(launch_kernel(attn_paged_plain_kernel, grid, 256, 0, stream, true, *a, softmax_scale, status));
+  if (a->page_shift < 4 || a->page_shift > 24) UA_FAIL("ua_attn_paged: pages of 2^%ld tokens", a->page_shift);
+  if (!(softmax_scale > 0.f)) UA_FAIL("ua_attn_paged: the softmax scale must be positive");
+  const PagedPlan d = plan_paged(a);
+  const int ctas = sm_count();
+  PagedParams p;
+  memset(&p, 0, sizeof(p));
+  {
+    const uint64_t dims[3] = {PD, static_cast<uint64_t>(a->heads), static_cast<uint64_t>(a->tokens)};
+    const uint64_t str[2] = {stride_bytes(a->q_head, a->heads), stride_bytes(a->q_token, a->tokens)};
+    const uint32_t box[3] = {64, 1u << d.pack_shift, static_cast<uint32_t>(PT >> d.pack_shift)};
+    if (make_tmap_2byte(&p.tm_q, a->q, 3, dims, str, box)) return -1;
+  }
+  const long page_size = 1l << a->page_shift;
+  const uint64_t dims[4] = {PD, static_cast<uint64_t>(a->kv_heads), static_cast<uint64_t>(page_size), static_cast<uint64_t>(a->pages)};
+  const uint32_t box[4] = {64, 1, static_cast<uint32_t>(page_size < PT ? page_size : PT), 1};
+  const uint64_t ks[3] = {stride_bytes(a->k_head, a->kv_heads), stride_bytes(a->k_token, page_size), stride_bytes(a->k_page, a->pages)};
+  const uint64_t vs[3] = {stride_bytes(a->v_head, a->kv_heads), stride_bytes(a->v_token, page_size), stride_bytes(a->v_page, a->pages)};
+  if (make_tmap_2byte(&p.tm_k, a->k, 4, dims, ks, box) || make_tmap_2byte(&p.tm_v, a->v, 4, dims, vs, box)) return -1;
+  p.table = a->table;
+  p.table_stride = a->table_stride;
+  p.columns = static_cast<int>(a->columns);
+  p.pages = static_cast<int>(a->pages);
+  p.context = a->context;
+  p.cu_new = a->cu_new;
+  p.requests = static_cast<int>(a->requests);
+  p.tokens = static_cast<int>(a->tokens);
+  p.heads = static_cast<int>(a->heads);
+  p.kv_heads = static_cast<int>(a->kv_heads);
+  p.group = static_cast<int>(a->heads / a->kv_heads);
+  p.pack_shift = d.pack_shift;
+  p.page_shift = static_cast<int>(a->page_shift);
+  p.left = a->left < 0 ? -1 : a->left > 0x3FFFFFFF ? 0x3FFFFFFF : static_cast<int>(a->left);
+  p.sink = a->sink > 0x3FFFFFFF ? 0x3FFFFFFF : static_cast<int>(a->sink);
+  p.few_rows = d.few_limit;
+  p.other_form = d.few_rows > 0 && d.full_rows > 0;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.o = static_cast<__nv_bfloat16*>(a->o);
+  p.o_token = a->o_token;
+  p.o_head = a->o_head;
+  p.lse = a->lse;
+  p.lse_head = a->lse_head;
+  p.status = status;
+  for (int form = 0; form < 2; ++form) {
+    const int rows = form == 0 ? d.few_rows : d.full_rows;
+    if (rows == 0) continue;
+    p.part_rows = rows;
+    p.part_o = workspace;
+    p.part_lse = workspace + 2l * ctas * rows * PD;
+    p.part_desc = reinterpret_cast<int*>(p.part_lse + 2l * ctas * rows);
+    workspace += part_floats(rows, ctas);
+    if (form == 0 ? launch_paged<true>(p, ctas, stream) : launch_paged<false>(p, ctas, stream)) return -1;
+    const CombineParams c{p.part_o, p.part_lse, p.part_desc, rows, ctas, p.pack_shift, p.group, p.o, p.o_token, p.o_head, p.lse, p.lse_head};
+    UA_CUDA(launch_kernel(combine_parts_kernel, dim3(ctas, (rows + COMBINE_ROWS - 1) / COMBINE_ROWS), 256, 0, stream, true, c));
+  }
   return 0;
 }

@@ -291,11 +291,14 @@ def paged_attention(q, k_cache, v_cache, block_table, context_lens, cu_new, *, m
         o, lse = out
         if o.shape != q.shape or o.dtype != q.dtype or lse.shape != (H, T) or lse.dtype != torch.float32 or o.device != q.device or lse.device != q.device:
             raise ValueError("out is (o like q, lse [heads, tokens] fp32)")
+    scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"softmax_scale must be positive, not {softmax_scale}")
     most_new = T if most_new is None else min(int(most_new), T)
     if most_new < 0:
         raise ValueError("most_new must not be negative")
     if not q.is_cuda:
-        return paged_attention_reference(q, k_cache, v_cache, block_table, context_lens, cu_new, softmax_scale, (left, 0), sink_tokens, out)
+        return paged_attention_reference(q, k_cache, v_cache, block_table, context_lens, cu_new, scale, (left, 0), sink_tokens, out)
     if D != KERNEL_HEAD_DIM or q.dtype != torch.bfloat16:
         raise ValueError(f"the kernel takes bf16 heads of {KERNEL_HEAD_DIM} elements, not {q.dtype} of {D}")
     if page_size < 16:
@@ -311,12 +314,15 @@ def paged_attention(q, k_cache, v_cache, block_table, context_lens, cu_new, *, m
         o, lse = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(H, T, dtype=torch.float32, device=q.device)
     elif o.stride(2) != 1 or o.stride(0) % 8 or o.stride(1) % 8 or o.data_ptr() % 16 or (T > 1 and lse.stride(1) != 1):
         raise ValueError("the rows of o start on 16 bytes, the tokens of lse lie side by side")
-    scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
+    if H // hk > 128:
+        raise ValueError(f"at most 128 query heads share a key/value head, not {H // hk}")
     block = _ATTN.pack(q.data_ptr(), T, H, q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), pages, hk,
                        *k_cache.stride()[:3], *v_cache.stride()[:3], sh, block_table.data_ptr(), block_table.stride(0),
                        block_table.shape[1], context_lens.data_ptr(), cu_new.data_ptr(), n, most_new, left, int(sink_tokens),
                        o.data_ptr(), o.stride(0), o.stride(1), lse.data_ptr(), lse.stride(0))
     with _lib.on_device(q):
-        rc = _lib.load().ua_attn_paged(block, scale, status_buffer(q.device).data_ptr(), _lib.stream_of(q))
-    _lib.check(rc, "ua_attn_paged")
+        lib = _lib.load()
+        ws = torch.empty(lib.ua_attn_paged_workspace(block), dtype=torch.float32, device=q.device)
+        rc = lib.ua_attn_paged(block, scale, ws.data_ptr(), status_buffer(q.device).data_ptr(), _lib.stream_of(q))
+    _lib.check(rc, "ua_attn_paged", 2)
     return o, lse
