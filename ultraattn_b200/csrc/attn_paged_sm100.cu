@@ -31,8 +31,8 @@ constexpr int PA_REGS_LAUNCH = 168, PA_REGS_LOAD = 72, PA_REGS_SOFTMAX = 216;
 static_assert(2 * PA_REGS_SOFTMAX + PA_REGS_LOAD <= 3 * PA_REGS_LAUNCH, "setmaxnreg may only redistribute the launch-time pool");
 constexpr int PA_TILE_BYTES = PT * PD * 2;    // [2 d-halves][128 rows][128 B]
 // What the start and the end of an item cost, in key tiles of its form (a share's border is not put into them).
-template <bool FEW> constexpr int PA_ITEM_TILES = FEW ? 2 : 3;
-constexpr int PA_MIN_SHARE = 3;               // key tiles of a CTA at least, besides
+template <bool FEW> constexpr int PA_ITEM_TILES = FEW ? 3 : 3;
+constexpr int PA_MIN_SHARE = 2;               // key tiles of a CTA at least, besides
 
 struct PagedParams {
   CUtensorMap tm_q, tm_k, tm_v;
@@ -59,6 +59,7 @@ struct PagedParams {
   float* part_lse;           // [2 * CTAs][part_rows]
   int* part_desc;            // [CTAs][PA_DESC]
   int part_rows;
+  int two_q;                 // FEW: items of up to 64 rows, two of which have room (their product reads 128 rows all the same)
   int* status;
 };
 // What a CTA left behind: 0: the part of an item that begins here and goes on in the next CTA (1 / 0), its first token, first head and
@@ -85,10 +86,9 @@ struct __align__(1024) PagedSmem {
   uint8_t k[STAGES][PA_TILE_BYTES];
   uint8_t v[STAGES][PA_TILE_BYTES];
   uint8_t o_stage[FEW ? 1 : PA_SOFTMAX_WARPS][FEW ? 16 : 4096];
-  uint64_t q_full;
+  uint64_t q_full[2], q_empty[2];
   uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
   uint64_t s_full[2], p_full[2];
-  uint64_t q_empty;
   uint64_t s_free;           // the scores have been read into registers
   uint64_t pv_done[2];
   uint64_t item_full[2], item_empty[2];
@@ -103,7 +103,7 @@ struct __align__(1024) PagedSmem {
 };
 static_assert(sizeof(PagedSmem<false>) + 1024 <= 232448 && sizeof(PagedSmem<true>) + 1024 <= 232448, "a CTA may use 227 KB");
 
-__device__ __forceinline__ void paged_error(int* status, int where, int extra) {
+static __device__ __noinline__ void paged_error(int* status, int where, int extra) {
   if (atomicCAS(status, 0, UA_ERR_BAD_ARG) == 0) {
     status[1] = where;
     status[2] = static_cast<int>(blockIdx.x);
@@ -192,11 +192,13 @@ struct PagedWalk {
   long x0, x1;               // the share
   long s;                    // where the next item begins
   int r, head, tile;
+  int same;                  // a window: the weight of every item of the request (0: key tiles and PA_ITEM_TILES)
   PagedRequest<FEW> q;
 
   __device__ __forceinline__ void enter(const PagedParams& p) {
     while (r < p.requests) {
       q = paged_request<FEW>(p, r, false);
+      same = FEW || p.left < 0 ? 0 : static_cast<int>(q.weight(p, 1));
       if (q.row_tiles > 0) return;
       ++r;
     }
@@ -222,7 +224,7 @@ struct PagedWalk {
   __device__ __forceinline__ bool next(const PagedParams& p, PagedItem& it, int& part) {
     while (r < p.requests && s < x1) {
       const int total = q.tiles(p, tile, it);
-      const long w = q.weight(p, tile + 1) - q.weight(p, tile), e = s + w;
+      const long e = s + (same > 0 ? same : PA_ITEM_TILES<FEW> + total);
       const auto cut = [&](long x) -> int {
         const long t = x - s - PA_ITEM_TILES<FEW>;
         return x >= e || t > total ? total : t < 0 ? 0 : static_cast<int>(t);
@@ -388,6 +390,24 @@ __device__ __forceinline__ void paged_few_epilogue(const PagedParams& p, PagedSm
 __device__ __forceinline__ int paged_low(const PagedParams& p, int e, int pos) { return e == 0 || p.left < 0 ? 0 : max(0, pos - p.left); }
 __device__ __forceinline__ int paged_lim(const PagedParams& p, int e, int pos) { return e == 0 ? min(p.sink, pos - p.left) : pos + 1; }
 
+// The values of a tile that no row of the item sees, rows [0, lo) and [hi, 128), become zeros before its P is handed over: they may be
+// anything (places behind a request's last key, pages of others, pages that were not loaded), and P = 0 times NaN is one.
+static __device__ __noinline__ void clear_unseen(uint8_t* v, uint64_t* v_full, uint32_t parity, int lo, int hi, int thread, int threads,
+                                                 volatile int* abort_flag, int* status) {
+  const int a = min(max(lo, 0), PT), b = max(a, min(hi, PT)), dead = a + PT - b;
+  if (dead == 0) return;
+  const WaitCtx wc{abort_flag, status, 4000000000ull};
+  if (!mbar_wait_quiet(v_full, parity, wc)) report_error_call(abort_flag, status, UA_ERR_MBAR_TIMEOUT, 442, static_cast<int>(parity));
+  for (int i = thread; i < dead * 16; i += threads) {
+    const int x = i >> 4, r = x < a ? x : b + x - a;
+    *reinterpret_cast<uint4*>(v + ((i >> 3) & 1) * 16384 + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+}
+
+// A branch that is never taken, in front of the arithmetic behind an arrival that the other sub-tile waits for: see attn_fwd_sm100.cu.
+#define PIN if (__builtin_expect(cnt == 0xFFFFFFFFu, 0)) break;
+
 template <bool FEW>
 __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_constant__ PagedParams p) {
   constexpr int STAGES = PagedSmem<FEW>::STAGES;
@@ -399,8 +419,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
   const int act_warps = FEW ? (min(PT, p.part_rows) + 31) / 32 : 4;
 
   if (threadIdx.x == PA_TMA_WARP * 32) {
-    mbar_init(&s.q_full, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.q_full[i], 1);
+      mbar_init(&s.q_empty[i], 1);
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.p_full[i], act_warps);
       mbar_init(&s.pv_done[i], 1);
@@ -413,7 +434,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
       mbar_init(&s.v_full[i], 1);
       mbar_init(&s.v_empty[i], 1);
     }
-    mbar_init(&s.q_empty, 1);
     mbar_init(&s.s_free, act_warps);
     mbar_init(&s.stat_full, act_warps);
     mbar_init(&s.merged, act_warps);
@@ -452,7 +472,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
     total += s.sums[i];
   }
   // as many CTAs as have a share worth its start
-  const long most = total / (PA_ITEM_TILES<FEW> + PA_MIN_SHARE);
+  const long most = total / PA_MIN_SHARE;
   const int ctas = static_cast<int>(most < 1 ? 1 : most < gridDim.x ? most : gridDim.x);
   const int cta = blockIdx.x;
   const long x0 = total * cta / ctas, x1 = total * (cta + 1) / ctas;
@@ -495,75 +515,81 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
       const int boxes = 2 * (PT / box_rows);
       const int box = lane >> 1, half = lane & 1;
       const uint32_t box_bytes = static_cast<uint32_t>(box_rows) * 128;
+      const int q_boxes = FEW ? 2 : 4;
+      const uint32_t q_bytes = FEW && p.two_q ? PA_TILE_BYTES / 2 : q_boxes * (PA_TILE_BYTES / 2);
       int head_part[4] = {0, 0, 0, 0}, cont = 0;
       uint32_t j = 0, live = 0;
       bool ok = true;
+      PagedItem next;
+      int part = 0;
+      next.exists = walk.next(p, next, part);
       for (uint32_t n = 0; ok; ++n) {
-        PagedItem it;
-        int part = 0;
-        const bool got = walk.next(p, it, part);
         const uint32_t slot = n & 1;
         if (n >= 2 && !__all_sync(0xFFFFFFFFu, wait(&s.item_empty[slot], ((n - 2) >> 1) & 1, 403))) break;
-        it.exists = got;
-        it.slot = part == 0 ? -1 : 2 * cta + (part == 1);
-        if (got && part == 1) {
+        next.slot = part == 0 ? -1 : 2 * cta + (part == 1);
+        if (next.exists && part == 1) {
           head_part[0] = 1;
-          head_part[1] = it.q_row + it.tok0;
-          head_part[2] = it.kv_head * p.group;
-          head_part[3] = it.rows;
-        } else if (got && part > 1) {
+          head_part[1] = next.q_row + next.tok0;
+          head_part[2] = next.kv_head * p.group;
+          head_part[3] = next.rows;
+        } else if (next.exists && part > 1) {
           cont = part == 2 ? 1 : 2;
         }
         if (lane == 0) {
-          s.item[slot] = it;
+          s.item[slot] = next;
           mbar_arrive(&s.item_full[slot]);
         }
-        if (!got) break;
-        if (it.total == 0) continue;
-        // Q: the scores of the item before are complete
-        if (live > 0 && !__all_sync(0xFFFFFFFFu, wait(&s.q_empty, (live - 1) & 1, 402))) break;
-        ++live;
-        if (lane == 0) mbar_arrive_expect_tx(&s.q_full, (FEW ? 1 : 2) * PA_TILE_BYTES);
+        if (!next.exists) break;
         __syncwarp();
-        if (lane < (FEW ? 2 : 4)) {
-          const int w = lane >> 1;
-          tma_load_3d(s.q[w] + half * 16384, &p.tm_q, &s.q_full, half * 64, it.kv_head * p.group, it.q_row + it.tok0 + ((w * PT) >> psh));
-        }
+        const PagedItem& it = s.item[slot];
+        const int total = it.total, n0 = it.end[0] - it.first[0], f0 = it.first[0], f1 = it.first[1] - n0;
         const int* row = p.table + it.request * p.table_stride;
-        // this lane's page of tile t: its first key, and the entry (-1: the box is not loaded)
-        auto entry_of = [&](int e, int t) -> int {
-          if (lane >= boxes || t >= it.end[e]) return -1;
-          const int key = t * PT + box * box_rows;
-          if (key >= it.hi[e] || key + box_rows <= it.lo[e]) return -1;
+        // this lane's page of the item's tile i (-1: its box is not loaded)
+        auto entry_of = [&](int i) -> int {
+          const int e = i >= n0;
+          const int key = (i + (e ? f1 : f0)) * PT + box * box_rows;
+          if (lane >= boxes || i >= total || key >= it.hi[e] || key + box_rows <= it.lo[e]) return -1;
           const int col = key >> p.page_shift;
           const int page = col < p.columns ? row[col] : -1;
           if (page >= 0 && page < p.pages) return page;
           paged_error(p.status, 520, it.request);
           return -1;
         };
+        int page = entry_of(0);
 #pragma unroll 1
-        for (int e = 0; e < 2 && ok; ++e) {
-          int page = entry_of(e, it.first[e]);
-#pragma unroll 1
-          for (int t = it.first[e]; t < it.end[e]; ++t, ++j) {
-            const int next_page = entry_of(e, t + 1);
-            const int off = (t * PT + box * box_rows) & ((1 << p.page_shift) - 1);
-            const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, page >= 0)) * box_bytes;
-            const int st = j % STAGES;
-            const uint32_t ph = (j / STAGES) & 1;
-            ok = __all_sync(0xFFFFFFFFu, wait(&s.k_empty[st], ph ^ 1, 400));
+        for (int i = 0; i < total; ++i, ++j) {
+          const int next_page = entry_of(i + 1);
+          const int off = ((i + (i >= n0 ? f1 : f0)) * PT + box * box_rows) & ((1 << p.page_shift) - 1);
+          const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, page >= 0)) * box_bytes;
+          const int st = j % STAGES;
+          const uint32_t ph = (j / STAGES) & 1;
+          ok = __all_sync(0xFFFFFFFFu, wait(&s.k_empty[st], ph ^ 1, 400));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&s.k_full[st], bytes);
+          __syncwarp();
+          if (page >= 0) tma_load_4d(s.k[st] + half * 16384 + box * box_bytes, &p.tm_k, &s.k_full[st], half * 64, it.kv_head, off, page);
+          if (i == 0) {
+            // Q, behind the first keys: its room is free when the scores of the item before (of the one before that, where there are
+            // two) are complete, later than that of a key tile
+            const uint32_t qb = p.two_q ? live & 1 : 0, use = p.two_q ? live >> 1 : live;
+            ok = __all_sync(0xFFFFFFFFu, wait(&s.q_empty[qb], (use & 1) ^ 1, 402));
             if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(&s.k_full[st], bytes);
+            ++live;
+            if (lane == 0) mbar_arrive_expect_tx(&s.q_full[qb], q_bytes);
             __syncwarp();
-            if (page >= 0) tma_load_4d(s.k[st] + half * 16384 + box * box_bytes, &p.tm_k, &s.k_full[st], half * 64, it.kv_head, off, page);
-            ok = __all_sync(0xFFFFFFFFu, wait(&s.v_empty[st], ph ^ 1, 401));
-            if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(&s.v_full[st], bytes);
-            __syncwarp();
-            if (page >= 0) tma_load_4d(s.v[st] + half * 16384 + box * box_bytes, &p.tm_v, &s.v_full[st], half * 64, it.kv_head, off, page);
-            page = next_page;
+            if (lane < q_boxes)
+              tma_load_3d(s.q[0] + (lane >> 1) * PA_TILE_BYTES + half * 16384 + qb * (PA_TILE_BYTES / 4), &p.tm_q, &s.q_full[qb], half * 64,
+                          it.kv_head * p.group, it.q_row + it.tok0 + (((lane >> 1) * PT) >> psh));
           }
+          ok = __all_sync(0xFFFFFFFFu, wait(&s.v_empty[st], ph ^ 1, 401));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&s.v_full[st], bytes);
+          __syncwarp();
+          if (page >= 0) tma_load_4d(s.v[st] + half * 16384 + box * box_bytes, &p.tm_v, &s.v_full[st], half * 64, it.kv_head, off, page);
+          page = next_page;
+          if (i == 0) next.exists = walk.next(p, next, part);           // (while those are on their way)
         }
+        if (total == 0) next.exists = walk.next(p, next, part);
       }
       grid_trigger();
       if (lane == 0) {
@@ -580,8 +606,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
         const uint32_t v_desc = desc_lo(smem_u32(s.v[0]), 16384);
         constexpr uint32_t HI = desc_hi_sw128(1024);
         constexpr uint32_t TILE16 = PA_TILE_BYTES >> 4;
+        uint32_t q_buf = 0;
         auto issue_s = [&](int w, int st) {
-          const uint32_t qa = q_desc + (FEW ? 0 : w) * TILE16, ka = k_desc + st * TILE16;
+          const uint32_t qa = q_desc + (FEW ? q_buf * (TILE16 / 4) : w * TILE16), ka = k_desc + st * TILE16;
           const uint32_t tS = tmem_base + (FEW ? w * 128 : 0);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk) {
@@ -607,7 +634,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
           for (uint32_t n = 0; ok && item_there(n); ++n) {
             const int n_total = take_total(n);
             if (n_total == 0) continue;
-            if (!wait(&s.q_full, live & 1, 430)) break;
+            q_buf = p.two_q ? live & 1 : 0;
+            if (!wait(&s.q_full[q_buf], (p.two_q ? live >> 1 : live) & 1, 430)) break;
             auto next_s = [&](int i) -> bool {
               const uint32_t g = kv + i;
               if (!wait(&s.k_full[g % STAGES], (g / STAGES) & 1, 431)) return false;
@@ -615,7 +643,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
               issue_s(i & 1, g % STAGES);
               tc_commit(&s.s_full[i & 1]);
               tc_commit(&s.k_empty[g % STAGES]);
-              if (i + 1 == n_total) tc_commit(&s.q_empty);
+              if (i + 1 == n_total) tc_commit(&s.q_empty[q_buf]);
               return true;
             };
             ok = next_s(0) && (n_total < 2 || next_s(1));
@@ -646,14 +674,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
           for (uint32_t n = 0; ok && item_there(n); ++n) {
             const int n_total = take_total(n);
             if (n_total == 0) continue;
-            if (!wait(&s.q_full, live & 1, 430)) break;
+            if (!wait(&s.q_full[0], live & 1, 430)) break;
             for (int i = 0; i < n_total && ok; ++i, ++kv) {
               const int st = kv % STAGES;
               ok = wait(&s.k_full[st], (kv / STAGES) & 1, 431) && scores(0, st) && scores(1, st);
               if (ok) tc_commit(&s.k_empty[st]);
             }
             if (!ok) break;
-            tc_commit(&s.q_empty);
+            tc_commit(&s.q_empty[0]);
             ++live;
           }
         } else {
@@ -707,30 +735,20 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
             some_end = (max(0, paged_lim(p, e, last)) + PT - 1) >> 7;
             some_first = paged_low(p, e, first) >> 7;
             clear_first = (paged_low(p, e, last) + PT - 1) >> 7;
-            if (r_cta - lane >= it.rows) some_end = 0;
+            if (r_cta - lane >= it.rows) some_end = clear_end = 0;     // (rows behind the last one)
           }
 #pragma unroll 1
           for (; t < t_end; ++t, ++j) {
             if (FEW && (j & 1) != static_cast<uint32_t>(w)) continue;
+            // (of two sub-tiles the first does it: its product is issued before the other's; a tile with such keys is clear for no warp)
+            if ((FEW || w == 0) && (t < clear_first || t >= clear_end)) {
+              const uint32_t g = kv + j;
+              clear_unseen(s.v[g % STAGES], &s.v_full[g % STAGES], (g / STAGES) & 1, it.lo[e] - t * PT, it.hi[e] - t * PT, threadIdx.x - w * PT,
+                           act_warps * 32, wc.abort_flag, p.status);
+            }
             ok = mbar_wait_quiet(&s.s_full[w], cnt & 1, wc);
             ++cnt;
             tc_fence_after_sync();
-            // Values that no row of the item sees (behind the last key, before the first of a window, pages that were not loaded)
-            // may be anything, and P = 0 times NaN is one: they become zeros before the tile's P is handed over. (Of two sub-tiles the
-            // first does it: its product is issued before the other's.)
-            const int c0 = t * PT;
-            if ((FEW || w == 0) && (c0 < it.lo[e] || c0 + PT > it.hi[e])) {
-              const uint32_t g = kv + j;
-              const int st = g % STAGES;
-              ok = mbar_wait_quiet(&s.v_full[st], (g / STAGES) & 1, wc) && ok;
-              const int a = max(it.lo[e] - c0, 0), b = min(it.hi[e] - c0, PT);
-              const int dead = a + PT - b;
-              for (int i = threadIdx.x - w * PT; i < dead * 16; i += act_warps * 32) {
-                const int x = i >> 4, r = x < a ? x : b + x - a;
-                *reinterpret_cast<uint4*>(s.v[st] + ((i >> 3) & 1) * 16384 + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-              }
-              fence_proxy_async_smem();
-            }
             if (t < some_first || t >= some_end) {
               // nothing to see for these 32 rows: P = 0, maximum and sum stay
               if (!FEW) mbar_arrive_warp(&s.s_free);
@@ -758,9 +776,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
             if (!FEW) {
               tc_fence_before_sync();
               mbar_arrive_warp(&s.s_free);
+              PIN
             }
             if (t < clear_first || t >= clear_end) {
               const int pos = it.past + it.tok0;
+              const int c0 = t * PT;
               const int at = pos + (r_cta >> psh), first = pos + ((r_cta - lane) >> psh), last = pos + ((r_cta - lane + 31) >> psh);
               const int low = paged_low(p, e, at) - c0, lim = paged_lim(p, e, at) - c0;
               const int clear_lo = paged_low(p, e, last) - c0, clear_hi = paged_lim(p, e, first) - c0;
@@ -782,7 +802,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
 #pragma unroll
               for (int k = 0; k < 8; ++k) mx8[k] = fmax3(mx8[k], sv[i + k], sv[i + 8 + k]);
             float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]));
-            mx = fmax3(mx, mx8[6], mx8[7]) * p.scale_log2;
+            mx = fmax3(mx, mx8[6], mx8[7]);
+            PIN
+            mx *= p.scale_log2;
             const float m_new = fmaxf(m_use, mx);
             // P V of the tile before is complete: P may be overwritten, and O rescaled
             bool need = false;
@@ -832,6 +854,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
             tmem_wait_st();
             tc_fence_before_sync();
             mbar_arrive_warp(&s.p_full[w]);
+            PIN
             float ls4[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -1010,11 +1033,15 @@ extern "C" int ua_attn_paged(const UaPagedAttn* a, float softmax_scale, float* w
   const int ctas = sm_count();
   PagedParams p;
   memset(&p, 0, sizeof(p));
+  CUtensorMap tm_q[2];
   {
     const uint64_t dims[3] = {PD, static_cast<uint64_t>(a->heads), static_cast<uint64_t>(a->tokens)};
     const uint64_t str[2] = {stride_bytes(a->q_head, a->heads), stride_bytes(a->q_token, a->tokens)};
-    const uint32_t box[3] = {64, 1u << d.pack_shift, static_cast<uint32_t>(PT >> d.pack_shift)};
-    if (make_tmap_2byte(&p.tm_q, a->q, 3, dims, str, box)) return -1;
+    for (int form = 0; form < 2; ++form) {
+      const int rows = form == 0 && d.few_rows <= PT / 2 ? PT / 2 : PT;
+      const uint32_t box[3] = {64, 1u << d.pack_shift, static_cast<uint32_t>(rows >> d.pack_shift)};
+      if ((form == 0 ? d.few_rows : d.full_rows) > 0 && make_tmap_2byte(&tm_q[form], a->q, 3, dims, str, box)) return -1;
+    }
   }
   const long page_size = 1l << a->page_shift;
   const uint64_t dims[4] = {PD, static_cast<uint64_t>(a->kv_heads), static_cast<uint64_t>(page_size), static_cast<uint64_t>(a->pages)};
@@ -1050,6 +1077,8 @@ extern "C" int ua_attn_paged(const UaPagedAttn* a, float softmax_scale, float* w
     const int rows = form == 0 ? d.few_rows : d.full_rows;
     if (rows == 0) continue;
     p.part_rows = rows;
+    p.tm_q = tm_q[form];
+    p.two_q = form == 0 && rows <= PT / 2;
     p.part_o = workspace;
     p.part_lse = workspace + 2l * ctas * rows * PD;
     p.part_desc = reinterpret_cast<int*>(p.part_lse + 2l * ctas * rows);
