@@ -1,0 +1,398 @@
+// Attention over a paged cache for requests of at most 16 or 32 rows: decoding.
+//
+// With four rows a tile of 128 x 128 scores is a tile of 4 x 128, and its exponentials, taken by one warp whose lanes are rows, cost
+// 1024 clocks of the special-function unit for 28 idle lanes. So the products are turned around: S^T = K Q^T (128 keys x N rows) and
+// O^T += V^T P^T (128 head-dim elements x N rows), keys and values being the operands with 128 rows. A lane is a key, four warps
+// take N exponentials each, the maximum of a row is found only when a score is more than 2^8 above the one in use (one
+// vote of the four warps per tile), the row sums stay spread over the lanes until the item's end, and O^T is N columns of tensor
+// memory. Bound by reading the keys and values (64 KB a tile, three tiles in flight).
+//
+// Two groups of four warps take the key tiles in turn, each with its own S^T, P^T and O^T; one warp loads, one issues the products.
+#include "paged_attn.cuh"
+
+namespace ua {
+
+constexpr int PF_THREADS = 320;
+constexpr int PF_TMA_WARP = 8;
+constexpr int PF_MMA_WARP = 9;                // issues the products; owns the TMEM allocation
+
+template <int N>
+struct __align__(1024) FewSmem {
+  static constexpr int STAGES = 3;
+  // P^T of a group, [N rows][128 keys] bf16 without swizzle: core matrices of 8 rows x 8 keys (128 B), the row groups side by
+  // side and 16 bytes between the key groups, so that a warp's 32 keys of a row lie in different banks
+  static constexpr int P_KEYS8 = N * 16 + 16;
+  static constexpr int P_BYTES = 16 * P_KEYS8;
+  static constexpr int QS = N == 16 ? 2 : 1;  // items whose queries have room
+  uint8_t q[QS][N * PD * 2];                  // [2 d-halves][N rows][128 B]
+  uint8_t k[STAGES][PA_TILE_BYTES];
+  uint8_t v[STAGES][PA_TILE_BYTES];
+  uint8_t p[2][P_BYTES];                      // (at an item's end: a group's row sums by warp, and its maxima)
+  float mx[2][N][4];                          // a tile's maxima by warp
+  uint64_t q_full[2], q_empty[2];
+  uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
+  uint64_t s_full[2], p_full[2], pv_done[2];
+  uint64_t item_full[2], item_empty[2];
+  uint64_t stat_full, merged;
+  PagedItem item[2];
+  PagedScalars c;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(FewSmem<16>) + 1024 <= 232448 && sizeof(FewSmem<32>) + 1024 <= 232448, "a CTA may use 227 KB");
+
+// A barrier of the 128 threads of a group, and whether some thread's `x` holds.
+__device__ __forceinline__ bool group_any(int id, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(x)), "r"(id)
+      : "memory");
+  return r != 0;
+}
+template <int N>
+__device__ __forceinline__ void tmem_ld_n(uint32_t t, uint32_t (&r)[N]) {
+  if constexpr (N == 16) tmem_ld_x16(t, r);
+  else tmem_ld_x32(t, r);
+}
+
+// What `op` makes of every row's N x 32 values of a warp: lanes exchange halves of their rows until one has one row, row_of(lane) (of 16
+// rows a pair of lanes has the same). N + 1 exchanges instead of 5 N, and the results lie where a row is worked on further.
+template <int N>
+__device__ __forceinline__ int row_of(int lane) { return N == 16 ? lane >> 1 : lane; }
+template <int N, typename Op>
+__device__ __forceinline__ float reduce_rows(float (&v)[N], int lane, Op op) {
+#pragma unroll
+  for (int half = N / 2, bit = 16; half >= 1; half >>= 1, bit >>= 1) {
+    const bool up = lane & bit;
+#pragma unroll
+    for (int x = 0; x < half; ++x) {
+      const float give = up ? v[x] : v[x + half], keep = up ? v[x + half] : v[x];
+      v[x] = op(keep, __shfl_xor_sync(0xFFFFFFFFu, give, bit));
+    }
+  }
+  return N == 16 ? op(v[0], __shfl_xor_sync(0xFFFFFFFFu, v[0], 1)) : v[0];
+}
+
+constexpr float PF_UNSEEN = 1e30f;            // minus the maximum of a row that has seen no key: any score is above it
+
+template <int N>
+__global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __grid_constant__ PagedParams maps) {
+  using Smem = FewSmem<N>;
+  constexpr int STAGES = Smem::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x < sizeof(PagedScalars) / 4) reinterpret_cast<int*>(&s.c)[threadIdx.x] = reinterpret_cast<const int*>(&maps.c)[threadIdx.x];
+  const PagedScalars& p = s.c;
+
+  if (threadIdx.x == PF_TMA_WARP * 32) {
+    tma_prefetch_desc(&maps.tm_q);
+    tma_prefetch_desc(&maps.tm_k);
+    tma_prefetch_desc(&maps.tm_v);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.q_full[i], 1);
+      mbar_init(&s.q_empty[i], 1);
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], 4);
+      mbar_init(&s.pv_done[i], 1);
+      mbar_init(&s.item_full[i], 1);
+      mbar_init(&s.item_empty[i], 1 + 8);
+    }
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&s.k_full[i], 1);
+      mbar_init(&s.k_empty[i], 1);
+      mbar_init(&s.v_full[i], 1);
+      mbar_init(&s.v_empty[i], 1);
+    }
+    mbar_init(&s.stat_full, 8);
+    mbar_init(&s.merged, 4);
+    s.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == PF_MMA_WARP) {
+    tmem_alloc(&s.tmem_base, 128);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = s.tmem_base;            // S0 | S1 | O0 | O1, N columns each
+  grid_wait();
+  const int psh = p.pack_shift;
+
+  WaitCtx wc{&s.abort_flag, p.status, 4000000000ull};
+  auto wait = [&](uint64_t* bar, uint32_t parity, int where) -> bool {
+    if (mbar_wait_quiet(bar, parity, wc)) return true;
+    report_error_call(wc.abort_flag, wc.status, UA_ERR_MBAR_TIMEOUT, where, static_cast<int>(parity));
+    return false;
+  };
+  auto item_there = [&](uint32_t n) -> bool { return wait(&s.item_full[n & 1], (n >> 1) & 1, 450) && s.item[n & 1].exists != 0; };
+
+  if (warp == PF_TMA_WARP) {
+    paged_producer<N>(maps, s, wait, [&](const PagedItem& it, uint32_t live) -> bool {
+      const uint32_t qb = live % Smem::QS;
+      if (!__all_sync(0xFFFFFFFFu, wait(&s.q_empty[qb], ((live / Smem::QS) & 1) ^ 1, 451))) return false;
+      if (lane == 0) mbar_arrive_expect_tx(&s.q_full[qb], N * PD * 2);
+      __syncwarp();
+      if (lane < 2) tma_load_3d(s.q[qb] + lane * (N * 128), &maps.tm_q, &s.q_full[qb], lane * 64, it.kv_head * p.group, it.q_row + it.tok0);
+      return true;
+    });
+  } else if (warp == PF_MMA_WARP) {
+    if (elect_one()) {
+      const uint32_t idesc_s = make_idesc_bf16(128, N, 0, 0);      // S^T = K Q^T, both K-major
+      const uint32_t idesc_o = make_idesc_bf16(128, N, 1, 0);      // O^T += V^T P^T: V with its head dim side by side, P^T with its keys
+      constexpr uint32_t HI = desc_hi_sw128(1024), HI_P = desc_hi_noswz(128);
+      constexpr uint32_t TILE16 = PA_TILE_BYTES >> 4;
+      const uint32_t k_desc = desc_lo(smem_u32(s.k[0]), 16), v_desc = desc_lo(smem_u32(s.v[0]), 16384);
+      const uint32_t q_desc = desc_lo(smem_u32(s.q[0]), 16), p_desc = desc_lo(smem_u32(s.p[0]), Smem::P_KEYS8);
+      bool ok = true;
+      uint32_t kv = 0, live = 0, phase = 0;
+      for (uint32_t n = 0; ok && item_there(n); ++n) {
+        const int total = s.item[n & 1].total;
+        mbar_arrive(&s.item_empty[n & 1]);
+        if (total == 0) continue;
+        const uint32_t qb = live % Smem::QS;
+        if (!wait(&s.q_full[qb], (live / Smem::QS) & 1, 452)) break;
+        // key tile i belongs to group i & 1; its scores are issued two tiles ahead
+        auto scores = [&](int i) -> bool {
+          const uint32_t g = kv + i;
+          if (!wait(&s.k_full[g % STAGES], (g / STAGES) & 1, 453)) return false;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            umma_ss_lo<HI, HI>(tmem_base + (i & 1) * N, k_desc + (g % STAGES) * TILE16 + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+                               q_desc + ((qb * (N * 256) + (kk >> 2) * (N * 128) + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+          tc_commit(&s.s_full[i & 1]);
+          tc_commit(&s.k_empty[g % STAGES]);
+          if (i + 1 == total) tc_commit(&s.q_empty[qb]);
+          return true;
+        };
+        ok = scores(0) && (total < 2 || scores(1));
+        for (int i = 0; i < total && ok; ++i) {
+          const int w = i & 1, st = (kv + i) % STAGES;
+          ok = wait(&s.v_full[st], ((kv + i) / STAGES) & 1, 454) && wait(&s.p_full[w], (phase >> w) & 1, 455);
+          if (!ok) break;
+          phase ^= 1u << w;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)          // 16 keys: two of P's key groups
+            umma_ss_lo<HI, HI_P>(tmem_base + (2 + w) * N, v_desc + st * TILE16 + ((kk * 2048) >> 4),
+                                 p_desc + ((w * Smem::P_BYTES + kk * 2 * Smem::P_KEYS8) >> 4), idesc_o, (i >= 2 || kk > 0) ? 1u : 0u);
+          tc_commit(&s.pv_done[w]);
+          tc_commit(&s.v_empty[st]);
+          if (i + 2 < total) ok = scores(i + 2);
+        }
+        kv += total;
+        ++live;
+      }
+    }
+  } else {
+    // =============================== softmax + epilogue: a lane is a key, then a head-dim element ===============================
+    const int w = warp >> 2, quad = warp & 3;
+    const int key_lane = quad * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t tS = tmem_base + lane_base + w * N, tO = tmem_base + lane_base + (2 + w) * N;
+    uint8_t* const p_mine = s.p[w] + (key_lane >> 3) * Smem::P_KEYS8 + (key_lane & 7) * 2;
+    const float scale = p.scale_log2;
+    uint32_t cnt = 0;                        // tiles of this group so far
+    uint32_t kv = 0;                         // key tiles of this CTA so far
+    for (uint32_t n = 0; __all_sync(0xFFFFFFFFu, item_there(n)); ++n) {
+      const PagedItem& it = s.item[n & 1];
+      float nm[N], l[N];                     // minus a row's reference maximum in log2 units, this lane's share of its sum
+      float nm_lane = PF_UNSEEN;             // nm of row `lane`
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        nm[x] = PF_UNSEEN;
+        l[x] = 0.f;
+      }
+      bool ok = true, dead = false;          // (dead: a wait of some thread of the group gave up; all of them know)
+      uint32_t j = 0;
+      const int pos0 = it.past + it.tok0, pos1 = pos0 + ((it.rows - 1) >> psh);
+      const uint32_t cnt0 = cnt;
+#pragma unroll 1
+      for (int e = 0; e < 2 && !dead; ++e) {
+        // all rows see all of the tiles [clear_first, clear_end)
+        const int clear_end = max(0, paged_lim(p, e, pos0)) >> 7, clear_first = (paged_low(p, e, pos1) + PT - 1) >> 7;
+        const int t_end = it.end[e];
+#pragma unroll 1
+        for (int t = it.first[e]; t < t_end; ++t, ++j) {
+          if ((j & 1) != static_cast<uint32_t>(w)) continue;
+          const bool edge = t < clear_first || t >= clear_end;
+          if (edge) {
+            const uint32_t g = kv + j;
+            clear_unseen(s.v[g % STAGES], &s.v_full[g % STAGES], (g / STAGES) & 1, it.lo[e] - t * PT, it.hi[e] - t * PT, threadIdx.x & 127, 128,
+                         wc.abort_flag, p.status);
+          }
+          ok = mbar_wait_quiet(&s.s_full[w], cnt & 1, wc) && ok;
+          ++cnt;
+          tc_fence_after_sync();
+          float sv[N];
+          tmem_ld_n<N>(tS, reinterpret_cast<uint32_t(&)[N]>(sv));
+          tmem_wait_ld();
+          if (edge) {
+            const int key = t * PT + key_lane;
+            if (pos0 == pos1) {
+              if (key < paged_low(p, e, pos0) || key >= paged_lim(p, e, pos0)) {
+#pragma unroll
+                for (int x = 0; x < N; ++x) sv[x] = -INFINITY;
+              }
+            } else {
+#pragma unroll
+              for (int x = 0; x < N; ++x) {
+                const int pos = pos0 + (x >> psh);
+                sv[x] = key >= paged_low(p, e, pos) && key < paged_lim(p, e, pos) ? sv[x] : -INFINITY;
+              }
+            }
+          }
+          float top = -INFINITY;
+#pragma unroll
+          for (int x = 0; x < N; ++x) top = fmaxf(top, fmaf(sv[x], scale, nm[x]));
+          // (the wait that gave up takes the same way, so that all threads of the group go on together)
+          if (group_any(1 + w, top > 8.0f || !ok)) {
+            float v[N];
+#pragma unroll
+            for (int x = 0; x < N; ++x) v[x] = sv[x];
+            s.mx[w][row_of<N>(lane)][quad] = reduce_rows<N>(v, lane, [](float a, float b) { return fmaxf(a, b); });
+            dead = group_any(1 + w, !ok);
+            if (dead) break;
+            const bool have = cnt - cnt0 > 1;        // O^T holds something
+            if (have) {
+              ok = mbar_wait_quiet(&s.pv_done[w], cnt & 1, wc);
+              tc_fence_after_sync();
+            }
+            // lane x: row x
+            const float4 m4 = *reinterpret_cast<const float4*>(s.mx[w][lane & (N - 1)]);
+            const float m = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w)) * scale;
+            const float nm_new = m == -INFINITY ? nm_lane : fminf(nm_lane, -m);
+            if (have) {
+              const float alpha = nm_lane == PF_UNSEEN ? 1.f : fast_exp2(nm_new - nm_lane);       // (1: there is nothing to scale)
+#pragma unroll
+              for (int c = 0; c < N; c += 16) {
+                uint32_t ov[16];
+                tmem_ld_x16(tO + c, ov);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const float a = __shfl_sync(0xFFFFFFFFu, alpha, c + i);
+                  ov[i] = __float_as_uint(__uint_as_float(ov[i]) * a);
+                  l[c + i] *= a;
+                }
+                tmem_st_x16(tO + c, ov);
+              }
+              tmem_wait_st();
+            }
+            nm_lane = nm_new;
+#pragma unroll
+            for (int x = 0; x < N; ++x) nm[x] = __shfl_sync(0xFFFFFFFFu, nm_new, x);
+          }
+          if (cnt - cnt0 > 1) ok = mbar_wait_quiet(&s.pv_done[w], cnt & 1, wc) && ok;     // P may be overwritten
+#pragma unroll
+          for (int x = 0; x < N; ++x) {
+            const float f = fast_exp2(fmaf(sv[x], scale, nm[x]));
+            l[x] += f;
+            *reinterpret_cast<__nv_bfloat16*>(p_mine + (x >> 3) * 128 + (x & 7) * 16) = __float2bfloat16_rn(f);   // (an operand of P V; the sum takes it unrounded)
+          }
+          fence_proxy_async_smem();
+          tc_fence_before_sync();
+          mbar_arrive_warp(&s.p_full[w]);
+        }
+      }
+      // ---------------------------------- epilogue --------------------------------------------
+      kv += it.total;
+      ok = ok && !dead;
+      const bool any = it.total > w;
+      if (any && ok) ok = mbar_wait_quiet(&s.pv_done[w], (cnt & 1) ^ 1, wc);
+      tc_fence_after_sync();
+      float* const stat = reinterpret_cast<float*>(s.p[w]);        // [N][4] sums by warp, [N] maxima
+      const float l_row = reduce_rows<N>(l, lane, [](float a, float b) { return a + b; });
+      stat[row_of<N>(lane) * 4 + quad] = any ? l_row : 0.f;
+      if (quad == 0 && lane < N) stat[4 * N + lane] = any && nm_lane != PF_UNSEEN ? -nm_lane : -INFINITY;
+      tc_fence_before_sync();
+      mbar_arrive_warp(&s.stat_full);
+      if (w == 0) {
+        ok = mbar_wait_quiet(&s.stat_full, n & 1, wc) && ok;
+        tc_fence_after_sync();
+        float o0[N], o1[N];
+        tmem_ld_n<N>(tO, reinterpret_cast<uint32_t(&)[N]>(o0));
+        tmem_ld_n<N>(tO + N, reinterpret_cast<uint32_t(&)[N]>(o1));
+        tmem_wait_ld();
+        // Row `lane` of this lane: the factors of its two O, and where they go.
+        const bool part = it.slot >= 0;
+        const float *st0 = reinterpret_cast<const float*>(s.p[0]), *st1 = reinterpret_cast<const float*>(s.p[1]);
+        const int x = lane & (N - 1);
+        const float m0 = st0[4 * N + x], m1 = st1[4 * N + x], m = fmaxf(m0, m1);
+        const float4 a = *reinterpret_cast<const float4*>(st0 + 4 * x), b = *reinterpret_cast<const float4*>(st1 + 4 * x);
+        const float l0 = (a.x + a.y) + (a.z + a.w), l1 = (b.x + b.y) + (b.z + b.w);
+        const float a0 = fast_exp2(m0 - m), a1 = fast_exp2(m1 - m);
+        const bool in0 = m0 > -INFINITY, in1 = m1 > -INFINITY;
+        const float sum = (in0 || l0 != l0 ? a0 * l0 : 0.f) + (in1 || l1 != l1 ? a1 * l1 : 0.f);
+        const bool seen = sum > 0.f && m > -INFINITY;
+        const float lse = seen ? (m + __log2f(sum)) * 0.6931471805599453f : -INFINITY;
+        // (0: what tensor memory holds of a group without a key is not used)
+        const float inv = __fdividef(1.f, sum);
+        const float f0 = seen && in0 ? a0 * inv : 0.f, f1 = seen && in1 ? a1 * inv : 0.f;
+        long tok;
+        int head;
+        const bool valid = paged_row(p, it, x, tok, head) && lane < N;
+        const long prow = static_cast<long>(it.slot) * p.part_rows + x;
+        const unsigned rows = __ballot_sync(0xFFFFFFFFu, valid);
+        if (valid && quad == 0) {
+          if (part) p.part_lse[prow] = sum != sum ? sum : lse;           // (a NaN score: see combine_parts_kernel)
+          else p.lse[head * p.lse_head + tok] = lse;
+        }
+        const uintptr_t dst = part ? reinterpret_cast<uintptr_t>(p.part_o + prow * PD + key_lane - lane)
+                                   : reinterpret_cast<uintptr_t>(p.o + tok * p.o_token + head * p.o_head + key_lane - lane);
+#pragma unroll
+        for (int y = 0; y < N; ++y) {
+          if (!((rows >> y) & 1u)) continue;
+          const float g0 = __shfl_sync(0xFFFFFFFFu, f0, y), g1 = __shfl_sync(0xFFFFFFFFu, f1, y);
+          const uintptr_t to = __shfl_sync(0xFFFFFFFFu, static_cast<unsigned long long>(dst), y);
+          const float o = (g0 != 0.f ? o0[y] * g0 : 0.f) + (g1 != 0.f ? o1[y] * g1 : 0.f);
+          if (part) reinterpret_cast<float*>(to)[lane] = o;
+          else reinterpret_cast<__nv_bfloat16*>(to)[lane] = __float2bfloat16_rn(o);
+        }
+        tc_fence_before_sync();
+        mbar_arrive_warp(&s.merged);
+      }
+      ok = mbar_wait_quiet(&s.merged, n & 1, wc) && ok;            // (the sums, O and P are free for the next item)
+      if (!ok) report_error_call(wc.abort_flag, wc.status, UA_ERR_MBAR_TIMEOUT, 456 + w, static_cast<int>(j));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.item_empty[n & 1]);
+      if (!__all_sync(0xFFFFFFFFu, ok)) break;
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == PF_MMA_WARP) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 128);
+  }
+}
+
+template <int N>
+static int launch_few(const PagedParams& p, int ctas, cudaStream_t stream) {
+  static int smem_set[64] = {0};
+  const int smem_bytes = sizeof(FewSmem<N>) + 1024;
+  int dev = 0;
+  UA_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !smem_set[dev]) {
+    UA_CUDA(cudaFuncSetAttribute(attn_paged_few_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes));
+    if (dev < 64) smem_set[dev] = 1;
+  }
+  UA_CUDA(launch_kernel(attn_paged_few_kernel<N>, ctas, PF_THREADS, smem_bytes, stream, true, p));
+  return 0;
+}
+
+int launch_paged_few_rows(const PagedParams& p, int rows, int ctas, cudaStream_t stream) {
+  return rows == 16 ? launch_few<16>(p, ctas, stream) : launch_few<32>(p, ctas, stream);
+}
+
+}  // namespace ua

@@ -10,18 +10,11 @@
 // A row is a query head of a token: row x of an item is token x / G', head x % G' of the group of G heads that shares a key/value head,
 // G' the next power of two (rows of heads behind G are computed and not stored), so that a key is read once for its group.
 //
-// What is different: the work is found on the GPU. The lengths are in device memory, and every CTA (one per SM) sums the requests' key
-// tiles up, takes an equal share of the line of all (request, key/value head, row tile) items and walks it: no table to build, no host,
-// no waiting for the longest request. An item that a border cuts leaves fp32 parts behind, at most two per CTA, which
-// combine_parts merges in the order of the keys. Keys come page by page (a TMA box is a page, or 128 tokens of a larger one).
-#include "host_common.cuh"
-#include "paged_args.h"
-#include "ptx.cuh"
+// How the work is found and shared out, and the loads: paged_attn.cuh.
+#include "paged_attn.cuh"
 
 namespace ua {
 
-constexpr int PD = 128;                       // head dim
-constexpr int PT = 128;                       // tile edge
 constexpr int PA_SOFTMAX_WARPS = 8;
 constexpr int PA_TMA_WARP = 8;
 constexpr int PA_QK_WARP = 9;                 // issues S = Q K^T; owns the TMEM allocation
@@ -29,55 +22,6 @@ constexpr int PA_PV_WARP = 10;                // issues O += P V
 constexpr int PA_THREADS = 384;
 constexpr int PA_REGS_LAUNCH = 168, PA_REGS_LOAD = 72, PA_REGS_SOFTMAX = 216;
 static_assert(2 * PA_REGS_SOFTMAX + PA_REGS_LOAD <= 3 * PA_REGS_LAUNCH, "setmaxnreg may only redistribute the launch-time pool");
-constexpr int PA_TILE_BYTES = PT * PD * 2;    // [2 d-halves][128 rows][128 B]
-// What the start and the end of an item cost, in key tiles of its form (a share's border is not put into them).
-template <bool FEW> constexpr int PA_ITEM_TILES = FEW ? 3 : 3;
-constexpr int PA_MIN_SHARE = 2;               // key tiles of a CTA at least, besides
-
-struct PagedParams {
-  CUtensorMap tm_q, tm_k, tm_v;
-  const int* table;
-  long table_stride;
-  int columns;
-  int pages;
-  const int* context;
-  const int* cu_new;
-  int requests;
-  int tokens;
-  int heads, kv_heads, group;
-  int pack_shift;            // log2 of the rows of a token
-  int page_shift;
-  int left, sink;            // left < 0: no window
-  int few_rows;              // requests of up to so many rows belong to the FEW form
-  int other_form;            // the launch is one of two; else it has to take every request
-  float scale_log2;
-  __nv_bfloat16* o;
-  long o_token, o_head;
-  float* lse;
-  long lse_head;
-  float* part_o;             // [2 * CTAs][part_rows][128]
-  float* part_lse;           // [2 * CTAs][part_rows]
-  int* part_desc;            // [CTAs][PA_DESC]
-  int part_rows;
-  int two_q;                 // FEW: items of up to 64 rows, two of which have room (their product reads 128 rows all the same)
-  int* status;
-};
-// What a CTA left behind: 0: the part of an item that begins here and goes on in the next CTA (1 / 0), its first token, first head and
-// rows (1 - 3); 4: the part of one that began before (0 none, 1 goes on, 2 ends)
-constexpr int PA_DESC = 8;
-
-// A piece of an item: the key tiles that this CTA takes of it.
-struct PagedItem {
-  int exists, total;
-  int q_row;                 // row of q of the request's first new token
-  int tok0, rows;            // first token of the tile in the request, rows of the tile
-  int kv_head;
-  int past;                  // position of the request's first new token
-  int request;
-  int slot;                  // part to write, -1: the result
-  int first[2], end[2];      // key tiles: of the sinks, of the band
-  int lo[2], hi[2];          // keys that some row sees, of each
-};
 
 template <bool FEW>
 struct __align__(1024) PagedSmem {
@@ -94,183 +38,17 @@ struct __align__(1024) PagedSmem {
   uint64_t item_full[2], item_empty[2];
   uint64_t stat_full, merged;
   PagedItem item[2];
+  PagedScalars c;
   float2 stat[FEW ? PT : 1];
-  long sums[12];
-  long start_x;              // where in its request the CTA's share begins
-  int start_r;
   uint32_t tmem_base;
   int abort_flag;
 };
 static_assert(sizeof(PagedSmem<false>) + 1024 <= 232448 && sizeof(PagedSmem<true>) + 1024 <= 232448, "a CTA may use 227 KB");
 
-static __device__ __noinline__ void paged_error(int* status, int where, int extra) {
-  if (atomicCAS(status, 0, UA_ERR_BAD_ARG) == 0) {
-    status[1] = where;
-    status[2] = static_cast<int>(blockIdx.x);
-    status[3] = extra;
-  }
-}
-
-// ---- the line of all items ------------------------------------------------------------------------------------------------
-// Sum over i = 1 .. m of ceil((a + i) / 2^k)
-__device__ __forceinline__ long ceil_sum(long a, long m, int k) {
-  auto upto = [&](long n) {                    // sum of ceil(i / 2^k), i = 1 .. n
-    const long q = n >> k, r = n & ((1l << k) - 1);
-    return ((q * (q + 1) / 2) << k) + r * (q + 1);
-  };
-  return upto(a + m) - upto(a);
-}
-
-// A request as this form sees it.
-template <bool FEW>
-struct PagedRequest {
-  int n, past, q_row, row_tiles;     // row_tiles 0: nothing to do
-  // key tiles of the row tile that begins with token t0: [first, end) of sinks and band, and the keys of each that some row sees
-  __device__ __forceinline__ int tiles(const PagedParams& p, int tile, PagedItem& it) const {
-    const int tpt = (FEW ? PT : 2 * PT) >> p.pack_shift;
-    it.tok0 = tile * tpt;
-    const int toks = min(tpt, n - it.tok0);
-    it.rows = toks << p.pack_shift;
-    const int last = past + it.tok0 + toks - 1;                       // position of the last row; < 0: sees nothing
-    it.lo[0] = it.hi[0] = it.first[0] = it.end[0] = 0;
-    it.hi[1] = max(0, last + 1);
-    it.lo[1] = p.left < 0 ? 0 : max(0, past + it.tok0 - p.left);
-    if (p.left >= 0) {
-      it.hi[0] = max(0, min(p.sink, last - p.left));
-      it.end[0] = (it.hi[0] + PT - 1) / PT;
-    }
-    it.first[1] = it.lo[1] / PT;
-    it.end[1] = (it.hi[1] + PT - 1) / PT;
-    if (it.hi[1] == 0) it.first[1] = it.lo[1] = 0;
-    return it.end[0] + it.end[1] - it.first[1];
-  }
-  // weight of the first m row tiles of a key/value head: their key tiles and PA_ITEM_TILES each (a window: an upper bound that is
-  // the same for all; what a share's border means is settled per item, with its own number of tiles)
-  __device__ __forceinline__ long weight(const PagedParams& p, int m) const {
-    if (FEW) {
-      PagedItem it;
-      return m == 0 ? 0 : PA_ITEM_TILES<FEW> + tiles(p, 0, it);
-    }
-    const int tpt = 2 * PT >> p.pack_shift;
-    long w = static_cast<long>(m) * PA_ITEM_TILES<FEW>;
-    if (p.left >= 0) {
-      const int most = (max(past + n, 0) + PT - 1) / PT;
-      return w + static_cast<long>(m) * min(most, (p.left + tpt) / PT + 2 + (p.sink + PT - 1) / PT);
-    }
-    const int full = min(m, n / tpt);          // tiles whose rows are all there
-    if (full < m) w += (max(past + n, 0) + PT - 1) / PT;
-    if (past < 0) {                            // (more new tokens than the request has)
-      for (int i = 0; i < full; ++i) w += max(0, past + (i + 1) * tpt + PT - 1) / PT;
-    } else if (tpt < PT) {                     // sum of ceil((past + i tpt) / 128): tpt divides 128 ...
-      w += ceil_sum((past + tpt - 1) / tpt, full, p.pack_shift - 1);
-    } else {                                   // ... or is 128 or 256
-      w += static_cast<long>(full) * ((past + PT - 1) / PT) + (tpt / PT) * (static_cast<long>(full) * (full + 1) / 2);
-    }
-    return w;
-  }
-};
-
-template <bool FEW>
-__device__ __forceinline__ PagedRequest<FEW> paged_request(const PagedParams& p, int r, bool report) {
-  PagedRequest<FEW> q;
-  const int first = p.cu_new[r], next = p.cu_new[r + 1];
-  const int c = max(p.context[r], 0);
-  q.q_row = first;
-  q.n = next - first;
-  q.past = c - q.n;
-  const bool bad = first < 0 || next > p.tokens || q.n < 0;
-  const long rows = bad ? 0 : static_cast<long>(q.n) << p.pack_shift;
-  const bool mine = FEW ? rows <= p.few_rows : rows > p.few_rows;
-  if (report && (bad || (!mine && !p.other_form && rows > 0))) paged_error(p.status, bad ? 521 : 522, r);
-  q.row_tiles = bad || !mine ? 0 : static_cast<int>((rows + (FEW ? PT : 2 * PT) - 1) / (FEW ? PT : 2 * PT));
-  return q;
-}
-
-// This CTA's share [x0, x1) of the line, walked item by item.
-template <bool FEW>
-struct PagedWalk {
-  long x0, x1;               // the share
-  long s;                    // where the next item begins
-  int r, head, tile;
-  int same;                  // a window: the weight of every item of the request (0: key tiles and PA_ITEM_TILES)
-  PagedRequest<FEW> q;
-
-  __device__ __forceinline__ void enter(const PagedParams& p) {
-    while (r < p.requests) {
-      q = paged_request<FEW>(p, r, false);
-      same = FEW || p.left < 0 ? 0 : static_cast<int>(q.weight(p, 1));
-      if (q.row_tiles > 0) return;
-      ++r;
-    }
-  }
-  __device__ __forceinline__ void begin(const PagedParams& p, int r0, long in_request, long a, long b) {
-    x0 = a;
-    x1 = b;
-    r = r0;
-    enter(p);
-    const long per_head = q.weight(p, q.row_tiles);
-    head = static_cast<int>(in_request / per_head);
-    const long y = in_request - head * per_head;
-    int lo = 0, hi = q.row_tiles;             // last tile whose items begin at y or before
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (q.weight(p, mid) <= y) lo = mid;
-      else hi = mid;
-    }
-    tile = lo;
-    s = a - y + q.weight(p, lo);
-  }
-  // the next piece of this share; false: there is none. `part`: 0 whole item, 1 its beginning, 2 its middle, 3 its end
-  __device__ __forceinline__ bool next(const PagedParams& p, PagedItem& it, int& part) {
-    while (r < p.requests && s < x1) {
-      const int total = q.tiles(p, tile, it);
-      const long e = s + (same > 0 ? same : PA_ITEM_TILES<FEW> + total);
-      const auto cut = [&](long x) -> int {
-        const long t = x - s - PA_ITEM_TILES<FEW>;
-        return x >= e || t > total ? total : t < 0 ? 0 : static_cast<int>(t);
-      };
-      const int t0 = cut(x0), t1 = cut(x1);
-      const bool valid = t1 > t0 || (total == 0 && x0 < e && e <= x1);
-      it.q_row = q.q_row;
-      it.kv_head = head;
-      it.past = q.past;
-      it.request = r;
-      it.total = t1 - t0;
-      part = t0 > 0 ? (t1 < total ? 2 : 3) : (t1 < total ? 1 : 0);
-      // of the sinks' tiles and the band's behind them, those numbered t0 .. t1 - 1
-      const int n0 = it.end[0], f1 = it.first[1];
-      it.first[0] = min(t0, n0);
-      it.end[0] = min(t1, n0);
-      it.first[1] = f1 + max(t0 - n0, 0);
-      it.end[1] = f1 + max(t1 - n0, 0);
-      s = e;
-      if (++tile == q.row_tiles) {
-        tile = 0;
-        if (++head == p.kv_heads) {
-          head = 0;
-          ++r;
-          enter(p);
-        }
-      }
-      if (valid) return true;
-    }
-    return false;
-  }
-};
-
-// ---- outputs ----------------------------------------------------------------------------------------------------------------
-// Where row x of an item goes: token and head; false: nowhere.
-__device__ __forceinline__ bool paged_row(const PagedParams& p, const PagedItem& it, int x, long& tok, int& head) {
-  const int h = x & ((1 << p.pack_shift) - 1);
-  tok = static_cast<long>(it.q_row) + it.tok0 + (x >> p.pack_shift);
-  head = it.kv_head * p.group + h;
-  return x < it.rows && h < p.group;
-}
-
 // 256 rows: this thread's row (l: row sum, m: reference maximum in log2 units; any: its sub-tile has seen a key tile), turned around in
 // shared memory so that a store covers whole 128-byte blocks of rows.
 template <typename Ready>
-__device__ __forceinline__ void paged_epilogue(const PagedParams& p, PagedSmem<false>& s, const PagedItem& it, uint32_t tO, float l, float m, bool any,
+__device__ __forceinline__ void paged_epilogue(const PagedScalars& p, PagedSmem<false>& s, const PagedItem& it, uint32_t tO, float l, float m, bool any,
                                                Ready ready) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int w = warp >> 2, quad = warp & 3;
@@ -343,7 +121,7 @@ __device__ __forceinline__ void paged_epilogue(const PagedParams& p, PagedSmem<f
 }
 
 // Up to 128 rows, of whose key tiles each sub-tile has seen half: sub-tile 0's warps merge both O from tensor memory.
-__device__ __forceinline__ void paged_few_epilogue(const PagedParams& p, PagedSmem<true>& s, const PagedItem& it, uint32_t tO, float l0, float m0) {
+__device__ __forceinline__ void paged_few_epilogue(const PagedScalars& p, PagedSmem<true>& s, const PagedItem& it, uint32_t tO, float l0, float m0) {
   const int x = threadIdx.x;
   const float2 other = s.stat[x];
   const float m = fmaxf(m0, other.x);
@@ -386,39 +164,24 @@ __device__ __forceinline__ void paged_few_epilogue(const PagedParams& p, PagedSm
   }
 }
 
-// The columns [low, lim) of a tile row's keys that a token at position `pos` sees: of the sinks (e = 0) or of the band.
-__device__ __forceinline__ int paged_low(const PagedParams& p, int e, int pos) { return e == 0 || p.left < 0 ? 0 : max(0, pos - p.left); }
-__device__ __forceinline__ int paged_lim(const PagedParams& p, int e, int pos) { return e == 0 ? min(p.sink, pos - p.left) : pos + 1; }
-
-// The values of a tile that no row of the item sees, rows [0, lo) and [hi, 128), become zeros before its P is handed over: they may be
-// anything (places behind a request's last key, pages of others, pages that were not loaded), and P = 0 times NaN is one.
-static __device__ __noinline__ void clear_unseen(uint8_t* v, uint64_t* v_full, uint32_t parity, int lo, int hi, int thread, int threads,
-                                                 volatile int* abort_flag, int* status) {
-  const int a = min(max(lo, 0), PT), b = max(a, min(hi, PT)), dead = a + PT - b;
-  if (dead == 0) return;
-  const WaitCtx wc{abort_flag, status, 4000000000ull};
-  if (!mbar_wait_quiet(v_full, parity, wc)) report_error_call(abort_flag, status, UA_ERR_MBAR_TIMEOUT, 442, static_cast<int>(parity));
-  for (int i = thread; i < dead * 16; i += threads) {
-    const int x = i >> 4, r = x < a ? x : b + x - a;
-    *reinterpret_cast<uint4*>(v + ((i >> 3) & 1) * 16384 + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-  }
-  fence_proxy_async_smem();
-}
-
 // A branch that is never taken, in front of the arithmetic behind an arrival that the other sub-tile waits for: see attn_fwd_sm100.cu.
 #define PIN if (__builtin_expect(cnt == 0xFFFFFFFFu, 0)) break;
 
 template <bool FEW>
-__global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_constant__ PagedParams p) {
+__global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_constant__ PagedParams maps) {
   constexpr int STAGES = PagedSmem<FEW>::STAGES;
   extern __shared__ uint8_t smem_raw[];
   PagedSmem<FEW>& s = *reinterpret_cast<PagedSmem<FEW>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int psh = p.pack_shift;
+  if (threadIdx.x < sizeof(PagedScalars) / 4) reinterpret_cast<int*>(&s.c)[threadIdx.x] = reinterpret_cast<const int*>(&maps.c)[threadIdx.x];
+  const PagedScalars& p = s.c;
   // FEW: warps behind the last row that an item may have are idle
-  const int act_warps = FEW ? (min(PT, p.part_rows) + 31) / 32 : 4;
+  const int act_warps = FEW ? (min(PT, maps.c.part_rows) + 31) / 32 : 4;
 
   if (threadIdx.x == PA_TMA_WARP * 32) {
+    tma_prefetch_desc(&maps.tm_q);
+    tma_prefetch_desc(&maps.tm_k);
+    tma_prefetch_desc(&maps.tm_v);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.q_full[i], 1);
       mbar_init(&s.q_empty[i], 1);
@@ -444,53 +207,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
     tmem_alloc(&s.tmem_base, 512);
     tmem_relinquish();
   }
-  grid_wait();
-
-  // ---- the share of this CTA: sums of the requests' weights -------------------------------------------------------------------
-  const int per = (p.requests + PA_THREADS - 1) / PA_THREADS;
-  const int r0 = min(p.requests, static_cast<int>(threadIdx.x) * per), r1 = min(p.requests, r0 + per);
-  long mine = 0;
-  for (int r = r0; r < r1; ++r) {
-    const PagedRequest<FEW> q = paged_request<FEW>(p, r, blockIdx.x == 0);
-    if (q.row_tiles > 0) mine += p.kv_heads * q.weight(p, q.row_tiles);
-  }
-  long before = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long y = __shfl_up_sync(0xFFFFFFFFu, before, d);
-    if (lane >= d) before += y;
-  }
-  if (lane == 31) s.sums[warp] = before;
-  before -= mine;
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = s.tmem_base;
-  long total = 0;
-  for (int i = 0; i < PA_THREADS / 32; ++i) {
-    if (i < warp) before += s.sums[i];
-    total += s.sums[i];
-  }
-  // as many CTAs as have a share worth its start
-  const long most = total / PA_MIN_SHARE;
-  const int ctas = static_cast<int>(most < 1 ? 1 : most < gridDim.x ? most : gridDim.x);
-  const int cta = blockIdx.x;
-  const long x0 = total * cta / ctas, x1 = total * (cta + 1) / ctas;
-  const bool work = total > 0 && cta < ctas;
-  if (work && x0 >= before && x0 < before + mine) {
-    long at = before;
-    for (int r = r0; r < r1; ++r) {
-      const PagedRequest<FEW> q = paged_request<FEW>(p, r, false);
-      const long w = q.row_tiles > 0 ? p.kv_heads * q.weight(p, q.row_tiles) : 0;
-      if (x0 < at + w) {
-        s.start_r = r;
-        s.start_x = x0 - at;
-        break;
-      }
-      at += w;
-    }
-  }
-  __syncthreads();
+  grid_wait();
+  const int psh = p.pack_shift;
 
   WaitCtx wc{&s.abort_flag, p.status, 4000000000ull};
   auto wait = [&](uint64_t* bar, uint32_t parity, int where) -> bool {
@@ -501,102 +223,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
   // Consumers: item n is in its slot, and there is one (false: no more, or a wait gave up). They hand it back by an arrival on item_empty.
   auto item_there = [&](uint32_t n) -> bool { return wait(&s.item_full[n & 1], (n >> 1) & 1, 420) && s.item[n & 1].exists != 0; };
 
-  if (!work) {
-    if (threadIdx.x < PA_DESC) p.part_desc[cta * PA_DESC + threadIdx.x] = 0;
-    grid_trigger();
-  } else if (warp >= PA_SOFTMAX_WARPS) {
+  if (warp >= PA_SOFTMAX_WARPS) {
     reg_dealloc<PA_REGS_LOAD>();
     if (warp == PA_TMA_WARP) {
       // =============================== walker and TMA producer =================================
-      // All lanes walk; a lane issues the box of one page and d-half of a tile.
-      PagedWalk<FEW> walk;
-      walk.begin(p, s.start_r, s.start_x, x0, x1);
-      const int box_rows = p.page_shift < 7 ? 1 << p.page_shift : PT;
-      const int boxes = 2 * (PT / box_rows);
-      const int box = lane >> 1, half = lane & 1;
-      const uint32_t box_bytes = static_cast<uint32_t>(box_rows) * 128;
-      const int q_boxes = FEW ? 2 : 4;
-      const uint32_t q_bytes = FEW && p.two_q ? PA_TILE_BYTES / 2 : q_boxes * (PA_TILE_BYTES / 2);
-      int head_part[4] = {0, 0, 0, 0}, cont = 0;
-      uint32_t j = 0, live = 0;
-      bool ok = true;
-      PagedItem next;
-      int part = 0;
-      next.exists = walk.next(p, next, part);
-      for (uint32_t n = 0; ok; ++n) {
-        const uint32_t slot = n & 1;
-        if (n >= 2 && !__all_sync(0xFFFFFFFFu, wait(&s.item_empty[slot], ((n - 2) >> 1) & 1, 403))) break;
-        next.slot = part == 0 ? -1 : 2 * cta + (part == 1);
-        if (next.exists && part == 1) {
-          head_part[0] = 1;
-          head_part[1] = next.q_row + next.tok0;
-          head_part[2] = next.kv_head * p.group;
-          head_part[3] = next.rows;
-        } else if (next.exists && part > 1) {
-          cont = part == 2 ? 1 : 2;
-        }
-        if (lane == 0) {
-          s.item[slot] = next;
-          mbar_arrive(&s.item_full[slot]);
-        }
-        if (!next.exists) break;
+      const int boxes = FEW ? 2 : 4;
+      const uint32_t bytes = FEW && p.two_q ? PA_TILE_BYTES / 2 : boxes * (PA_TILE_BYTES / 2);
+      paged_producer<FEW ? PT : 2 * PT>(maps, s, wait, [&](const PagedItem& it, uint32_t live) -> bool {
+        const uint32_t qb = p.two_q ? live & 1 : 0, use = p.two_q ? live >> 1 : live;
+        if (!__all_sync(0xFFFFFFFFu, wait(&s.q_empty[qb], (use & 1) ^ 1, 402))) return false;
+        if (lane == 0) mbar_arrive_expect_tx(&s.q_full[qb], bytes);
         __syncwarp();
-        const PagedItem& it = s.item[slot];
-        const int total = it.total, n0 = it.end[0] - it.first[0], f0 = it.first[0], f1 = it.first[1] - n0;
-        const int* row = p.table + it.request * p.table_stride;
-        // this lane's page of the item's tile i (-1: its box is not loaded)
-        auto entry_of = [&](int i) -> int {
-          const int e = i >= n0;
-          const int key = (i + (e ? f1 : f0)) * PT + box * box_rows;
-          if (lane >= boxes || i >= total || key >= it.hi[e] || key + box_rows <= it.lo[e]) return -1;
-          const int col = key >> p.page_shift;
-          const int page = col < p.columns ? row[col] : -1;
-          if (page >= 0 && page < p.pages) return page;
-          paged_error(p.status, 520, it.request);
-          return -1;
-        };
-        int page = entry_of(0);
-#pragma unroll 1
-        for (int i = 0; i < total; ++i, ++j) {
-          const int next_page = entry_of(i + 1);
-          const int off = ((i + (i >= n0 ? f1 : f0)) * PT + box * box_rows) & ((1 << p.page_shift) - 1);
-          const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, page >= 0)) * box_bytes;
-          const int st = j % STAGES;
-          const uint32_t ph = (j / STAGES) & 1;
-          ok = __all_sync(0xFFFFFFFFu, wait(&s.k_empty[st], ph ^ 1, 400));
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&s.k_full[st], bytes);
-          __syncwarp();
-          if (page >= 0) tma_load_4d(s.k[st] + half * 16384 + box * box_bytes, &p.tm_k, &s.k_full[st], half * 64, it.kv_head, off, page);
-          if (i == 0) {
-            // Q, behind the first keys: its room is free when the scores of the item before (of the one before that, where there are
-            // two) are complete, later than that of a key tile
-            const uint32_t qb = p.two_q ? live & 1 : 0, use = p.two_q ? live >> 1 : live;
-            ok = __all_sync(0xFFFFFFFFu, wait(&s.q_empty[qb], (use & 1) ^ 1, 402));
-            if (!ok) break;
-            ++live;
-            if (lane == 0) mbar_arrive_expect_tx(&s.q_full[qb], q_bytes);
-            __syncwarp();
-            if (lane < q_boxes)
-              tma_load_3d(s.q[0] + (lane >> 1) * PA_TILE_BYTES + half * 16384 + qb * (PA_TILE_BYTES / 4), &p.tm_q, &s.q_full[qb], half * 64,
-                          it.kv_head * p.group, it.q_row + it.tok0 + (((lane >> 1) * PT) >> psh));
-          }
-          ok = __all_sync(0xFFFFFFFFu, wait(&s.v_empty[st], ph ^ 1, 401));
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&s.v_full[st], bytes);
-          __syncwarp();
-          if (page >= 0) tma_load_4d(s.v[st] + half * 16384 + box * box_bytes, &p.tm_v, &s.v_full[st], half * 64, it.kv_head, off, page);
-          page = next_page;
-          if (i == 0) next.exists = walk.next(p, next, part);           // (while those are on their way)
-        }
-        if (total == 0) next.exists = walk.next(p, next, part);
-      }
-      grid_trigger();
-      if (lane == 0) {
-        int* d = p.part_desc + cta * PA_DESC;
-        for (int i = 0; i < 4; ++i) d[i] = head_part[i];
-        d[4] = cont;
-      }
+        if (lane < boxes)
+          tma_load_3d(s.q[0] + (lane >> 1) * PA_TILE_BYTES + (lane & 1) * 16384 + qb * (PA_TILE_BYTES / 4), &maps.tm_q, &s.q_full[qb], (lane & 1) * 64,
+                      it.kv_head * p.group, it.q_row + it.tok0 + (((lane >> 1) * PT) >> psh));
+        return true;
+      });
     } else if (warp == PA_QK_WARP || (!FEW && warp == PA_PV_WARP)) {
       // =============================== MMA issuers ============================================
       if (elect_one()) {
@@ -714,7 +356,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
       const uint32_t tS = tmem_base + lane_base + (FEW ? w * 128 : 0);
       const uint32_t tP = FEW ? tS : tmem_base + lane_base + 128 + w * 64;
       const uint32_t tO = tmem_base + lane_base + 256 + w * 128;
-      const float NEG_INF = -INFINITY;
+      const float NEG_INF = -INFINITY, scale = p.scale_log2;
       uint32_t cnt = 0;                        // score tiles of this sub-tile so far
       uint32_t kv = 0;                         // key tiles of this CTA so far
       for (uint32_t n = 0; __all_sync(0xFFFFFFFFu, item_there(n)); ++n) {
@@ -804,7 +446,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
             float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]));
             mx = fmax3(mx, mx8[6], mx8[7]);
             PIN
-            mx *= p.scale_log2;
+            mx *= scale;
             const float m_new = fmaxf(m_use, mx);
             // P V of the tile before is complete: P may be overwritten, and O rescaled
             bool need = false;
@@ -833,7 +475,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
               }
             }
             const float m_eff = (m_use == NEG_INF) ? 0.f : m_use;
-            const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
+            const uint64_t sc2 = f2_pack(scale, scale);
             const uint64_t nm2 = f2_pack(-m_eff, -m_eff);
             uint64_t ls2[4];
 #pragma unroll
@@ -907,12 +549,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
 }
 
 // The parts of a cut item, in the order of its keys: O = sum_i w_i O_i with w_i = exp(lse_i - lse), fp32, one warp per row, 4 elements per
-// lane. Block x: the item that begins in CTA x and goes on behind it, if there is one.
+// lane. Block (x, y, z): rows 8 y .. of the item that begins in CTA x of launch z and goes on behind it, if there is one.
 struct CombineParams {
-  const float* part_o;
-  const float* part_lse;
-  const int* desc;
-  int part_rows, ctas;
+  const float* part_o[3];
+  const float* part_lse[3];
+  const int* desc[3];
+  int part_rows[3];
+  int ctas;
   int pack_shift, group;
   __nv_bfloat16* o;
   long o_token, o_head;
@@ -923,21 +566,30 @@ constexpr int COMBINE_ROWS = 8;        // rows of a block
 __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constant__ CombineParams p) {
   grid_wait();
   grid_trigger();
-  const int first = blockIdx.x, lane = threadIdx.x & 31;
-  const int* d = p.desc + first * PA_DESC;
+  const int first = blockIdx.x, z = blockIdx.z, lane = threadIdx.x & 31;
+  const int* desc = p.desc[z];
+  const float *part_o = p.part_o[z], *part_lse = p.part_lse[z];
+  const long part_rows = p.part_rows[z];
+  // its head, and how far it goes: up to the next CTA that does not say that its part goes on (one load for all)
   const int x = blockIdx.y * COMBINE_ROWS + (threadIdx.x >> 5);
-  if (d[0] == 0 || x >= d[3]) return;
+  const int* d = desc + first * PA_DESC;
+  const int d0 = d[0], token = d[1], head0 = d[2], rows = d[3];
+  const int ahead = first + 1 + lane < p.ctas ? desc[(first + 1 + lane) * PA_DESC + 4] : 0;
   const int h = x & ((1 << p.pack_shift) - 1);
-  if (h >= p.group) return;
-  // the slots of its parts: 2 first + 1, then 2 (first + 1), 2 (first + 2) .. up to the CTA in which it ends
+  if (d0 == 0 || x >= rows || h >= p.group) return;
+  unsigned ends = __ballot_sync(0xFFFFFFFFu, ahead != 1);
   int n = 1;
-  while (first + n < p.ctas && p.desc[(first + n) * PA_DESC + 4] == 1) ++n;
-  ++n;
+  while (ends == 0) {
+    n += 32;
+    ends = __ballot_sync(0xFFFFFFFFu, first + n + lane >= p.ctas || desc[(first + n + lane) * PA_DESC + 4] != 1);
+  }
+  n += __ffs(ends);
+  // the slots of its parts: 2 first + 1, then 2 (first + 1), 2 (first + 2) ..
   auto slot = [&](int i) -> long { return i == 0 ? 2 * first + 1 : 2 * (first + i); };
   float mx = -INFINITY;
   bool bad = false;                    // a NaN score: O = 0 and lse = -inf, as in an item that is not cut
   for (int i = lane; i < n; i += 32) {
-    const float y = p.part_lse[slot(i) * p.part_rows + x];
+    const float y = part_lse[slot(i) * part_rows + x];
     bad |= y != y;
     mx = fmaxf(mx, y);
   }
@@ -949,9 +601,9 @@ __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constan
   if (mx > -INFINITY) {
 #pragma unroll 4
     for (int i = 0; i < n; ++i) {
-      const long row = slot(i) * p.part_rows + x;
-      const float w = __expf(p.part_lse[row] - mx);
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + row * PD + lane * 4);
+      const long row = slot(i) * part_rows + x;
+      const float w = __expf(part_lse[row] - mx);
+      const float4 v = *reinterpret_cast<const float4*>(part_o + row * PD + lane * 4);
       tot += w;
       acc.x += w * v.x;
       acc.y += w * v.y;
@@ -960,8 +612,8 @@ __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constan
     }
   }
   const float inv = tot > 0.f ? 1.f / tot : 0.f;
-  const long tok = d[1] + (x >> p.pack_shift);
-  const int head = d[2] + h;
+  const long tok = token + (x >> p.pack_shift);
+  const int head = head0 + h;
   uint2 o;
   o.x = pack_bf16x2(acc.x * inv, acc.y * inv);
   o.y = pack_bf16x2(acc.z * inv, acc.w * inv);
@@ -970,25 +622,38 @@ __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constan
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
-// Which forms a call needs, and the rows of a part of each (0: not launched).
+// The launches of a call: the form (rows of an item), the requests that each takes by their rows, and the rows of its parts.
 struct PagedPlan {
-  int pack_shift, few_rows, full_rows, few_limit;
+  int pack_shift, n;
+  struct { int form, min_rows, max_rows, part_rows; } launch[3];
 };
 static PagedPlan plan_paged(const UaPagedAttn* a) {
   PagedPlan d{};
   const long group = a->heads / a->kv_heads;
   while ((1l << d.pack_shift) < group) ++d.pack_shift;
   const long most = a->most_new << d.pack_shift;
-  if (most <= PT) {
-    d.few_rows = static_cast<int>(most);
-    d.few_limit = d.few_rows;
-  } else {
-    d.full_rows = 2 * PT;
-    if (a->requests > 1) d.few_rows = d.few_limit = PT;
+  auto add = [&](int form, int min_rows, long max_rows) {
+    d.launch[d.n++] = {form, min_rows, static_cast<int>(max_rows < 0x7FFFFFFF ? max_rows : 0x7FFFFFFF),
+                       static_cast<int>(max_rows < form ? max_rows : form)};
+  };
+  if (most <= 32) {
+    add(most <= 16 ? 16 : 32, 0, most);
+    return d;
   }
+  // several requests: most of them may bring a token each
+  int below = 0;
+  if (a->requests > 1 && (1 << d.pack_shift) <= 32) {
+    below = (1 << d.pack_shift) <= 16 ? 16 : 32;
+    add(below, 0, below);
+  }
+  if (most <= PT || a->requests > 1) {
+    add(PT, below, most < PT ? most : PT);
+    below = PT;
+  }
+  if (most > PT) add(2 * PT, below, most);
   return d;
 }
-static long part_floats(int rows, int ctas) { return rows > 0 ? static_cast<long>(ctas) * (2l * rows * (PD + 1) + PA_DESC) : 0; }
+static long part_floats(int rows, int ctas) { return static_cast<long>(ctas) * (2l * rows * (PD + 1) + PA_DESC); }
 
 template <bool FEW>
 static int launch_paged(const PagedParams& p, int ctas, cudaStream_t stream) {
@@ -1015,7 +680,9 @@ using namespace ua;
 extern "C" long ua_attn_paged_workspace(const UaPagedAttn* a) {
   if (a->kv_heads <= 0 || a->heads % a->kv_heads != 0) return 0;
   const PagedPlan d = plan_paged(a);
-  return part_floats(d.few_rows, sm_count()) + part_floats(d.full_rows, sm_count());
+  long n = 0;
+  for (int i = 0; i < d.n; ++i) n += part_floats(d.launch[i].part_rows, sm_count());
+  return n;
 }
 
 extern "C" int ua_attn_paged(const UaPagedAttn* a, float softmax_scale, float* workspace, int* status, cudaStream_t stream) {
@@ -1033,59 +700,66 @@ extern "C" int ua_attn_paged(const UaPagedAttn* a, float softmax_scale, float* w
   const int ctas = sm_count();
   PagedParams p;
   memset(&p, 0, sizeof(p));
-  CUtensorMap tm_q[2];
-  {
-    const uint64_t dims[3] = {PD, static_cast<uint64_t>(a->heads), static_cast<uint64_t>(a->tokens)};
-    const uint64_t str[2] = {stride_bytes(a->q_head, a->heads), stride_bytes(a->q_token, a->tokens)};
-    for (int form = 0; form < 2; ++form) {
-      const int rows = form == 0 && d.few_rows <= PT / 2 ? PT / 2 : PT;
-      const uint32_t box[3] = {64, 1u << d.pack_shift, static_cast<uint32_t>(rows >> d.pack_shift)};
-      if ((form == 0 ? d.few_rows : d.full_rows) > 0 && make_tmap_2byte(&tm_q[form], a->q, 3, dims, str, box)) return -1;
-    }
-  }
   const long page_size = 1l << a->page_shift;
   const uint64_t dims[4] = {PD, static_cast<uint64_t>(a->kv_heads), static_cast<uint64_t>(page_size), static_cast<uint64_t>(a->pages)};
   const uint32_t box[4] = {64, 1, static_cast<uint32_t>(page_size < PT ? page_size : PT), 1};
   const uint64_t ks[3] = {stride_bytes(a->k_head, a->kv_heads), stride_bytes(a->k_token, page_size), stride_bytes(a->k_page, a->pages)};
   const uint64_t vs[3] = {stride_bytes(a->v_head, a->kv_heads), stride_bytes(a->v_token, page_size), stride_bytes(a->v_page, a->pages)};
   if (make_tmap_2byte(&p.tm_k, a->k, 4, dims, ks, box) || make_tmap_2byte(&p.tm_v, a->v, 4, dims, vs, box)) return -1;
-  p.table = a->table;
-  p.table_stride = a->table_stride;
-  p.columns = static_cast<int>(a->columns);
-  p.pages = static_cast<int>(a->pages);
-  p.context = a->context;
-  p.cu_new = a->cu_new;
-  p.requests = static_cast<int>(a->requests);
-  p.tokens = static_cast<int>(a->tokens);
-  p.heads = static_cast<int>(a->heads);
-  p.kv_heads = static_cast<int>(a->kv_heads);
-  p.group = static_cast<int>(a->heads / a->kv_heads);
-  p.pack_shift = d.pack_shift;
-  p.page_shift = static_cast<int>(a->page_shift);
-  p.left = a->left < 0 ? -1 : a->left > 0x3FFFFFFF ? 0x3FFFFFFF : static_cast<int>(a->left);
-  p.sink = a->sink > 0x3FFFFFFF ? 0x3FFFFFFF : static_cast<int>(a->sink);
-  p.few_rows = d.few_limit;
-  p.other_form = d.few_rows > 0 && d.full_rows > 0;
-  p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  p.o = static_cast<__nv_bfloat16*>(a->o);
-  p.o_token = a->o_token;
-  p.o_head = a->o_head;
-  p.lse = a->lse;
-  p.lse_head = a->lse_head;
-  p.status = status;
-  for (int form = 0; form < 2; ++form) {
-    const int rows = form == 0 ? d.few_rows : d.full_rows;
-    if (rows == 0) continue;
-    p.part_rows = rows;
-    p.tm_q = tm_q[form];
-    p.two_q = form == 0 && rows <= PT / 2;
-    p.part_o = workspace;
-    p.part_lse = workspace + 2l * ctas * rows * PD;
-    p.part_desc = reinterpret_cast<int*>(p.part_lse + 2l * ctas * rows);
-    workspace += part_floats(rows, ctas);
-    if (form == 0 ? launch_paged<true>(p, ctas, stream) : launch_paged<false>(p, ctas, stream)) return -1;
-    const CombineParams c{p.part_o, p.part_lse, p.part_desc, rows, ctas, p.pack_shift, p.group, p.o, p.o_token, p.o_head, p.lse, p.lse_head};
-    UA_CUDA(launch_kernel(combine_parts_kernel, dim3(ctas, (rows + COMBINE_ROWS - 1) / COMBINE_ROWS), 256, 0, stream, true, c));
+  p.c.table = a->table;
+  p.c.table_stride = a->table_stride;
+  p.c.columns = static_cast<int>(a->columns);
+  p.c.pages = static_cast<int>(a->pages);
+  p.c.context = a->context;
+  p.c.cu_new = a->cu_new;
+  p.c.requests = static_cast<int>(a->requests);
+  p.c.tokens = static_cast<int>(a->tokens);
+  p.c.heads = static_cast<int>(a->heads);
+  p.c.kv_heads = static_cast<int>(a->kv_heads);
+  p.c.group = static_cast<int>(a->heads / a->kv_heads);
+  p.c.pack_shift = d.pack_shift;
+  p.c.page_shift = static_cast<int>(a->page_shift);
+  p.c.left = a->left < 0 ? -1 : a->left > 0x3FFFFFFF ? 0x3FFFFFFF : static_cast<int>(a->left);
+  p.c.sink = a->sink > 0x3FFFFFFF ? 0x3FFFFFFF : static_cast<int>(a->sink);
+  p.c.most_rows = d.launch[d.n - 1].max_rows;
+  p.c.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.c.o = static_cast<__nv_bfloat16*>(a->o);
+  p.c.o_token = a->o_token;
+  p.c.o_head = a->o_head;
+  p.c.lse = a->lse;
+  p.c.lse_head = a->lse_head;
+  p.c.status = status;
+  CombineParams c;
+  memset(&c, 0, sizeof(c));
+  int most_part_rows = 0;
+  for (int i = 0; i < d.n; ++i) {
+    const auto& l = d.launch[i];
+    p.c.min_rows = l.min_rows;
+    p.c.max_rows = l.max_rows;
+    p.c.part_rows = l.part_rows;
+    p.c.two_q = l.form == PT && l.part_rows <= PT / 2;
+    const int box_rows = l.form < PT ? l.form : p.c.two_q ? PT / 2 : PT;
+    const uint64_t q_dims[3] = {PD, static_cast<uint64_t>(a->heads), static_cast<uint64_t>(a->tokens)};
+    const uint64_t q_str[2] = {stride_bytes(a->q_head, a->heads), stride_bytes(a->q_token, a->tokens)};
+    const uint32_t q_box[3] = {64, 1u << d.pack_shift, static_cast<uint32_t>(box_rows >> d.pack_shift)};
+    if (make_tmap_2byte(&p.tm_q, a->q, 3, q_dims, q_str, q_box)) return -1;
+    c.part_o[i] = p.c.part_o = workspace;
+    c.part_lse[i] = p.c.part_lse = workspace + 2l * ctas * l.part_rows * PD;
+    c.desc[i] = p.c.part_desc = reinterpret_cast<int*>(p.c.part_lse + 2l * ctas * l.part_rows);
+    c.part_rows[i] = l.part_rows;
+    workspace += part_floats(l.part_rows, ctas);
+    if (l.part_rows > most_part_rows) most_part_rows = l.part_rows;
+    if (l.form < PT ? launch_paged_few_rows(p, l.form, ctas, stream) : l.form == PT ? launch_paged<true>(p, ctas, stream) : launch_paged<false>(p, ctas, stream))
+      return -1;
   }
+  c.ctas = ctas;
+  c.pack_shift = p.c.pack_shift;
+  c.group = p.c.group;
+  c.o = p.c.o;
+  c.o_token = p.c.o_token;
+  c.o_head = p.c.o_head;
+  c.lse = p.c.lse;
+  c.lse_head = p.c.lse_head;
+  UA_CUDA(launch_kernel(combine_parts_kernel, dim3(ctas, (most_part_rows + COMBINE_ROWS - 1) / COMBINE_ROWS, d.n), 256, 0, stream, true, c));
   return 0;
 }

@@ -1,0 +1,434 @@
+// What the forms of attention over a paged cache share (attn_paged_sm100.cu, attn_paged_few_rows_sm100.cu): parameters, the line of all
+// work and a CTA's share of it, the loads.
+//
+// A row is a query head of a token: row x of an item is token x / G', head x % G' of the group of G heads that shares a key/value head, G'
+// the next power of two (rows of heads behind G are computed and not stored), so that a key is read once for its group. An item
+// is ROWS rows of a request and key/value head:
+//   16, 32   decoding and the like   (attn_paged_few_rows_sm100.cu)
+//   128      short chunks            (attn_paged_sm100.cu)
+//   256      the others
+// and every launch takes the requests with p.min_rows < rows <= p.max_rows.
+//
+// The work is found on the GPU. The lengths are in device memory, and every CTA (one per SM) sums the requests' key tiles up, takes an
+// equal share of the line of all items and walks it: no table to build, no host, no waiting for the longest request. An item that
+// a border cuts leaves fp32 parts behind, at most two per CTA, which combine_parts_kernel merges in the order of the keys.
+#pragma once
+#include "host_common.cuh"
+#include "paged_args.h"
+#include "ptx.cuh"
+
+namespace ua {
+
+constexpr int PD = 128;                       // head dim
+constexpr int PT = 128;                       // keys of a tile
+constexpr int PA_TILE_BYTES = PT * PD * 2;    // [2 d-halves][128 rows][128 B]
+// What the start and the end of an item cost, in key tiles of its form (a share's border is not put into them).
+template <int ROWS> constexpr int PA_ITEM_TILES = ROWS <= 32 ? 1 : 3;
+constexpr int PA_MIN_SHARE = 2;               // key tiles of a CTA at least
+
+// (Every block copies these into its shared memory before it waits for the kernel in front of it: parameters that have not been
+// touched for a while come through the constant cache with several hundred clocks a miss, one after the other.)
+struct PagedScalars {
+  const int* table;
+  long table_stride;
+  int columns;
+  int pages;
+  const int* context;
+  const int* cu_new;
+  int requests;
+  int tokens;
+  int heads, kv_heads, group;
+  int pack_shift;            // log2 of the rows of a token
+  int page_shift;
+  int left, sink;            // left < 0: no window
+  int min_rows, max_rows;    // the requests of this launch
+  int most_rows;             // no request may have more (in any launch of the call)
+  float scale_log2;
+  __nv_bfloat16* o;
+  long o_token, o_head;
+  float* lse;
+  long lse_head;
+  float* part_o;             // [2 * CTAs][part_rows][128]
+  float* part_lse;           // [2 * CTAs][part_rows]
+  int* part_desc;            // [CTAs][PA_DESC]
+  int part_rows;
+  int two_q;                 // ROWS 128: items of up to 64 rows, two of which have room (their product reads 128 rows all the same)
+  int* status;
+};
+struct PagedParams {
+  CUtensorMap tm_q, tm_k, tm_v;
+  PagedScalars c;
+};
+static_assert(sizeof(PagedScalars) % 4 == 0 && sizeof(PagedScalars) <= 64 * 4, "copied by 64 threads");
+// What a CTA left behind: 0: the part of an item that begins here and goes on in the next CTA (1 / 0), its first token, first head and
+// rows (1 - 3); 4: the part of one that began before (0 none, 1 goes on, 2 ends)
+constexpr int PA_DESC = 8;
+
+constexpr int PA_NO_PAGE = -0x7FFFFFFF;
+
+// A piece of an item: the key tiles that this CTA takes of it.
+struct PagedItem {
+  int exists, total;
+  int q_row;                 // row of q of the request's first new token
+  int tok0, rows;            // first token of the tile in the request, rows of the tile
+  int kv_head;
+  int past;                  // position of the request's first new token
+  int request;
+  int slot;                  // part to write, -1: the result
+  int first[2], end[2];      // key tiles: of the sinks, of the band
+  int lo[2], hi[2];          // keys that some row sees, of each
+};
+
+static __device__ __noinline__ void paged_error(int* status, int where, int extra) {
+  if (atomicCAS(status, 0, UA_ERR_BAD_ARG) == 0) {
+    status[1] = where;
+    status[2] = static_cast<int>(blockIdx.x);
+    status[3] = extra;
+  }
+}
+
+// ---- the line of all items ------------------------------------------------------------------------------------------------
+// Sum over i = 1 .. m of ceil((a + i) / 2^k)
+__device__ __forceinline__ long ceil_sum(long a, long m, int k) {
+  auto upto = [&](long n) {                    // sum of ceil(i / 2^k), i = 1 .. n
+    const long q = n >> k, r = n & ((1l << k) - 1);
+    return ((q * (q + 1) / 2) << k) + r * (q + 1);
+  };
+  return upto(a + m) - upto(a);
+}
+
+// A request as this form sees it.
+template <int ROWS>
+struct PagedRequest {
+  int n, past, q_row, row_tiles;     // row_tiles 0: nothing to do
+  // key tiles of the row tile that begins with token t0: [first, end) of sinks and band, and the keys of each that some row sees
+  __device__ __forceinline__ int tiles(const PagedScalars& p, int tile, PagedItem& it) const {
+    const int tpt = ROWS >> p.pack_shift;
+    it.tok0 = tile * tpt;
+    const int toks = min(tpt, n - it.tok0);
+    it.rows = toks << p.pack_shift;
+    const int last = past + it.tok0 + toks - 1;                       // position of the last row; < 0: sees nothing
+    it.lo[0] = it.hi[0] = it.first[0] = it.end[0] = 0;
+    it.hi[1] = max(0, last + 1);
+    it.lo[1] = p.left < 0 ? 0 : max(0, past + it.tok0 - p.left);
+    if (p.left >= 0) {
+      it.hi[0] = max(0, min(p.sink, last - p.left));
+      it.end[0] = (it.hi[0] + PT - 1) / PT;
+    }
+    it.first[1] = it.lo[1] / PT;
+    it.end[1] = (it.hi[1] + PT - 1) / PT;
+    if (it.hi[1] == 0) it.first[1] = it.lo[1] = 0;
+    return it.end[0] + it.end[1] - it.first[1];
+  }
+  // weight of the first m row tiles of a key/value head: their key tiles and PA_ITEM_TILES each (a window: an upper bound that is
+  // the same for all; what a share's border means is settled per item, with its own number of tiles)
+  __device__ __forceinline__ long weight(const PagedScalars& p, int m) const {
+    if (ROWS < 256) {
+      PagedItem it;
+      return m == 0 ? 0 : PA_ITEM_TILES<ROWS> + tiles(p, 0, it);
+    }
+    const int tpt = ROWS >> p.pack_shift;
+    long w = static_cast<long>(m) * PA_ITEM_TILES<ROWS>;
+    if (p.left >= 0) {
+      const int most = (max(past + n, 0) + PT - 1) / PT;
+      return w + static_cast<long>(m) * min(most, (p.left + tpt) / PT + 2 + (p.sink + PT - 1) / PT);
+    }
+    const int full = min(m, n / tpt);          // tiles whose rows are all there
+    if (full < m) w += (max(past + n, 0) + PT - 1) / PT;
+    if (past < 0) {                            // (more new tokens than the request has)
+      for (int i = 0; i < full; ++i) w += max(0, past + (i + 1) * tpt + PT - 1) / PT;
+    } else if (tpt < PT) {                     // sum of ceil((past + i tpt) / 128): tpt divides 128 ...
+      w += ceil_sum((past + tpt - 1) / tpt, full, p.pack_shift - 1);
+    } else {                                   // ... or is 128 or 256
+      w += static_cast<long>(full) * ((past + PT - 1) / PT) + (tpt / PT) * (static_cast<long>(full) * (full + 1) / 2);
+    }
+    return w;
+  }
+};
+
+template <int ROWS>
+__device__ __forceinline__ PagedRequest<ROWS> paged_request(const PagedScalars& p, int r, int first, int next, int context, bool report) {
+  PagedRequest<ROWS> q;
+  const int c = max(context, 0);
+  q.q_row = first;
+  q.n = next - first;
+  q.past = c - q.n;
+  const bool bad = first < 0 || next > p.tokens || q.n < 0;
+  const long rows = bad ? 0 : static_cast<long>(q.n) << p.pack_shift;
+  const bool mine = rows > p.min_rows && rows <= p.max_rows;
+  if (report && (bad || rows > p.most_rows)) paged_error(p.status, bad ? 521 : 522, r);
+  q.row_tiles = mine ? static_cast<int>((rows + ROWS - 1) / ROWS) : 0;
+  return q;
+}
+
+template <int ROWS>
+__device__ __forceinline__ PagedRequest<ROWS> paged_request(const PagedScalars& p, int r, bool report) {
+  return paged_request<ROWS>(p, r, p.cu_new[r], p.cu_new[r + 1], p.context[r], report);
+}
+
+// This CTA's share [x0, x1) of the line, walked item by item.
+template <int ROWS>
+struct PagedWalk {
+  long x0, x1;               // the share
+  long s;                    // where the next item begins
+  int r, head, tile;
+  int same;                  // a window: the weight of every item of the request (0: key tiles and PA_ITEM_TILES)
+  PagedRequest<ROWS> q;
+  int ahead[3];              // cu_new[r + 1], cu_new[r + 2], context[r + 1]: a request's lengths are loaded while the one before is walked
+
+  __device__ __forceinline__ void look_ahead(const PagedScalars& p) {
+    if (r + 1 >= p.requests) return;
+    ahead[0] = p.cu_new[r + 1];
+    ahead[1] = p.cu_new[r + 2];
+    ahead[2] = p.context[r + 1];
+  }
+  // the first request from r on with something to do
+  __device__ __forceinline__ void enter(const PagedScalars& p) {
+    while (r < p.requests) {
+      q = paged_request<ROWS>(p, r, ahead[0], ahead[1], ahead[2], false);
+      look_ahead(p);
+      same = ROWS < 256 || p.left < 0 ? 0 : static_cast<int>(q.weight(p, 1));
+      if (q.row_tiles > 0) return;
+      ++r;
+    }
+  }
+  // Finds the share of CTA `cta` of `ctas` (a whole warp; false: it has none). Few requests: one load each for a lane, so this is
+  // a load's latency and a sum over the warp.
+  __device__ __forceinline__ bool start(const PagedScalars& p, int cta, int all_ctas) {
+    const int lane = threadIdx.x & 31;
+    const int per = (p.requests + 31) / 32;
+    const int r0 = min(p.requests, lane * per), r1 = min(p.requests, r0 + per);
+    long mine = 0;
+    PagedRequest<ROWS> mine_last{};
+    for (int i = r0; i < r1; ++i) {
+      mine_last = paged_request<ROWS>(p, i, cta == 0);
+      if (mine_last.row_tiles > 0) mine += p.kv_heads * mine_last.weight(p, mine_last.row_tiles);
+    }
+    long before = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long y = __shfl_up_sync(0xFFFFFFFFu, before, d);
+      if (lane >= d) before += y;
+    }
+    const long total = __shfl_sync(0xFFFFFFFFu, before, 31);
+    before -= mine;
+    // as many CTAs as have a share worth its start
+    const long most = total / PA_MIN_SHARE;
+    const int ctas = static_cast<int>(most < 1 ? 1 : most < all_ctas ? most : all_ctas);
+    if (total == 0 || cta >= ctas) return false;
+    const auto border = [&](int k) -> long {            // total * k / ctas; (a 64-bit division is a hundred instructions)
+      if (total >> 32) return total * k / ctas;
+      const unsigned t = static_cast<unsigned>(total), d = t / ctas, rest = t % ctas;
+      return static_cast<long>(d) * k + rest * static_cast<unsigned>(k) / ctas;
+    };
+    x0 = border(cta);
+    x1 = border(cta + 1);
+    const bool here = x0 >= before && x0 < before + mine;
+    int found = r0;
+    long at = before;
+    if (here && per > 1)
+      for (int i = r0; i < r1; ++i) {
+        mine_last = paged_request<ROWS>(p, i, false);
+        const long w = mine_last.row_tiles > 0 ? p.kv_heads * mine_last.weight(p, mine_last.row_tiles) : 0;
+        found = i;
+        if (x0 < at + w) break;
+        at += w;
+      }
+    const int from = __ffs(__ballot_sync(0xFFFFFFFFu, here)) - 1;
+    r = __shfl_sync(0xFFFFFFFFu, found, from);
+    long y = x0 - __shfl_sync(0xFFFFFFFFu, at, from);    // where in the request
+    q = mine_last;
+    q.n = __shfl_sync(0xFFFFFFFFu, q.n, from);
+    q.past = __shfl_sync(0xFFFFFFFFu, q.past, from);
+    q.q_row = __shfl_sync(0xFFFFFFFFu, q.q_row, from);
+    q.row_tiles = __shfl_sync(0xFFFFFFFFu, q.row_tiles, from);
+    same = ROWS < 256 || p.left < 0 ? 0 : static_cast<int>(q.weight(p, 1));
+    look_ahead(p);
+    const long per_head = q.weight(p, q.row_tiles);
+    head = (y >> 32) == 0 ? static_cast<int>(static_cast<unsigned>(y) / static_cast<unsigned>(per_head)) : static_cast<int>(y / per_head);
+    y -= head * per_head;
+    int lo = 0, hi = q.row_tiles;             // last tile whose items begin at y or before
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (q.weight(p, mid) <= y) lo = mid;
+      else hi = mid;
+    }
+    tile = lo;
+    s = x0 - y + q.weight(p, lo);
+    return true;
+  }
+  // the next piece of this share; false: there is none. `part`: 0 whole item, 1 its beginning, 2 its middle, 3 its end
+  __device__ __forceinline__ bool next(const PagedScalars& p, PagedItem& it, int& part) {
+    while (r < p.requests && s < x1) {
+      const int total = q.tiles(p, tile, it);
+      const long e = s + (same > 0 ? same : PA_ITEM_TILES<ROWS> + total);
+      const auto cut = [&](long x) -> int {
+        const long t = x - s - PA_ITEM_TILES<ROWS>;
+        return x >= e || t > total ? total : t < 0 ? 0 : static_cast<int>(t);
+      };
+      const int t0 = cut(x0), t1 = cut(x1);
+      const bool valid = t1 > t0 || (total == 0 && x0 < e && e <= x1);
+      it.q_row = q.q_row;
+      it.kv_head = head;
+      it.past = q.past;
+      it.request = r;
+      it.total = t1 - t0;
+      part = t0 > 0 ? (t1 < total ? 2 : 3) : (t1 < total ? 1 : 0);
+      // of the sinks' tiles and the band's behind them, those numbered t0 .. t1 - 1
+      const int n0 = it.end[0], f1 = it.first[1];
+      it.first[0] = min(t0, n0);
+      it.end[0] = min(t1, n0);
+      it.first[1] = f1 + max(t0 - n0, 0);
+      it.end[1] = f1 + max(t1 - n0, 0);
+      s = e;
+      if (++tile == q.row_tiles) {
+        tile = 0;
+        if (++head == p.kv_heads) {
+          head = 0;
+          ++r;
+          enter(p);
+        }
+      }
+      if (valid) return true;
+    }
+    return false;
+  }
+};
+
+// ---- outputs ----------------------------------------------------------------------------------------------------------------
+// Where row x of an item goes: token and head; false: nowhere.
+__device__ __forceinline__ bool paged_row(const PagedScalars& p, const PagedItem& it, int x, long& tok, int& head) {
+  const int h = x & ((1 << p.pack_shift) - 1);
+  tok = static_cast<long>(it.q_row) + it.tok0 + (x >> p.pack_shift);
+  head = it.kv_head * p.group + h;
+  return x < it.rows && h < p.group;
+}
+
+// The columns [low, lim) of a tile row's keys that a token at position `pos` sees: of the sinks (e = 0) or of the band.
+__device__ __forceinline__ int paged_low(const PagedScalars& p, int e, int pos) { return e == 0 || p.left < 0 ? 0 : max(0, pos - p.left); }
+__device__ __forceinline__ int paged_lim(const PagedScalars& p, int e, int pos) { return e == 0 ? min(p.sink, pos - p.left) : pos + 1; }
+
+// The values of a tile that no row of the item sees, rows [0, lo) and [hi, 128), become zeros before its P is handed over: they may be
+// anything (places behind a request's last key, pages of others, pages that were not loaded), and P = 0 times NaN is one.
+static __device__ __noinline__ void clear_unseen(uint8_t* v, uint64_t* v_full, uint32_t parity, int lo, int hi, int thread, int threads,
+                                                 volatile int* abort_flag, int* status) {
+  const int a = min(max(lo, 0), PT), b = max(a, min(hi, PT)), dead = a + PT - b;
+  if (dead == 0) return;
+  const WaitCtx wc{abort_flag, status, 4000000000ull};
+  if (!mbar_wait_quiet(v_full, parity, wc)) report_error_call(abort_flag, status, UA_ERR_MBAR_TIMEOUT, 442, static_cast<int>(parity));
+  for (int i = thread; i < dead * 16; i += threads) {
+    const int x = i >> 4, r = x < a ? x : b + x - a;
+    *reinterpret_cast<uint4*>(v + ((i >> 3) & 1) * 16384 + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+}
+
+// The producer's warp: walks the share, hands the pieces over, and loads their keys and values page by page (a TMA box is a page, or
+// 128 tokens of a larger one; a lane issues the boxes of one page and d-half). All lanes walk. load_q(item, live) loads the queries
+// of the live-th item that has keys.
+template <int ROWS, typename Smem, typename Wait, typename LoadQ>
+__device__ __forceinline__ void paged_producer(const PagedParams& maps, Smem& s, Wait wait, LoadQ load_q) {
+  const PagedScalars& p = s.c;
+  constexpr int STAGES = Smem::STAGES;
+  const int lane = threadIdx.x & 31, cta = blockIdx.x;
+  PagedWalk<ROWS> walk;
+  const int box_rows = p.page_shift < 7 ? 1 << p.page_shift : PT;
+  const int boxes = PT / box_rows;          // pages of a tile: lane b holds the entry of page b
+  const uint32_t box_bytes = static_cast<uint32_t>(box_rows) * 128;
+  int begun = 0, begun_tok = 0, begun_head = 0, begun_rows = 0, cont = 0;
+  uint32_t j = 0, live = 0;
+  bool ok = true;
+  PagedItem next;
+  int part = 0;
+  // this lane's entry of tile i of an item (PA_NO_PAGE: not needed); it is looked at when the tile is loaded, a tile later
+  auto entry_of = [&](const PagedItem& it, int i) -> int {
+    const int n0 = it.end[0] - it.first[0];
+    const bool band = i >= n0;
+    const int key = (band ? it.first[1] + i - n0 : it.first[0] + i) * PT + lane * box_rows;
+    if (lane >= boxes || i >= it.total || key >= (band ? it.hi[1] : it.hi[0]) || key + box_rows <= (band ? it.lo[1] : it.lo[0])) return PA_NO_PAGE;
+    const int col = key >> p.page_shift;
+    return col < p.columns ? p.table[it.request * p.table_stride + col] : -1;
+  };
+  // A tile's boxes: up to eight pages in two d-halves. One thread issues them, one behind the other: 20 clocks each. (A box per lane: the
+  // lanes are taken one by one, 60 to 130 clocks each, and pages of 16 come at 0.6 of the memory's rate.)
+  auto load_tile = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, unsigned there, const int (&pages)[8], int head, int off) {
+    if (elect_one()) {
+      mbar_arrive_expect_tx(bar, __popc(there) * 2 * box_bytes);
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+        if ((there >> b) & 1u) {
+          tma_load_4d(dst + b * box_bytes, map, bar, 0, head, off, pages[b]);
+          tma_load_4d(dst + 16384 + b * box_bytes, map, bar, 64, head, off, pages[b]);
+        }
+    }
+    __syncwarp();
+  };
+  next.exists = walk.start(p, cta, gridDim.x) && walk.next(p, next, part);
+  int first_page = next.exists ? entry_of(next, 0) : PA_NO_PAGE;
+  for (uint32_t n = 0; ok; ++n) {
+    const uint32_t slot = n & 1;
+    if (n >= 2 && !__all_sync(0xFFFFFFFFu, wait(&s.item_empty[slot], ((n - 2) >> 1) & 1, 403))) break;
+    next.slot = part == 0 ? -1 : 2 * cta + (part == 1);
+    if (next.exists && part == 1) {
+      begun = 1;
+      begun_tok = next.q_row + next.tok0;
+      begun_head = next.kv_head * p.group;
+      begun_rows = next.rows;
+    } else if (next.exists && part > 1) {
+      cont = part == 2 ? 1 : 2;
+    }
+    if (lane == 0) {
+      s.item[slot] = next;
+      mbar_arrive(&s.item_full[slot]);
+    }
+    if (!next.exists) break;
+    __syncwarp();
+    const PagedItem& it = s.item[slot];
+    const int total = it.total, n0 = it.end[0] - it.first[0], f0 = it.first[0], f1 = it.first[1] - n0, head = it.kv_head;
+    int page = first_page;
+#pragma unroll 1
+    for (int i = 0; i < total; ++i, ++j) {
+      const int next_page = entry_of(it, i + 1);
+      const int off = ((i + (i >= n0 ? f1 : f0)) * PT) & ((1 << p.page_shift) - 1);       // (in a page of more than a tile)
+      const int st = j % STAGES;
+      const uint32_t ph = (j / STAGES) & 1;
+      ok = __all_sync(0xFFFFFFFFu, wait(&s.k_empty[st], ph ^ 1, 400));
+      if (!ok) break;
+      const unsigned there = __ballot_sync(0xFFFFFFFFu, page >= 0 && page < p.pages);
+      if (page != PA_NO_PAGE && !((there >> lane) & 1u)) paged_error(p.status, 520, it.request);
+      int pages[8];
+#pragma unroll
+      for (int b = 0; b < 8; ++b) pages[b] = __shfl_sync(0xFFFFFFFFu, page, b);
+      load_tile(s.k[st], &maps.tm_k, &s.k_full[st], there, pages, head, off);
+      if (i == 0) {
+        // Q, behind the first keys: its room is free when the scores of the item before (of the one before that, where there are
+        // two) are complete, later than that of a key tile
+        ok = load_q(it, live);
+        if (!ok) break;
+        ++live;
+      }
+      ok = __all_sync(0xFFFFFFFFu, wait(&s.v_empty[st], ph ^ 1, 401));
+      if (!ok) break;
+      load_tile(s.v[st], &maps.tm_v, &s.v_full[st], there, pages, head, off);
+      page = next_page;
+      if (i == 0) {                            // (while those are on their way)
+        next.exists = walk.next(p, next, part);
+        first_page = next.exists ? entry_of(next, 0) : PA_NO_PAGE;
+      }
+    }
+    if (total == 0) {
+      next.exists = walk.next(p, next, part);
+      first_page = next.exists ? entry_of(next, 0) : PA_NO_PAGE;
+    }
+  }
+  grid_trigger();
+  if (lane == 0) {
+    int* d = p.part_desc + cta * PA_DESC;
+    *reinterpret_cast<int4*>(d) = make_int4(begun, begun_tok, begun_head, begun_rows);
+    d[4] = cont;
+  }
+}
+
+int launch_paged_few_rows(const PagedParams& p, int rows, int ctas, cudaStream_t stream);       // attn_paged_few_rows_sm100.cu
+
+}  // namespace ua
