@@ -143,6 +143,7 @@ def host():
             address = lambda name: ctypes.cast(getattr(lib, name), c_void_p).value
             mod.init(address("ua_attn_fwd_dense_parts"), address("ua_attn_fwd_dense"), address("ua_attn_bwd_local"),
                      address("ua_last_error"))
+            mod.init_paged(*map(address, ("ua_rotary", "ua_attn_paged_workspace", "ua_attn_paged", "ua_assign_pages", "ua_release_pages")))
         _host.append(mod)
     return _host[0]
 

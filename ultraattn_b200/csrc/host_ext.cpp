@@ -11,6 +11,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include "arg_blocks.h"
+#include "paged_args.h"
 
 namespace {
 
@@ -18,6 +19,19 @@ int (*fwd_dense_parts)(int, int, int, int, int, int, int);
 int (*fwd_dense)(const UaDenseFwd*, int, float, int, float*, int*, void*);
 int (*bwd_local)(const UaLocalBwd*, float, int*, void*);
 const char* (*last_error)();
+int (*rotary_launch)(const UaRotary*, float, int*, void*);
+long (*paged_workspace)(const UaPagedAttn*);
+int (*paged_attn)(const UaPagedAttn*, float, float*, int*, void*);
+int (*pages_assign)(const int*, const int*, int, int*, long, int, const int*, int, const int*, int*, int, int, int*, int*, int*, int*, void*);
+int (*pages_release)(const unsigned char*, const int*, int, const int*, long, int, int*, int, const int*, int*, int, int*, void*);
+
+void init_paged(uintptr_t rotary, uintptr_t workspace, uintptr_t attn, uintptr_t assign, uintptr_t release) {
+  rotary_launch = reinterpret_cast<decltype(rotary_launch)>(rotary);
+  paged_workspace = reinterpret_cast<decltype(paged_workspace)>(workspace);
+  paged_attn = reinterpret_cast<decltype(paged_attn)>(attn);
+  pages_assign = reinterpret_cast<decltype(pages_assign)>(assign);
+  pages_release = reinterpret_cast<decltype(pages_release)>(release);
+}
 
 void init(uintptr_t parts, uintptr_t dense, uintptr_t local, uintptr_t error) {
   fwd_dense_parts = reinterpret_cast<decltype(fwd_dense_parts)>(parts);
@@ -94,9 +108,186 @@ py::object local_backward(const at::Tensor& q, const at::Tensor& k, const at::Te
   return py::make_tuple(dq, dk, dv);
 }
 
+// ---- rotary embedding and paged cache: the calls of ops/rotary.py and ops/paged.py whose arguments are the usual ones. Whatever is not
+// (other types or layouts, wrong shapes) is left to Python, which refuses it or lays it out first.
+using at::Tensor;
+
+bool is_int(const Tensor& t, const at::Device& dev, int64_t n) {       // n int32 side by side
+  return t.scalar_type() == at::kInt && t.device() == dev && t.dim() == 1 && t.size(0) == n && (n < 2 || t.stride(0) == 1);
+}
+bool is_table(const Tensor& t, const at::Device& dev) {
+  return t.scalar_type() == at::kInt && t.device() == dev && t.dim() == 2 && (t.size(1) < 2 || t.stride(1) == 1);
+}
+int log2_of(int64_t n) {                                               // -1: no power of two
+  if (n < 1 || (n & (n - 1)) != 0) return -1;
+  int s = 0;
+  while ((int64_t{1} << s) < n) ++s;
+  return s;
+}
+int* i32(const Tensor& t) { return static_cast<int*>(t.data_ptr()); }
+void* stream_ptr(uintptr_t s) { return reinterpret_cast<void*>(s); }
+int rotary_type(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? 0 : t.scalar_type() == at::kHalf ? 1 : t.scalar_type() == at::kFloat ? 2 : -1; }
+
+// [tokens, heads, dim] or [batch, tokens, heads, dim]
+UaRotPart rot_part(const Tensor& src, const Tensor& dst, bool rotate, bool paged) {
+  const int64_t k = src.dim() - 3, kd = dst.dim() - 3;
+  return UaRotPart{src.data_ptr(), dst.data_ptr(), src.size(k + 1), rotate, paged, k ? src.stride(0) : 0, src.stride(k), src.stride(k + 1),
+                   kd ? dst.stride(0) : 0, dst.stride(kd), dst.stride(kd + 1)};
+}
+bool angles_fit(const Tensor& x, const Tensor& pos, const Tensor& inv_freq) {
+  const int64_t k = x.dim() - 3;
+  return inv_freq.scalar_type() == at::kDouble && inv_freq.dim() == 1 && (inv_freq.size(0) < 2 || inv_freq.stride(0) == 1) &&
+         2 * inv_freq.size(0) <= x.size(k + 2) && inv_freq.size(0) <= 256 && inv_freq.device() == x.device() && pos.device() == x.device() &&
+         (pos.scalar_type() == at::kInt || pos.scalar_type() == at::kLong) && pos.dim() == k + 1 && pos.size(0) == x.size(0) &&
+         (k == 0 || pos.size(1) == x.size(1));
+}
+void rotary_common(UaRotary& a, const Tensor& like, const Tensor& pos, const Tensor* inv_freq, bool interleaved, bool inverse) {
+  const int64_t k = like.dim() - 3;
+  a.batch = k ? like.size(0) : 1;
+  a.per_batch = like.size(k);
+  a.pos = pos.data_ptr();
+  a.pos64 = pos.scalar_type() == at::kLong;
+  a.pos_batch = k ? pos.stride(0) : 0;
+  a.pos_token = pos.stride(k);
+  a.inv_freq = inv_freq ? static_cast<const double*>(inv_freq->data_ptr()) : nullptr;
+  a.pairs = inv_freq ? inv_freq->size(0) : 0;
+  a.dim = like.size(k + 2);
+  a.interleaved = interleaved;
+  a.inverse = inverse;
+  a.dtype = rotary_type(like);
+}
+
+// (q', k') in new tensors
+py::object rotate_pair(const Tensor& q, const Tensor& k, const Tensor& pos, const Tensor& inv_freq, bool interleaved, double magnitude,
+                       bool inverse, uintptr_t status, uintptr_t stream) {
+  const int64_t d = q.dim() - 1;
+  if (!q.is_cuda() || d < 2 || d > 3 || k.dim() != d + 1 || rotary_type(q) < 0 || k.scalar_type() != q.scalar_type() || k.device() != q.device() ||
+      q.stride(d) != 1 || k.stride(d) != 1 || q.size(d) != k.size(d) || q.numel() == 0 || k.numel() == 0 || q.size(0) != k.size(0) ||
+      (d == 3 && q.size(1) != k.size(1)) || !angles_fit(q, pos, inv_freq))
+    return py::none();
+  const Tensor q2 = at::empty(q.sizes(), q.options()), k2 = at::empty(k.sizes(), k.options());
+  UaRotary a{};
+  a.part[0] = rot_part(q, q2, true, false);
+  a.part[1] = rot_part(k, k2, true, false);
+  a.n_parts = 2;
+  rotary_common(a, q, pos, &inv_freq, interleaved, inverse);
+  {
+    py::gil_scoped_release nogil;
+    check(rotary_launch(&a, static_cast<float>(magnitude), reinterpret_cast<int*>(status), stream_ptr(stream)), "ua_rotary");
+  }
+  return py::make_tuple(q2, k2);
+}
+
+// q' in a new tensor; the cache is written
+py::object rotary_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& pos, const Tensor& slots, const Tensor& k_cache,
+                         const Tensor& v_cache, const Tensor& inv_freq, bool interleaved, double magnitude, uintptr_t status, uintptr_t stream) {
+  const at::Device dev = q.device();
+  if (!dev.is_cuda() || q.dim() != 3 || k.dim() != 3 || v.dim() != 3 || k_cache.dim() != 4 || v_cache.dim() != 4) return py::none();
+  const int64_t T = q.size(0), dim = q.size(2), sh = log2_of(k_cache.size(1));
+  for (const Tensor* t : {&k, &v, &k_cache, &v_cache})
+    if (t->scalar_type() != q.scalar_type() || t->device() != dev || t->size(t->dim() - 1) != dim || t->stride(t->dim() - 1) != 1) return py::none();
+  if (T == 0 || rotary_type(q) < 0 || sh < 0 || q.stride(2) != 1 || k.sizes() != v.sizes() || k.size(0) != T || k_cache.sizes() != v_cache.sizes() ||
+      k_cache.size(2) != k.size(1) || !is_int(slots, dev, T) || pos.dim() != 1 || !angles_fit(q, pos, inv_freq))
+    return py::none();
+  const Tensor out = at::empty(q.sizes(), q.options());
+  UaRotary a{};
+  a.part[0] = rot_part(q, out, true, false);
+  a.part[1] = rot_part(k, k_cache, true, true);
+  a.part[2] = rot_part(v, v_cache, false, true);
+  a.n_parts = 3;
+  rotary_common(a, q, pos, &inv_freq, interleaved, false);
+  a.slots = i32(slots);
+  a.page_shift = sh;
+  a.n_slots = k_cache.size(0) << sh;
+  {
+    py::gil_scoped_release nogil;
+    check(rotary_launch(&a, static_cast<float>(magnitude), reinterpret_cast<int*>(status), stream_ptr(stream)), "ua_rotary");
+  }
+  return py::cast(out);
+}
+
+// (cu_new, pos, slots, pages left)
+py::object assign_pages(const Tensor& context, const Tensor& fresh, const Tensor& table, const Tensor& free_pages, const Tensor& count,
+                        int64_t page_size, int64_t tokens, const c10::optional<Tensor>& count_out, int64_t most_requests, uintptr_t status,
+                        uintptr_t stream) {
+  const at::Device dev = table.device();
+  const int sh = log2_of(page_size);
+  const int64_t n = table.dim() == 2 ? table.size(0) : -1;
+  if (!dev.is_cuda() || sh < 0 || tokens < 0 || n < 0 || n > most_requests || !is_table(table, dev) || !is_int(context, dev, n) || !is_int(fresh, dev, n) ||
+      free_pages.dim() != 1 || !is_int(free_pages, dev, free_pages.size(0)) || !is_int(count, dev, 1) || (count_out && !is_int(*count_out, dev, 1)))
+    return py::none();
+  const auto opt = table.options();
+  const Tensor cu = at::empty({n + 1}, opt), pos = at::empty({tokens}, opt), slots = at::empty({tokens}, opt);
+  const Tensor left = count_out ? *count_out : at::empty({1}, opt);
+  {
+    py::gil_scoped_release nogil;
+    check(pages_assign(i32(context), i32(fresh), static_cast<int>(n), i32(table), table.stride(0), static_cast<int>(table.size(1)), i32(free_pages),
+                       static_cast<int>(free_pages.size(0)), i32(count), i32(left), sh, static_cast<int>(tokens), i32(cu), i32(pos), i32(slots),
+                       reinterpret_cast<int*>(status), stream_ptr(stream)),
+          "ua_assign_pages");
+  }
+  return py::make_tuple(cu, pos, slots, left);
+}
+
+py::object release_pages(const Tensor& ended, const Tensor& context, const Tensor& table, const Tensor& free_pages, const Tensor& count,
+                         int64_t page_size, const c10::optional<Tensor>& count_out, int64_t most_requests, uintptr_t status, uintptr_t stream) {
+  const at::Device dev = table.device();
+  const int sh = log2_of(page_size);
+  const int64_t n = table.dim() == 2 ? table.size(0) : -1;
+  if (!dev.is_cuda() || sh < 0 || n < 0 || n > most_requests || !is_table(table, dev) || !is_int(context, dev, n) || free_pages.dim() != 1 ||
+      !is_int(free_pages, dev, free_pages.size(0)) || !is_int(count, dev, 1) || (count_out && !is_int(*count_out, dev, 1)) ||
+      ended.scalar_type() != at::kBool || ended.device() != dev || ended.dim() != 1 || ended.size(0) != n || !ended.is_contiguous())
+    return py::none();
+  const Tensor left = count_out ? *count_out : at::empty({1}, table.options());
+  {
+    py::gil_scoped_release nogil;
+    check(pages_release(static_cast<const unsigned char*>(ended.data_ptr()), i32(context), static_cast<int>(n), i32(table), table.stride(0),
+                        static_cast<int>(table.size(1)), i32(free_pages), static_cast<int>(free_pages.size(0)), i32(count), i32(left), sh,
+                        reinterpret_cast<int*>(status), stream_ptr(stream)),
+          "ua_release_pages");
+  }
+  return py::cast(left);
+}
+
+// (o, lse) in new tensors
+py::object paged_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& context, const Tensor& cu,
+                           int64_t most_new, double scale, int64_t left, int64_t sink, int64_t most_requests, uintptr_t status, uintptr_t stream) {
+  const at::Device dev = q.device();
+  if (!dev.is_cuda() || q.dim() != 3 || kc.dim() != 4 || vc.dim() != 4 || table.dim() != 2) return py::none();
+  const int64_t T = q.size(0), H = q.size(1), hk = kc.size(2), n = table.size(0), sh = log2_of(kc.size(1));
+  for (const Tensor* t : {&q, &kc, &vc}) {
+    const int64_t d = t->dim() - 1;
+    if (t->scalar_type() != at::kBFloat16 || t->device() != dev || t->size(d) != D || t->stride(d) != 1 || reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 != 0)
+      return py::none();
+    for (int64_t i = 0; i < d; ++i)
+      if (t->stride(i) % 8 != 0) return py::none();
+  }
+  if (kc.sizes() != vc.sizes() || sh < 4 || hk == 0 || H % hk != 0 || H / hk > 128 || n > most_requests || !is_table(table, dev) || !is_int(context, dev, n) ||
+      !is_int(cu, dev, n + 1) || most_new < 0 || !(scale > 0.0 && scale < 1e30) || sink < 0 || (sink > 0 && left < 0))
+    return py::none();
+  const Tensor o = at::empty(q.sizes(), q.options());
+  const Tensor lse = at::empty({H, T}, q.options().dtype(at::kFloat));
+  const UaPagedAttn a{q.data_ptr(), T, H, q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(), kc.size(0), hk,
+                      kc.stride(0), kc.stride(1), kc.stride(2), vc.stride(0), vc.stride(1), vc.stride(2), sh, i32(table), table.stride(0), table.size(1),
+                      i32(context), i32(cu), n, most_new < T ? most_new : T, left, sink, o.data_ptr(), o.stride(0), o.stride(1),
+                      static_cast<float*>(lse.data_ptr()), lse.stride(0)};
+  const Tensor ws = at::empty({paged_workspace(&a)}, lse.options());
+  {
+    py::gil_scoped_release nogil;
+    check(paged_attn(&a, static_cast<float>(scale), static_cast<float*>(ws.data_ptr()), reinterpret_cast<int*>(status), stream_ptr(stream)), "ua_attn_paged");
+  }
+  return py::make_tuple(o, lse);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(ua_host, m) {
+  m.def("init_paged", &init_paged);
+  m.def("rotate_pair", &rotate_pair);
+  m.def("rotary_append", &rotary_append);
+  m.def("assign_pages", &assign_pages);
+  m.def("release_pages", &release_pages);
+  m.def("paged_attention", &paged_attention);
   m.def("init", &init);
   m.def("dense_forward", &dense_forward);
   m.def("local_backward", &local_backward);

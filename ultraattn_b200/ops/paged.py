@@ -28,7 +28,7 @@ import torch
 
 from .. import _lib
 from . import rotary as R
-from .attention import KERNEL_HEAD_DIM, status_buffer
+from .attention import KERNEL_HEAD_DIM, _native, status_buffer
 
 MAX_REQUESTS = 8192
 _ATTN = struct.Struct("30q")          # struct UaPagedAttn of csrc/paged_args.h
@@ -84,6 +84,13 @@ def assign_pages(context_lens, new_lens, block_table, free_pages, free_count, *,
     ``free_count`` itself is not changed unless it is given as ``count_out`` too; else the pages left are in the result
     alone. All int32. A new token in front of position 0 (``new > context``) gets no slot. If the pages do not suffice, or a row of
     the table, or ``tokens``, nothing is assigned: every slot is -1, ``cu_new`` is 0 (and the error reported, see above)."""
+    if _native(block_table, context_lens, new_lens, free_pages, free_count):
+        with _lib.on_device(block_table):
+            r = _lib.host().assign_pages(context_lens, new_lens, block_table, free_pages, free_count, page_size, tokens, count_out, MAX_REQUESTS,
+                                         status_buffer(block_table.device).data_ptr(), _lib.stream_of(block_table))
+        if r is not None:
+            _lib.LAUNCHES[0] += 1
+            return PagedStep(*r)
     sh = _shift(page_size)
     _check_pool(dict(context_lens=context_lens, new_lens=new_lens), block_table, free_pages, free_count, count_out)
     if tokens < 0:
@@ -135,6 +142,13 @@ def release_pages(ended, context_lens, block_table, free_pages, free_count, *, p
     onto the stack ``free_pages``, in the order of the requests; the table itself is left as it is. Returns the number
     of free pages, in ``count_out`` if given (``free_count`` itself may be). If the stack has no room for them (a page given
     back twice), nothing changes and the error is reported."""
+    if _native(block_table, ended, context_lens, free_pages, free_count):
+        with _lib.on_device(block_table):
+            r = _lib.host().release_pages(ended, context_lens, block_table, free_pages, free_count, page_size, count_out, MAX_REQUESTS,
+                                          status_buffer(block_table.device).data_ptr(), _lib.stream_of(block_table))
+        if r is not None:
+            _lib.LAUNCHES[0] += 1
+            return r
     sh = _shift(page_size)
     _check_pool(dict(context_lens=context_lens), block_table, free_pages, free_count, count_out)
     n = block_table.shape[0]
@@ -175,6 +189,13 @@ def rotary_append(q, k, v, pos, slots, k_cache, v_cache, inv_freq=None, *, inter
     fp32). A token whose slot is negative is not written to the cache. ``inv_freq``, ``interleaved``, ``magnitude`` as in
     :func:`ultraattn_b200.rotary`; without ``inv_freq`` nothing is turned. Returns the queries, in ``q_out`` if given (``q``
     itself: in place). Slots must differ: of two tokens with the same slot either may end up in it."""
+    if inv_freq is not None and q_out is None and _native(q, k, v, pos, slots, k_cache, v_cache, inv_freq):
+        with _lib.on_device(q):
+            r = _lib.host().rotary_append(q, k, v, pos, slots, k_cache, v_cache, inv_freq, interleaved, magnitude,
+                                          status_buffer(q.device).data_ptr(), _lib.stream_of(q))
+        if r is not None:
+            _lib.LAUNCHES[0] += 1
+            return r
     sh = _check_cache(k_cache, v_cache)
     T, hk, dim = k.shape if k.dim() == 3 else (-1, -1, -1)
     if q.dim() != 3 or k.shape != v.shape or q.shape[0] != T or q.shape[2] != dim or tuple(k_cache.shape[2:]) != (hk, dim):
@@ -267,6 +288,14 @@ def paged_attention(q, k_cache, v_cache, block_table, context_lens, cu_new, *, m
     ``o [tokens, heads, 128]`` bf16 and ``lse [heads, tokens]`` fp32, in ``out = (o, lse)`` if given; rows behind the
     last request are not written. A query that sees no key (``context < n``) gives 0 and -inf. What the cache holds in places that no
     query of a request sees (behind its last token, in pages before its window) does not matter, NaN included. Forward only."""
+    if out is None and window_size[1] in (0, -1) and _native(q, k_cache, v_cache, block_table, context_lens, cu_new):
+        with _lib.on_device(q):
+            r = _lib.host().paged_attention(q, k_cache, v_cache, block_table, context_lens, cu_new, q.shape[0] if most_new is None else most_new,
+                                            q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale, window_size[0], sink_tokens, MAX_REQUESTS,
+                                            status_buffer(q.device).data_ptr(), _lib.stream_of(q))
+        if r is not None:
+            _lib.LAUNCHES[0] += 2
+            return r
     if q.dim() != 3 or k_cache.dim() != 4 or q.shape[2] != k_cache.shape[3]:
         raise ValueError("q is [tokens, heads, dim], the caches [pages, page_size, kv_heads, dim]")
     sh = _check_cache(k_cache, v_cache)

@@ -170,18 +170,29 @@ def rotate(tensors, pos, inv_freq, *, interleaved: bool = False, magnitude: floa
     return dst
 
 
+def _rotate_pair(q, k, pos, inv_freq, interleaved, magnitude, inverse):
+    from .attention import _native, status_buffer
+    if _native(q, k, pos, inv_freq):
+        with _lib.on_device(q):
+            r = _lib.host().rotate_pair(q, k, pos, inv_freq, interleaved, magnitude, inverse, status_buffer(q.device).data_ptr(), _lib.stream_of(q))
+        if r is not None:
+            _lib.LAUNCHES[0] += 1
+            return r
+    return rotate((q, k), pos, inv_freq, interleaved=interleaved, magnitude=magnitude, inverse=inverse)
+
+
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, pos, inv_freq, interleaved, magnitude):
         ctx.save_for_backward(pos, inv_freq)
         ctx.form = (interleaved, magnitude)
-        return rotate((q, k), pos, inv_freq, interleaved=interleaved, magnitude=magnitude)
+        return _rotate_pair(q, k, pos, inv_freq, interleaved, magnitude, False)
 
     @staticmethod
     def backward(ctx, dq, dk):
         pos, inv_freq = ctx.saved_tensors
         interleaved, magnitude = ctx.form
-        dq, dk = rotate((dq, dk), pos, inv_freq, interleaved=interleaved, magnitude=magnitude, inverse=True)
+        dq, dk = _rotate_pair(dq, dk, pos, inv_freq, interleaved, magnitude, True)
         return dq, dk, None, None, None, None
 
 
