@@ -12,8 +12,9 @@
 
 namespace ua {
 
-constexpr int PF_THREADS = 320;
+constexpr int PF_THREADS = 352;
 constexpr int PF_TMA_WARP = 8;
+constexpr int PF_WALK_WARP = 10;
 constexpr int PF_MMA_WARP = 9;                // issues the products; owns the TMEM allocation
 
 template <int N>
@@ -32,9 +33,10 @@ struct __align__(1024) FewSmem {
   uint64_t q_full[2], q_empty[2];
   uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
   uint64_t s_full[2], p_full[2], pv_done[2];
-  uint64_t item_full[2], item_empty[2];
+  uint64_t item_full[PA_ITEMS], item_empty[PA_ITEMS];
   uint64_t stat_full, merged;
-  PagedItem item[2];
+  PagedItem item[PA_ITEMS];
+  int item_pages[PA_ITEMS][8];          // of its first tile
   PagedScalars c;
   uint32_t tmem_base;
   int abort_flag;
@@ -102,8 +104,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __g
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.p_full[i], 4);
       mbar_init(&s.pv_done[i], 1);
+    }
+    for (int i = 0; i < PA_ITEMS; ++i) {
       mbar_init(&s.item_full[i], 1);
-      mbar_init(&s.item_empty[i], 1 + 8);
+      mbar_init(&s.item_empty[i], 2 + 8);       // loader, issuer, softmax warps
     }
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&s.k_full[i], 1);
@@ -133,10 +137,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __g
     report_error_call(wc.abort_flag, wc.status, UA_ERR_MBAR_TIMEOUT, where, static_cast<int>(parity));
     return false;
   };
-  auto item_there = [&](uint32_t n) -> bool { return wait(&s.item_full[n & 1], (n >> 1) & 1, 450) && s.item[n & 1].exists != 0; };
+  auto item_there = [&](uint32_t n) -> bool { return wait(&s.item_full[n % PA_ITEMS], (n / PA_ITEMS) & 1, 450) && s.item[n % PA_ITEMS].exists != 0; };
 
-  if (warp == PF_TMA_WARP) {
-    paged_producer<N>(maps, s, wait, [&](const PagedItem& it, uint32_t live) -> bool {
+  if (warp == PF_WALK_WARP) {
+    paged_walker<N>(s, wait);
+  } else if (warp == PF_TMA_WARP) {
+    paged_loader(maps, s, wait, item_there, [&](const PagedItem& it, uint32_t live) -> bool {
       const uint32_t qb = live % Smem::QS;
       if (!__all_sync(0xFFFFFFFFu, wait(&s.q_empty[qb], ((live / Smem::QS) & 1) ^ 1, 451))) return false;
       if (lane == 0) mbar_arrive_expect_tx(&s.q_full[qb], N * PD * 2);
@@ -155,8 +161,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __g
       bool ok = true;
       uint32_t kv = 0, live = 0, phase = 0;
       for (uint32_t n = 0; ok && item_there(n); ++n) {
-        const int total = s.item[n & 1].total;
-        mbar_arrive(&s.item_empty[n & 1]);
+        const int total = s.item[n % PA_ITEMS].total;
+        mbar_arrive(&s.item_empty[n % PA_ITEMS]);
         if (total == 0) continue;
         const uint32_t qb = live % Smem::QS;
         if (!wait(&s.q_full[qb], (live / Smem::QS) & 1, 452)) break;
@@ -204,7 +210,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __g
     uint32_t cnt = 0;                        // tiles of this group so far
     uint32_t kv = 0;                         // key tiles of this CTA so far
     for (uint32_t n = 0; __all_sync(0xFFFFFFFFu, item_there(n)); ++n) {
-      const PagedItem& it = s.item[n & 1];
+      const PagedItem& it = s.item[n % PA_ITEMS];
       float nm[N], l[N];                     // minus a row's reference maximum in log2 units, this lane's share of its sum
       float nm_lane = PF_UNSEEN;             // nm of row `lane`
 #pragma unroll
@@ -364,7 +370,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __g
       ok = mbar_wait_quiet(&s.merged, n & 1, wc) && ok;            // (the sums, O and P are free for the next item)
       if (!ok) report_error_call(wc.abort_flag, wc.status, UA_ERR_MBAR_TIMEOUT, 456 + w, static_cast<int>(j));
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s.item_empty[n & 1]);
+      if (lane == 0) mbar_arrive(&s.item_empty[n % PA_ITEMS]);
       if (!__all_sync(0xFFFFFFFFu, ok)) break;
     }
   }

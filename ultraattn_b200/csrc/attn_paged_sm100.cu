@@ -19,6 +19,7 @@ constexpr int PA_SOFTMAX_WARPS = 8;
 constexpr int PA_TMA_WARP = 8;
 constexpr int PA_QK_WARP = 9;                 // issues S = Q K^T; owns the TMEM allocation
 constexpr int PA_PV_WARP = 10;                // issues O += P V
+constexpr int PA_WALK_WARP = 11;
 constexpr int PA_THREADS = 384;
 constexpr int PA_REGS_LAUNCH = 168, PA_REGS_LOAD = 72, PA_REGS_SOFTMAX = 216;
 static_assert(2 * PA_REGS_SOFTMAX + PA_REGS_LOAD <= 3 * PA_REGS_LAUNCH, "setmaxnreg may only redistribute the launch-time pool");
@@ -35,9 +36,10 @@ struct __align__(1024) PagedSmem {
   uint64_t s_full[2], p_full[2];
   uint64_t s_free;           // the scores have been read into registers
   uint64_t pv_done[2];
-  uint64_t item_full[2], item_empty[2];
+  uint64_t item_full[PA_ITEMS], item_empty[PA_ITEMS];
   uint64_t stat_full, merged;
-  PagedItem item[2];
+  PagedItem item[PA_ITEMS];
+  int item_pages[PA_ITEMS][8];          // of its first tile
   PagedScalars c;
   float2 stat[FEW ? PT : 1];
   uint32_t tmem_base;
@@ -188,8 +190,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.p_full[i], act_warps);
       mbar_init(&s.pv_done[i], 1);
+    }
+    for (int i = 0; i < PA_ITEMS; ++i) {
       mbar_init(&s.item_full[i], 1);
-      mbar_init(&s.item_empty[i], (FEW ? 1 : 2) + 2 * act_warps);
+      mbar_init(&s.item_empty[i], (FEW ? 2 : 3) + 2 * act_warps);       // loader, issuers, softmax warps
     }
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&s.k_full[i], 1);
@@ -221,15 +225,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
     return false;
   };
   // Consumers: item n is in its slot, and there is one (false: no more, or a wait gave up). They hand it back by an arrival on item_empty.
-  auto item_there = [&](uint32_t n) -> bool { return wait(&s.item_full[n & 1], (n >> 1) & 1, 420) && s.item[n & 1].exists != 0; };
+  auto item_there = [&](uint32_t n) -> bool { return wait(&s.item_full[n % PA_ITEMS], (n / PA_ITEMS) & 1, 420) && s.item[n % PA_ITEMS].exists != 0; };
 
   if (warp >= PA_SOFTMAX_WARPS) {
     reg_dealloc<PA_REGS_LOAD>();
     if (warp == PA_TMA_WARP) {
-      // =============================== walker and TMA producer =================================
+      // =============================== loader =================================
       const int boxes = FEW ? 2 : 4;
       const uint32_t bytes = FEW && p.two_q ? PA_TILE_BYTES / 2 : boxes * (PA_TILE_BYTES / 2);
-      paged_producer<FEW ? PT : 2 * PT>(maps, s, wait, [&](const PagedItem& it, uint32_t live) -> bool {
+      paged_loader(maps, s, wait, item_there, [&](const PagedItem& it, uint32_t live) -> bool {
         const uint32_t qb = p.two_q ? live & 1 : 0, use = p.two_q ? live >> 1 : live;
         if (!__all_sync(0xFFFFFFFFu, wait(&s.q_empty[qb], (use & 1) ^ 1, 402))) return false;
         if (lane == 0) mbar_arrive_expect_tx(&s.q_full[qb], bytes);
@@ -239,6 +243,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
                       it.kv_head * p.group, it.q_row + it.tok0 + (((lane >> 1) * PT) >> psh));
         return true;
       });
+    } else if (warp == PA_WALK_WARP) {
+      paged_walker<FEW ? PT : 2 * PT>(s, wait);
     } else if (warp == PA_QK_WARP || (!FEW && warp == PA_PV_WARP)) {
       // =============================== MMA issuers ============================================
       if (elect_one()) {
@@ -265,8 +271,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
           for (int kk = 0; kk < 8; ++kk) umma_ts_lo<HI>(tO, tP + kk * 8, va + ((kk * 2048) >> 4), idesc_o, (acc || kk > 0) ? 1u : 0u);
         };
         auto take_total = [&](uint32_t n) -> int {
-          const int t = s.item[n & 1].total;
-          mbar_arrive(&s.item_empty[n & 1]);
+          const int t = s.item[n % PA_ITEMS].total;
+          mbar_arrive(&s.item_empty[n % PA_ITEMS]);
           return t;
         };
         bool ok = true;
@@ -360,7 +366,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
       uint32_t cnt = 0;                        // score tiles of this sub-tile so far
       uint32_t kv = 0;                         // key tiles of this CTA so far
       for (uint32_t n = 0; __all_sync(0xFFFFFFFFu, item_there(n)); ++n) {
-        const PagedItem& it = s.item[n & 1];   // (stays in shared memory: the score loop needs the registers)
+        const PagedItem& it = s.item[n % PA_ITEMS];   // (stays in shared memory: the score loop needs the registers)
         float m_use = NEG_INF, l = 0.f;
         bool ok = true;
         uint32_t j = 0;
@@ -534,7 +540,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
         }
         if (!ok) report_error_call(wc.abort_flag, wc.status, UA_ERR_MBAR_TIMEOUT, 440 + w, static_cast<int>(j));
         __syncwarp();                            // every lane is done reading the item
-        if (lane == 0) mbar_arrive(&s.item_empty[n & 1]);
+        if (lane == 0) mbar_arrive(&s.item_empty[n % PA_ITEMS]);
         if (!__all_sync(0xFFFFFFFFu, ok)) break;
       }
     }

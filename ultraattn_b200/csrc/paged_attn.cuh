@@ -65,6 +65,7 @@ static_assert(sizeof(PagedScalars) % 4 == 0 && sizeof(PagedScalars) <= 64 * 4, "
 constexpr int PA_DESC = 8;
 
 constexpr int PA_NO_PAGE = -0x7FFFFFFF;
+constexpr int PA_ITEMS = 3;                   // items in shared memory: the one before may still be written out
 
 // A piece of an item: the key tiles that this CTA takes of it.
 struct PagedItem {
@@ -323,32 +324,69 @@ static __device__ __noinline__ void clear_unseen(uint8_t* v, uint64_t* v_full, u
   fence_proxy_async_smem();
 }
 
-// The producer's warp: walks the share, hands the pieces over, and loads their keys and values page by page (a TMA box is a page, or
-// 128 tokens of a larger one; a lane issues the boxes of one page and d-half). All lanes walk. load_q(item, live) loads the queries
-// of the live-th item that has keys.
-template <int ROWS, typename Smem, typename Wait, typename LoadQ>
-__device__ __forceinline__ void paged_producer(const PagedParams& maps, Smem& s, Wait wait, LoadQ load_q) {
+// This lane's entry of tile i of an item: lane b has that of the tile's page b (PA_NO_PAGE: not needed, -1: not in the table).
+__device__ __forceinline__ int page_entry(const PagedScalars& p, const PagedItem& it, int i, int lane) {
+  const int box_rows = p.page_shift < 7 ? 1 << p.page_shift : PT;
+  const int n0 = it.end[0] - it.first[0];
+  const bool band = i >= n0;
+  const int key = (band ? it.first[1] + i - n0 : it.first[0] + i) * PT + lane * box_rows;
+  if (lane >= PT / box_rows || i >= it.total || key >= (band ? it.hi[1] : it.hi[0]) || key + box_rows <= (band ? it.lo[1] : it.lo[0])) return PA_NO_PAGE;
+  const int col = key >> p.page_shift;
+  return col < p.columns ? p.table[it.request * p.table_stride + col] : -1;
+}
+
+// The walker's warp hands the pieces of the share over, with the pages of their first tiles, as far ahead as there is room. (Done by the warp
+// that loads, which shares its scheduler with two softmax warps, a hundred instructions at an item's end were 3000 to 5000
+// clocks in which nothing was loaded.)
+template <int ROWS, typename Smem, typename Wait>
+__device__ __forceinline__ void paged_walker(Smem& s, Wait wait) {
+  const PagedScalars& p = s.c;
+  const int lane = threadIdx.x & 31, cta = blockIdx.x;
+  int begun = 0, begun_tok = 0, begun_head = 0, begun_rows = 0, cont = 0;
+  PagedWalk<ROWS> walk;
+  bool exists = walk.start(p, cta, gridDim.x);
+  for (uint32_t m = 0;; ++m) {
+    PagedItem it;
+    int part = 0;
+    exists = exists && walk.next(p, it, part);
+    const uint32_t slot = m % PA_ITEMS;
+    int page = PA_NO_PAGE;
+    if (exists) page = page_entry(p, it, 0, lane);
+    it.exists = exists;
+    it.slot = part == 0 ? -1 : 2 * cta + (part == 1);
+    if (exists && part == 1) {
+      begun = 1;
+      begun_tok = it.q_row + it.tok0;
+      begun_head = it.kv_head * p.group;
+      begun_rows = it.rows;
+    } else if (exists && part > 1) {
+      cont = part == 2 ? 1 : 2;
+    }
+    if (m >= PA_ITEMS && !__all_sync(0xFFFFFFFFu, wait(&s.item_empty[slot], (m / PA_ITEMS - 1) & 1, 403))) break;
+    if (lane < 8) s.item_pages[slot][lane] = page;
+    __syncwarp();
+    if (lane == 0) {
+      s.item[slot] = it;
+      mbar_arrive(&s.item_full[slot]);
+    }
+    if (!exists) break;
+  }
+  grid_trigger();
+  if (lane == 0) {
+    int* d = p.part_desc + cta * PA_DESC;
+    *reinterpret_cast<int4*>(d) = make_int4(begun, begun_tok, begun_head, begun_rows);
+    d[4] = cont;
+  }
+}
+
+// The loader's warp: keys and values, page by page (a TMA box is a page, or 128 tokens of a larger one). load_q(item, live) loads the
+// queries of the live-th item that has keys.
+template <typename Smem, typename Wait, typename There, typename LoadQ>
+__device__ __forceinline__ void paged_loader(const PagedParams& maps, Smem& s, Wait wait, There item_there, LoadQ load_q) {
   const PagedScalars& p = s.c;
   constexpr int STAGES = Smem::STAGES;
-  const int lane = threadIdx.x & 31, cta = blockIdx.x;
-  PagedWalk<ROWS> walk;
-  const int box_rows = p.page_shift < 7 ? 1 << p.page_shift : PT;
-  const int boxes = PT / box_rows;          // pages of a tile: lane b holds the entry of page b
-  const uint32_t box_bytes = static_cast<uint32_t>(box_rows) * 128;
-  int begun = 0, begun_tok = 0, begun_head = 0, begun_rows = 0, cont = 0;
-  uint32_t j = 0, live = 0;
-  bool ok = true;
-  PagedItem next;
-  int part = 0;
-  // this lane's entry of tile i of an item (PA_NO_PAGE: not needed); it is looked at when the tile is loaded, a tile later
-  auto entry_of = [&](const PagedItem& it, int i) -> int {
-    const int n0 = it.end[0] - it.first[0];
-    const bool band = i >= n0;
-    const int key = (band ? it.first[1] + i - n0 : it.first[0] + i) * PT + lane * box_rows;
-    if (lane >= boxes || i >= it.total || key >= (band ? it.hi[1] : it.hi[0]) || key + box_rows <= (band ? it.lo[1] : it.lo[0])) return PA_NO_PAGE;
-    const int col = key >> p.page_shift;
-    return col < p.columns ? p.table[it.request * p.table_stride + col] : -1;
-  };
+  const int lane = threadIdx.x & 31;
+  const uint32_t box_bytes = (p.page_shift < 7 ? 1u << p.page_shift : PT) * 128u;
   // A tile's boxes: up to eight pages in two d-halves. One thread issues them, one behind the other: 20 clocks each. (A box per lane: the
   // lanes are taken one by one, 60 to 130 clocks each, and pages of 16 come at 0.6 of the memory's rate.)
   auto load_tile = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, unsigned there, const int (&pages)[8], int head, int off) {
@@ -363,42 +401,25 @@ __device__ __forceinline__ void paged_producer(const PagedParams& maps, Smem& s,
     }
     __syncwarp();
   };
-  next.exists = walk.start(p, cta, gridDim.x) && walk.next(p, next, part);
-  int first_page = next.exists ? entry_of(next, 0) : PA_NO_PAGE;
-  for (uint32_t n = 0; ok; ++n) {
-    const uint32_t slot = n & 1;
-    if (n >= 2 && !__all_sync(0xFFFFFFFFu, wait(&s.item_empty[slot], ((n - 2) >> 1) & 1, 403))) break;
-    next.slot = part == 0 ? -1 : 2 * cta + (part == 1);
-    if (next.exists && part == 1) {
-      begun = 1;
-      begun_tok = next.q_row + next.tok0;
-      begun_head = next.kv_head * p.group;
-      begun_rows = next.rows;
-    } else if (next.exists && part > 1) {
-      cont = part == 2 ? 1 : 2;
-    }
-    if (lane == 0) {
-      s.item[slot] = next;
-      mbar_arrive(&s.item_full[slot]);
-    }
-    if (!next.exists) break;
-    __syncwarp();
-    const PagedItem& it = s.item[slot];
+  uint32_t j = 0, live = 0;
+  bool ok = true;
+  for (uint32_t n = 0; ok && __all_sync(0xFFFFFFFFu, item_there(n)); ++n) {
+    const PagedItem& it = s.item[n % PA_ITEMS];
     const int total = it.total, n0 = it.end[0] - it.first[0], f0 = it.first[0], f1 = it.first[1] - n0, head = it.kv_head;
-    int page = first_page;
+    int page = lane < 8 ? s.item_pages[n % PA_ITEMS][lane] : PA_NO_PAGE;
 #pragma unroll 1
     for (int i = 0; i < total; ++i, ++j) {
-      const int next_page = entry_of(it, i + 1);
-      const int off = ((i + (i >= n0 ? f1 : f0)) * PT) & ((1 << p.page_shift) - 1);       // (in a page of more than a tile)
+      const int next_page = page_entry(p, it, i + 1, lane);          // (looked at a tile later)
+      const int off = ((i + (i >= n0 ? f1 : f0)) * PT) & ((1 << p.page_shift) - 1);       // in a page of more than a tile
       const int st = j % STAGES;
       const uint32_t ph = (j / STAGES) & 1;
-      ok = __all_sync(0xFFFFFFFFu, wait(&s.k_empty[st], ph ^ 1, 400));
-      if (!ok) break;
       const unsigned there = __ballot_sync(0xFFFFFFFFu, page >= 0 && page < p.pages);
       if (page != PA_NO_PAGE && !((there >> lane) & 1u)) paged_error(p.status, 520, it.request);
       int pages[8];
 #pragma unroll
       for (int b = 0; b < 8; ++b) pages[b] = __shfl_sync(0xFFFFFFFFu, page, b);
+      ok = __all_sync(0xFFFFFFFFu, wait(&s.k_empty[st], ph ^ 1, 400));
+      if (!ok) break;
       load_tile(s.k[st], &maps.tm_k, &s.k_full[st], there, pages, head, off);
       if (i == 0) {
         // Q, behind the first keys: its room is free when the scores of the item before (of the one before that, where there are
@@ -411,21 +432,9 @@ __device__ __forceinline__ void paged_producer(const PagedParams& maps, Smem& s,
       if (!ok) break;
       load_tile(s.v[st], &maps.tm_v, &s.v_full[st], there, pages, head, off);
       page = next_page;
-      if (i == 0) {                            // (while those are on their way)
-        next.exists = walk.next(p, next, part);
-        first_page = next.exists ? entry_of(next, 0) : PA_NO_PAGE;
-      }
     }
-    if (total == 0) {
-      next.exists = walk.next(p, next, part);
-      first_page = next.exists ? entry_of(next, 0) : PA_NO_PAGE;
-    }
-  }
-  grid_trigger();
-  if (lane == 0) {
-    int* d = p.part_desc + cta * PA_DESC;
-    *reinterpret_cast<int4*>(d) = make_int4(begun, begun_tok, begun_head, begun_rows);
-    d[4] = cont;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.item_empty[n % PA_ITEMS]);
   }
 }
 
