@@ -554,13 +554,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
   }
 }
 
-// The parts of a cut item, in the order of its keys: O = sum_i w_i O_i with w_i = exp(lse_i - lse), fp32, one warp per row, 4 elements per
-// lane. Block (x, y, z): rows 8 y .. of the item that begins in CTA x of launch z and goes on behind it, if there is one.
+// The parts of a cut item, in the order of its keys: O = sum_i w_i O_i with w_i = exp(lse_i - lse), fp32, 4 elements of a row per lane.
+// Block (x, y, z): rows 32 y .. of the item that begins in CTA x of launch z and goes on behind it, if there is one. Latency of the chain
+// description -> lse -> parts and the parts' bytes (mostly in L2): a warp has four rows under way, so that all blocks are there at once.
 struct CombineParams {
-  const float* part_o[3];
-  const float* part_lse[3];
-  const int* desc[3];
-  int part_rows[3];
+  const float* part_o[2];
+  const float* part_lse[2];
+  const int* desc[2];
+  int part_rows[2];
   int ctas;
   int pack_shift, group;
   __nv_bfloat16* o;
@@ -568,7 +569,7 @@ struct CombineParams {
   float* lse;
   long lse_head;
 };
-constexpr int COMBINE_ROWS = 8;        // rows of a block
+constexpr int COMBINE_ROWS = 32;       // rows of a block
 __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constant__ CombineParams p) {
   grid_wait();
   grid_trigger();
@@ -577,12 +578,10 @@ __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constan
   const float *part_o = p.part_o[z], *part_lse = p.part_lse[z];
   const long part_rows = p.part_rows[z];
   // its head, and how far it goes: up to the next CTA that does not say that its part goes on (one load for all)
-  const int x = blockIdx.y * COMBINE_ROWS + (threadIdx.x >> 5);
-  const int* d = desc + first * PA_DESC;
-  const int d0 = d[0], token = d[1], head0 = d[2], rows = d[3];
+  const int x0 = blockIdx.y * COMBINE_ROWS + (threadIdx.x >> 5);
+  const int4 d = *reinterpret_cast<const int4*>(desc + first * PA_DESC);
   const int ahead = first + 1 + lane < p.ctas ? desc[(first + 1 + lane) * PA_DESC + 4] : 0;
-  const int h = x & ((1 << p.pack_shift) - 1);
-  if (d0 == 0 || x >= rows || h >= p.group) return;
+  if (d.x == 0 || x0 >= d.w) return;
   unsigned ends = __ballot_sync(0xFFFFFFFFu, ahead != 1);
   int n = 1;
   while (ends == 0) {
@@ -591,47 +590,77 @@ __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constan
   }
   n += __ffs(ends);
   // the slots of its parts: 2 first + 1, then 2 (first + 1), 2 (first + 2) ..
-  auto slot = [&](int i) -> long { return i == 0 ? 2 * first + 1 : 2 * (first + i); };
-  float mx = -INFINITY;
-  bool bad = false;                    // a NaN score: O = 0 and lse = -inf, as in an item that is not cut
-  for (int i = lane; i < n; i += 32) {
-    const float y = part_lse[slot(i) * part_rows + x];
-    bad |= y != y;
-    mx = fmaxf(mx, y);
+  auto row_of = [&](int i, int x) -> long { return (i == 0 ? 2 * first + 1 : 2 * (first + i)) * part_rows + x; };
+  // lane i: the lse of part i (and of parts 32 + i ..), then its weight; the parts themselves in one go behind that
+  float mx[4];
+  bool bad[4];                         // a NaN score: O = 0 and lse = -inf, as in an item that is not cut
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    mx[k] = -INFINITY;
+    bad[k] = false;
+  }
+  for (int i = lane; i < n; i += 32)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float y = x0 + 8 * k < d.w ? part_lse[row_of(i, x0 + 8 * k)] : -INFINITY;
+      bad[k] |= y != y;
+      mx[k] = fmaxf(mx[k], y);
+    }
+  float tot[4];
+  float4 acc[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xFFFFFFFFu, mx[k], s));
+    if (__any_sync(0xFFFFFFFFu, bad[k])) mx[k] = -INFINITY;
+    tot[k] = 0.f;
+    acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    float w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = i0 + lane < n && mx[k] > -INFINITY ? __expf(part_lse[row_of(i0 + lane, x0 + 8 * k)] - mx[k]) : 0.f;
+      tot[k] += w[k];
+    }
+    const int here = min(32, n - i0);
+#pragma unroll 4
+    for (int i = 0; i < here; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = __shfl_sync(0xFFFFFFFFu, w[k], i);
+        if (!(mx[k] > -INFINITY)) continue;
+        const float4 v = *reinterpret_cast<const float4*>(part_o + row_of(i0 + i, x0 + 8 * k) * PD + lane * 4);
+        acc[k].x += f * v.x;           // (f = 0 times what is not finite: as P V does with P = 0)
+        acc[k].y += f * v.y;
+        acc[k].z += f * v.z;
+        acc[k].w += f * v.w;
+      }
   }
 #pragma unroll
-  for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, k));
-  if (__any_sync(0xFFFFFFFFu, bad)) mx = -INFINITY;
-  float tot = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (mx > -INFINITY) {
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const long row = slot(i) * part_rows + x;
-      const float w = __expf(part_lse[row] - mx);
-      const float4 v = *reinterpret_cast<const float4*>(part_o + row * PD + lane * 4);
-      tot += w;
-      acc.x += w * v.x;
-      acc.y += w * v.y;
-      acc.z += w * v.z;
-      acc.w += w * v.w;
-    }
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) tot[k] += __shfl_xor_sync(0xFFFFFFFFu, tot[k], s);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int x = x0 + 8 * k, h = x & ((1 << p.pack_shift) - 1);
+    if (x >= d.w || h >= p.group) continue;
+    const float inv = tot[k] > 0.f ? 1.f / tot[k] : 0.f;
+    const long tok = d.y + (x >> p.pack_shift);
+    const int head = d.z + h;
+    uint2 o;
+    o.x = pack_bf16x2(acc[k].x * inv, acc[k].y * inv);
+    o.y = pack_bf16x2(acc[k].z * inv, acc[k].w * inv);
+    *reinterpret_cast<uint2*>(p.o + tok * p.o_token + head * p.o_head + lane * 4) = o;
+    if (lane == 0) p.lse[head * p.lse_head + tok] = tot[k] > 0.f ? mx[k] + __logf(tot[k]) : -INFINITY;
   }
-  const float inv = tot > 0.f ? 1.f / tot : 0.f;
-  const long tok = token + (x >> p.pack_shift);
-  const int head = head0 + h;
-  uint2 o;
-  o.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-  o.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(p.o + tok * p.o_token + head * p.o_head + lane * 4) = o;
-  if (lane == 0) p.lse[head * p.lse_head + tok] = tot > 0.f ? mx + __logf(tot) : -INFINITY;
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 // The launches of a call: the form (rows of an item), the requests that each takes by their rows, and the rows of its parts.
 struct PagedPlan {
   int pack_shift, n;
-  struct { int form, min_rows, max_rows, part_rows; } launch[3];
+  struct { int form, min_rows, max_rows, part_rows; } launch[2];
 };
 static PagedPlan plan_paged(const UaPagedAttn* a) {
   PagedPlan d{};
@@ -652,11 +681,8 @@ static PagedPlan plan_paged(const UaPagedAttn* a) {
     below = (1 << d.pack_shift) <= 16 ? 16 : 32;
     add(below, 0, below);
   }
-  if (most <= PT || a->requests > 1) {
-    add(PT, below, most < PT ? most : PT);
-    below = PT;
-  }
-  if (most > PT) add(2 * PT, below, most);
+  // (requests of a few tokens beside a long one go with it: a launch of their own took 15 us in a step of 20 requests)
+  add(most <= PT ? PT : 2 * PT, below, most);
   return d;
 }
 static long part_floats(int rows, int ctas) { return static_cast<long>(ctas) * (2l * rows * (PD + 1) + PA_DESC); }

@@ -24,6 +24,9 @@ constexpr int PT = 128;                       // keys of a tile
 constexpr int PA_TILE_BYTES = PT * PD * 2;    // [2 d-halves][128 rows][128 B]
 // What the start and the end of an item cost, in key tiles of its form (a share's border is not put into them).
 template <int ROWS> constexpr int PA_ITEM_TILES = ROWS <= 32 ? 1 : 3;
+// An item of fewer tiles is not cut: the border moves to its nearer end. Writing and merging the fp32 parts of 256 rows takes as long as
+// six to eight key tiles of them, those of 16 rows nothing.
+template <int ROWS> constexpr int PA_WHOLE = ROWS <= 32 ? 0 : ROWS == 128 ? 8 : 20;
 constexpr int PA_MIN_SHARE = 2;               // key tiles of a CTA at least
 
 // (Every block copies these into its shared memory before it waits for the kernel in front of it: parameters that have not been
@@ -264,6 +267,7 @@ struct PagedWalk {
       const int total = q.tiles(p, tile, it);
       const long e = s + (same > 0 ? same : PA_ITEM_TILES<ROWS> + total);
       const auto cut = [&](long x) -> int {
+        if (total < PA_WHOLE<ROWS>) return 2 * (x - s) > e - s ? total : 0;
         const long t = x - s - PA_ITEM_TILES<ROWS>;
         return x >= e || t > total ? total : t < 0 ? 0 : static_cast<int>(t);
       };
