@@ -7,8 +7,7 @@
 // The angle. p f in fp32 is off by 0.03 rad at position 500k (half a step of 2^19), and 64-bit sines for every token cost more than
 // the rotation. But only the fraction of a turn matters: t = f / 2 pi is held as a 64-bit fraction, p t is an integer
 // product whose overflow drops the whole turns, and what is left is split into quarters of a turn and a rest of at most an eighth,
-// whose sine and cosine are good to fp32 (the rest is exact to 2^-32 turns). No table, no largest position; the 64
-// angles of a token are found once per block and shared by its heads.
+// whose sine and cosine are good to fp32 (the rest is exact to 2^-32 turns). No table, no largest position.
 //
 // Bound by memory: every element is read and written once.
 #include <cuda_bf16.h>
@@ -16,15 +15,18 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "host_common.cuh"
 #include "paged_args.h"
 #include "ptx.cuh"
 
 namespace ua {
 
-constexpr int ROT_THREADS = 256;
+constexpr int ROT_WARPS = 4;           // of a block
 constexpr int ROT_MAX_PAIRS = 256;     // rotated elements of a head: 512 at most
-constexpr int ROT_MAX_TOKENS = 8;      // tokens of a block
+constexpr int ROT_SHARES = 8;          // warps of an SM up to which a token is shared
+constexpr int ROT_BATCH = 4;           // heads that a lane has under way
 
 struct RotParams {
   UaRotPart part[3];
@@ -41,7 +43,8 @@ struct RotParams {
   int pairs, dim;
   float magnitude;
   int inverse;
-  int block_tokens;       // tokens of a block
+  int split_shift;        // log2 of the warps that share a token's heads
+  int rot_units, rot_lanes;       // of a head: units that are turned, lanes that take them side by side
   int* status;
 };
 
@@ -57,6 +60,47 @@ template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
+
+// Element k of a vector in fp32, and a vector from fp32: two 16-bit elements at a time (element by element it is twice the instructions
+// of the whole rotation).
+template <typename T, int V>
+__device__ __forceinline__ void widen(const Vec<T, V>& x, float (&f)[V]) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    const uint32_t(&w)[V / 2] = reinterpret_cast<const uint32_t(&)[V / 2]>(x);
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 y = __half22float2(reinterpret_cast<const __half2&>(w[k]));
+        f[2 * k] = y.x;
+        f[2 * k + 1] = y.y;
+      } else {
+        f[2 * k] = __uint_as_float(w[k] << 16);
+        f[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = to_f(x.v[k]);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void narrow(const float (&f)[V], Vec<T, V>& x) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    uint32_t(&w)[V / 2] = reinterpret_cast<uint32_t(&)[V / 2]>(x);
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 y = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
+        w[k] = reinterpret_cast<const uint32_t&>(y);
+      } else {
+        w[k] = pack_bf16x2(f[2 * k], f[2 * k + 1]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) x.v[k] = from_f<T>(f[k]);
+  }
+}
 
 // cos and sin of position * (turns / 2^64) turns, times m
 __device__ __forceinline__ float2 turn_of(long pos, unsigned long long turns, float m) {
@@ -75,110 +119,164 @@ __device__ __forceinline__ float2 turn_of(long pos, unsigned long long turns, fl
   }
 }
 
-// V: elements per load and store (one otherwise); a unit is V elements of each half of the pairs (interleaved: V pairs' worth,
-// 2 elements at least), or V elements that are copied.
+// A warp has a token, or an equal share of its heads. A unit is V elements (16 bytes, or one) of each half of the pairs; interleaved V
+// elements of pairs side by side, 2 at least. A lane keeps its unit's place in the head, so that its sines and cosines stay in
+// registers, and goes from head to head with ROT_BATCH heads loaded ahead; the first of them before the angles are found.
+// B200, 8192 tokens of 32 + 8 heads of 128 in bf16, there and back: 59 us (5.7 of the 6.5 TB/s that a copy reaches), 3003 tokens of 24
+// heads in fp32 25 us. One block for some tokens with the angles in shared memory and every thread looking its units up took 100 us:
+// 237 instructions a unit. 3, 6, 8 heads ahead: 65, 63, 62 us; blocks of 8 warps 60.7, of 2 59.2.
 template <typename T, int V, bool INTERLEAVED>
-__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const __grid_constant__ RotParams p) {
-  __shared__ float2 cs[ROT_MAX_TOKENS * ROT_MAX_PAIRS];
-  __shared__ long dst_off[ROT_MAX_TOKENS];       // of a token in its pages; negative: none
+__global__ void __launch_bounds__(ROT_WARPS * 32) rotary_kernel(const __grid_constant__ RotParams p) {
+  __shared__ __align__(16) float cs[ROT_WARPS][2][ROT_MAX_PAIRS];            // cosines, sines
+  __shared__ unsigned long long turns[ROT_MAX_PAIRS];                        // 2^64 f / 2 pi: found once for the block
+  constexpr int E = INTERLEAVED && V == 1 ? 2 : V;                           // elements of a unit of one half, or of pairs
+  constexpr int F = INTERLEAVED ? E / 2 : V;                                 // pairs of a unit
+  using W = Vec<T, INTERLEAVED && V == 1 ? 1 : V>;
+  using A = Vec<float, F < 4 ? F : 4>;
   grid_wait();
   grid_trigger();
-  const long tok0 = static_cast<long>(blockIdx.x) * p.block_tokens;
-  const int here = static_cast<int>(min(static_cast<long>(p.block_tokens), p.tokens - tok0));
-  auto pos_of = [&](long t) -> long {
-    const long i = t / p.per_batch * p.pos_batch + t % p.per_batch * p.pos_token;
-    return p.pos64 ? static_cast<const long*>(p.pos)[i] : static_cast<const int*>(p.pos)[i];
-  };
-  if (p.pairs > 0) {
-    for (int i = threadIdx.x; i < here * p.pairs; i += ROT_THREADS) {
-      const int t = i / p.pairs, f = i % p.pairs;
-      double turns = p.inv_freq[f] * 0.15915494309189535;                  // 1 / 2 pi
-      turns -= floor(turns);
-      const float2 v = turn_of(pos_of(tok0 + t), __double2ull_rn(turns * 18446744073709551616.0), p.magnitude);
-      cs[i] = make_float2(v.x, p.inverse ? -v.y : v.y);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long share = static_cast<long>(blockIdx.x) * ROT_WARPS + warp;
+  const long tok = min(share >> p.split_shift, p.tokens - 1);                // (a warp behind the last token leaves after the barrier)
+  const int slice = static_cast<int>(share & ((1 << p.split_shift) - 1));
+  const long seq = p.tokens == p.per_batch ? 0 : tok / p.per_batch, in_seq = tok - seq * p.per_batch;
+  // where the token's rows of tensor ip begin (false: it has none to go to)
+  auto rows = [&](int ip, const T*& src, T*& dst) -> bool {
+    const UaRotPart& q = p.part[ip];
+    src = static_cast<const T*>(q.src) + seq * q.src_batch + in_seq * q.src_token;
+    dst = static_cast<T*>(q.dst);
+    if (!q.paged) {
+      dst += seq * q.dst_batch + in_seq * q.dst_token;
+      return true;
     }
-  }
-  if (p.slots != nullptr && threadIdx.x < here) {
-    const int slot = p.slots[tok0 + threadIdx.x];
-    if (slot >= p.n_slots && atomicCAS(p.status, 0, UA_ERR_BAD_ARG) == 0) {
+    const long slot = p.slots[tok];
+    if (slot >= p.n_slots && lane == 0 && atomicCAS(p.status, 0, UA_ERR_BAD_ARG) == 0) {
       p.status[1] = 500;
       p.status[2] = static_cast<int>(blockIdx.x);
-      p.status[3] = slot;
+      p.status[3] = static_cast<int>(slot);
     }
-    dst_off[threadIdx.x] = slot >= p.n_slots ? -1 : slot;
+    if (slot < 0 || slot >= p.n_slots) return false;
+    dst += (slot >> p.page_shift) * q.dst_batch + (slot & ((1l << p.page_shift) - 1)) * q.dst_token;
+    return true;
+  };
+
+  for (int f = threadIdx.x; f < p.pairs; f += ROT_WARPS * 32) {
+    double t = p.inv_freq[f] * 0.15915494309189535;                          // 1 / 2 pi
+    t -= floor(t);
+    turns[f] = __double2ull_rn(t * 18446744073709551616.0);
   }
-  __syncthreads();
-  constexpr int E = INTERLEAVED && V == 1 ? 2 : V;                           // elements of a unit of one half, or of pairs
-  const int rot = 2 * p.pairs;
-  const int rot_units = INTERLEAVED ? rot / E : p.pairs / E;
-  const int units = rot_units + (p.dim - rot + V - 1) / V;
-#pragma unroll 1
+  const bool idle = share >> p.split_shift >= p.tokens;
+  bool angles = false;
+
+  // ---- turned units: lane = (head of a pass, unit) ----------------------------------------------------------------------------
+  if (p.rot_units > 0) {
+    const int per_pass = 32 / p.rot_lanes;             // heads of a pass
+    const int sub = lane / p.rot_lanes, step = per_pass << p.split_shift;
+    const int head0 = sub < per_pass ? slice * per_pass + sub : 0x3FFFFFFF;
+    float c[F], s[F];
+    W a[ROT_BATCH], b[ROT_BATCH];
+    for (int unit = lane % p.rot_lanes; unit - lane % p.rot_lanes < p.rot_units; unit += 32) {     // (more than 32 units: one head a pass)
+      bool fresh = true;
+      for (int ip = 0; ip < p.n_parts; ++ip) {
+        const UaRotPart& q = p.part[ip];
+        const T* src;
+        T* dst;
+        if (!q.rotate || !rows(ip, src, dst)) continue;
+        src += unit * E;
+        dst += unit * E;
+        const int heads = unit < p.rot_units ? static_cast<int>(q.heads) : 0;
+        auto load = [&](int h) {
+#pragma unroll
+          for (int i = 0; i < ROT_BATCH; ++i)
+            if (h + i * step < heads) {
+              const T* x = src + (h + i * step) * q.src_head;
+              a[i] = *reinterpret_cast<const W*>(x);
+              if constexpr (!INTERLEAVED) b[i] = *reinterpret_cast<const W*>(x + p.pairs);
+              else if constexpr (V == 1) b[i] = *reinterpret_cast<const W*>(x + 1);
+            }
+        };
+        load(head0);
+        if (!angles) {
+          const long at = seq * p.pos_batch + in_seq * p.pos_token;
+          const long pos = p.pos64 ? static_cast<const long*>(p.pos)[at] : static_cast<const int*>(p.pos)[at];
+          __syncthreads();                 // (once for every warp: the first tensor is turned and has a row for every token)
+          if (idle) return;
+          for (int f = lane; f < p.pairs; f += 32) {
+            const float2 v = turn_of(pos, turns[f], p.magnitude);
+            cs[warp][0][f] = v.x;
+            cs[warp][1][f] = p.inverse ? -v.y : v.y;
+          }
+          __syncwarp();
+          angles = true;
+        }
+        if (fresh && unit < p.rot_units) {
+#pragma unroll
+          for (int k = 0; k < F; k += sizeof(A) / 4) {
+            const A x = *reinterpret_cast<const A*>(&cs[warp][0][unit * F + k]), y = *reinterpret_cast<const A*>(&cs[warp][1][unit * F + k]);
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(sizeof(A) / 4); ++i) {
+              c[k + i] = x.v[i];
+              s[k + i] = y.v[i];
+            }
+          }
+        }
+        fresh = false;
+        for (int h = head0; h < heads; h += ROT_BATCH * step) {
+#pragma unroll
+          for (int i = 0; i < ROT_BATCH; ++i) {
+            if (h + i * step >= heads) break;
+            T* y = dst + (h + i * step) * q.dst_head;
+            W u, v;
+            if constexpr (INTERLEAVED && V > 1) {
+              float x[V], z[V];
+              widen<T, V>(a[i], x);
+#pragma unroll
+              for (int k = 0; k < F; ++k) {
+                z[2 * k] = x[2 * k] * c[k] - x[2 * k + 1] * s[k];
+                z[2 * k + 1] = x[2 * k + 1] * c[k] + x[2 * k] * s[k];
+              }
+              narrow<T, V>(z, u);
+              *reinterpret_cast<W*>(y) = u;
+            } else {
+              float x0[F], x1[F], z0[F], z1[F];
+              widen<T, F>(a[i], x0);
+              widen<T, F>(b[i], x1);
+#pragma unroll
+              for (int k = 0; k < F; ++k) {
+                z0[k] = x0[k] * c[k] - x1[k] * s[k];
+                z1[k] = x1[k] * c[k] + x0[k] * s[k];
+              }
+              narrow<T, F>(z0, u);
+              narrow<T, F>(z1, v);
+              *reinterpret_cast<W*>(y) = u;
+              *reinterpret_cast<W*>(y + (INTERLEAVED ? 1 : p.pairs)) = v;
+            }
+          }
+          load(h + ROT_BATCH * step);
+        }
+      }
+    }
+  }
+  if (idle) return;
+  // ---- copied units: what is not turned of a head, or all of it ---------------------------------------------------------------
   for (int ip = 0; ip < p.n_parts; ++ip) {
     const UaRotPart& q = p.part[ip];
-    const int per_token = q.heads * (q.rotate ? units : p.dim / V);
-    const T* src0 = static_cast<const T*>(q.src);
-    T* dst0 = static_cast<T*>(q.dst);
-#pragma unroll 2
-    for (int i = threadIdx.x; i < here * per_token; i += ROT_THREADS) {
-      const int t = i / per_token, in = i % per_token;
-      const int per_head = per_token / q.heads;
-      const int head = in / per_head;
-      int u = in % per_head;
-      const long tok = tok0 + t, b = tok / p.per_batch, s = tok % p.per_batch;
-      const T* src = src0 + b * q.src_batch + s * q.src_token + head * q.src_head;
-      T* dst = dst0 + head * q.dst_head;
-      if (q.paged) {
-        const long slot = dst_off[t];
-        if (slot < 0) continue;
-        dst += (slot >> p.page_shift) * q.dst_batch + (slot & ((1 << p.page_shift) - 1)) * q.dst_token;
-      } else {
-        dst += b * q.dst_batch + s * q.dst_token;
-      }
-      if (!q.rotate || u >= rot_units) {
-        const int e = q.rotate ? rot + (u - rot_units) * V : u * V;
-        *reinterpret_cast<Vec<T, V>*>(dst + e) = *reinterpret_cast<const Vec<T, V>*>(src + e);
-        continue;
-      }
-      const float2* w = cs + t * p.pairs;
-      if constexpr (INTERLEAVED) {
-        float x[E];
-        if constexpr (V > 1) {
-          const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(src + u * V);
+    const int first = q.rotate ? 2 * p.pairs : 0, units = (p.dim - first) / V;
+    const T* src;
+    T* dst;
+    if (units == 0 || !rows(ip, src, dst) || src == dst) continue;
+    const int lanes = units < 32 ? units : 32, per_pass = 32 / lanes, sub = lane / lanes, step = per_pass << p.split_shift;
+    if (sub >= per_pass) continue;
+    for (int unit = lane % lanes; unit < units; unit += lanes) {
+      const int heads = static_cast<int>(q.heads);
+      for (int h = slice * per_pass + sub; h < heads; h += ROT_BATCH * step) {
+        Vec<T, V> x[ROT_BATCH];
 #pragma unroll
-          for (int k = 0; k < V; ++k) x[k] = to_f(v.v[k]);
-        } else {
-          x[0] = to_f(src[u * 2]);
-          x[1] = to_f(src[u * 2 + 1]);
-        }
-        float y[E];
+        for (int i = 0; i < ROT_BATCH; ++i)
+          if (h + i * step < heads) x[i] = *reinterpret_cast<const Vec<T, V>*>(src + (h + i * step) * q.src_head + first + unit * V);
 #pragma unroll
-        for (int k = 0; k < E; k += 2) {
-          const float2 c = w[u * (E / 2) + k / 2];
-          y[k] = x[k] * c.x - x[k + 1] * c.y;
-          y[k + 1] = x[k + 1] * c.x + x[k] * c.y;
-        }
-        if constexpr (V > 1) {
-          Vec<T, V> o;
-#pragma unroll
-          for (int k = 0; k < V; ++k) o.v[k] = from_f<T>(y[k]);
-          *reinterpret_cast<Vec<T, V>*>(dst + u * V) = o;
-        } else {
-          dst[u * 2] = from_f<T>(y[0]);
-          dst[u * 2 + 1] = from_f<T>(y[1]);
-        }
-      } else {
-        const Vec<T, V> lo = *reinterpret_cast<const Vec<T, V>*>(src + u * V);
-        const Vec<T, V> hi = *reinterpret_cast<const Vec<T, V>*>(src + p.pairs + u * V);
-        Vec<T, V> a, b2;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float2 c = w[u * V + k];
-          const float x = to_f(lo.v[k]), y = to_f(hi.v[k]);
-          a.v[k] = from_f<T>(x * c.x - y * c.y);
-          b2.v[k] = from_f<T>(y * c.x + x * c.y);
-        }
-        *reinterpret_cast<Vec<T, V>*>(dst + u * V) = a;
-        *reinterpret_cast<Vec<T, V>*>(dst + p.pairs + u * V) = b2;
+        for (int i = 0; i < ROT_BATCH; ++i)
+          if (h + i * step < heads) *reinterpret_cast<Vec<T, V>*>(dst + (h + i * step) * q.dst_head + first + unit * V) = x[i];
       }
     }
   }
@@ -187,8 +285,8 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const __grid_consta
 template <typename T, bool INTERLEAVED>
 static int launch_rotary(const RotParams& p, bool wide, unsigned grid, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
-  if (wide) UA_CUDA(launch_kernel(rotary_kernel<T, V, INTERLEAVED>, grid, ROT_THREADS, 0, stream, true, p));
-  else UA_CUDA(launch_kernel(rotary_kernel<T, 1, INTERLEAVED>, grid, ROT_THREADS, 0, stream, true, p));
+  if (wide) UA_CUDA(launch_kernel(rotary_kernel<T, V, INTERLEAVED>, grid, ROT_WARPS * 32, 0, stream, true, p));
+  else UA_CUDA(launch_kernel(rotary_kernel<T, 1, INTERLEAVED>, grid, ROT_WARPS * 32, 0, stream, true, p));
   return 0;
 }
 
@@ -201,7 +299,8 @@ extern "C" int ua_rotary(const UaRotary* a, float magnitude, int* status, cudaSt
   if (a->n_parts < 0 || a->n_parts > 3) UA_FAIL("ua_rotary: %ld tensors (3 at most)", a->n_parts);
   if (a->pairs < 0 || a->pairs > ROT_MAX_PAIRS || 2 * a->pairs > a->dim)
     UA_FAIL("ua_rotary: %ld pairs in heads of %ld elements (%d pairs at most)", a->pairs, a->dim, ROT_MAX_PAIRS);
-  if (a->batch <= 0 || a->per_batch <= 0) return 0;
+  if (a->batch <= 0 || a->per_batch <= 0 || a->n_parts == 0) return 0;
+  if (a->pairs > 0 && (!a->part[0].rotate || a->part[0].paged)) UA_FAIL("ua_rotary: the first tensor has to be a turned one outside the cache");
   RotParams p;
   memset(&p, 0, sizeof(p));
   // 16 bytes at a time where every row of every tensor starts on 16 bytes and the parts of a head are whole vectors
@@ -227,8 +326,13 @@ extern "C" int ua_rotary(const UaRotary* a, float magnitude, int* status, cudaSt
   p.magnitude = magnitude;
   p.inverse = static_cast<int>(a->inverse);
   p.status = status;
-  p.block_tokens = 1;
-  const unsigned grid = static_cast<unsigned>((p.tokens + p.block_tokens - 1) / p.block_tokens);
+  const int v = wide ? V : 1;
+  p.rot_units = a->interleaved ? 2 * p.pairs / (v == 1 ? 2 : v) : p.pairs / v;
+  p.rot_lanes = p.rot_units < 32 ? (p.rot_units > 0 ? p.rot_units : 1) : 32;
+  // A warp for each token; two, four or eight as long as those are few: each finds the angles anew (1000 tokens, there and back: up to 8
+  // warps of an SM 9.3 us, 16 9.6, 40 13.8; 24 tokens with their keys and values into the cache: 8 warps a token 3.7).
+  while (p.split_shift < 3 && (p.tokens << (p.split_shift + 1)) <= ROT_SHARES * sm_count()) ++p.split_shift;
+  const unsigned grid = static_cast<unsigned>(((p.tokens << p.split_shift) + ROT_WARPS - 1) / ROT_WARPS);
   switch (a->dtype * 2 + (a->interleaved ? 1 : 0)) {
     case 0: return launch_rotary<__nv_bfloat16, false>(p, wide, grid, stream);
     case 1: return launch_rotary<__nv_bfloat16, true>(p, wide, grid, stream);
