@@ -368,6 +368,25 @@ def test_attention_window(device, name, left, sink, page):
     _check(_dev(device), *BATCHES[name], 8, 2, page, left, sink)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,heads,page", [(1, 32, 64), (1, 32, 16), (3, 32, 64), (12, 32, 64)])
+def test_attention_many_requests(new, heads, page):
+    """A batch that keeps the memory busy: loads of a CTA's tiles come late and in another order than they are asked for in. The
+    lengths end inside tiles; each run has to give the same bits, and those of the requests alone."""
+    dev = _dev("cuda")
+    g = torch.Generator().manual_seed(new)
+    context = [int(x) for x in torch.exp(torch.empty(48).uniform_(math.log(40), math.log(16000), generator=g))]
+    q, kc, vc, table, ctx, cu, keys, values = _problem(dev, context, [new] * 48, heads, 8, page)
+    o, lse = ua.paged_attention(q, kc, vc, table, ctx, cu, most_new=new)
+    for r in range(0, 48, 7):
+        sl = slice(r * new, (r + 1) * new)
+        _close(o[sl], lse[:, sl], *_exact(q[sl], keys[r], values[r], context[r], new, 128 ** -0.5, -1, 0))
+    for _ in range(20):
+        o2, lse2 = ua.paged_attention(q, kc, vc, table, ctx, cu, most_new=new)
+        assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    A.check_status(dev)
+
+
 @pytest.mark.parametrize("device", ["cpu", CUDA])
 def test_attention_ignores_pages_outside_the_window(device):
     """Pages that no query sees any more may be given back: their entries name no page, or one that holds anything."""

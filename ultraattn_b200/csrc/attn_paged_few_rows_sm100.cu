@@ -231,14 +231,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __g
         for (int t = it.first[e]; t < t_end; ++t, ++j) {
           if ((j & 1) != static_cast<uint32_t>(w)) continue;
           const bool edge = t < clear_first || t >= clear_end;
-          if (edge) {
+          ok = mbar_wait_quiet(&s.s_full[w], cnt & 1, wc) && ok;
+          ++cnt;
+          tc_fence_after_sync();
+          if (edge) {          // (behind the scores: their issue means that the values before these in the stage have come, so that the parity is theirs)
             const uint32_t g = kv + j;
             clear_unseen(s.v[g % STAGES], &s.v_full[g % STAGES], (g / STAGES) & 1, it.lo[e] - t * PT, it.hi[e] - t * PT, threadIdx.x & 127, 128,
                          wc.abort_flag, p.status);
           }
-          ok = mbar_wait_quiet(&s.s_full[w], cnt & 1, wc) && ok;
-          ++cnt;
-          tc_fence_after_sync();
           float sv[N];
           tmem_ld_n<N>(tS, reinterpret_cast<uint32_t(&)[N]>(sv));
           tmem_wait_ld();

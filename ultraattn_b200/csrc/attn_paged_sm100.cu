@@ -388,15 +388,17 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
 #pragma unroll 1
           for (; t < t_end; ++t, ++j) {
             if (FEW && (j & 1) != static_cast<uint32_t>(w)) continue;
-            // (of two sub-tiles the first does it: its product is issued before the other's; a tile with such keys is clear for no warp)
+            ok = mbar_wait_quiet(&s.s_full[w], cnt & 1, wc);
+            ++cnt;
+            tc_fence_after_sync();
+            // (Behind the scores: FEW: their issue means that the values before these in the stage have come, so that the parity is theirs; else
+            // P V of the tile before last is complete. Of two sub-tiles the first does it: its product is issued before the other's. A tile
+            // with such keys is clear for no warp.)
             if ((FEW || w == 0) && (t < clear_first || t >= clear_end)) {
               const uint32_t g = kv + j;
               clear_unseen(s.v[g % STAGES], &s.v_full[g % STAGES], (g / STAGES) & 1, it.lo[e] - t * PT, it.hi[e] - t * PT, threadIdx.x - w * PT,
                            act_warps * 32, wc.abort_flag, p.status);
             }
-            ok = mbar_wait_quiet(&s.s_full[w], cnt & 1, wc);
-            ++cnt;
-            tc_fence_after_sync();
             if (t < some_first || t >= some_end) {
               // nothing to see for these 32 rows: P = 0, maximum and sum stay
               if (!FEW) mbar_arrive_warp(&s.s_free);
