@@ -129,7 +129,32 @@ def test_gradient_against_differences():
     pos = torch.tensor([0, 1, 777, 123456])
     for inter in (False, True):
         f, m = ua.rotary_frequencies(8, scaling="yarn", factor=2.0)
-        assert torch.autograd.gradcheck(lambda a, b: ua.rotary(a, b, pos, f, interleaved=inter, magnitude=m), (q, k))
+        turn = lambda a, b: ua.rotary(a, b, pos, f, interleaved=inter, magnitude=m)
+        assert torch.autograd.gradcheck(turn, (q, k)) and torch.autograd.gradgradcheck(turn, (q, k))
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_gradients_of_parts(device):
+    """Only one of the outputs used, gradients that are one number seen by all, gradients of gradients, inputs that need none."""
+    dev = _dev(device)
+    g = torch.Generator().manual_seed(6)
+    q, k = (torch.randn(5, n, 64, generator=g).to(dev).requires_grad_() for n in (4, 2))
+    pos, f = torch.arange(5, device=dev) * 1000, ua.rotary_frequencies(64, device=dev)[0]
+    q2, k2 = ua.rotary(q, k, pos, f)
+    ones = torch.ones_like(q)
+    want = _exact(ones, pos, f, inverse=True)
+    dq, dk = torch.autograd.grad(q2.sum(), (q, k), allow_unused=True, retain_graph=True)
+    _assert_close(dq, ones, want, 32, 1.0, False)
+    assert dk is None or not dk.any()
+    # d/dq of <dq'(q), dq'(q)> with dq' = R q: the rotation there and back
+    (g1,) = torch.autograd.grad(q2, q, q2, create_graph=True, retain_graph=True)
+    assert torch.allclose(g1, q, rtol=1e-5, atol=1e-5)
+    (g2,) = torch.autograd.grad(g1.sum(), q)
+    assert torch.allclose(g2, ones, rtol=1e-5, atol=1e-5)
+    with torch.no_grad():
+        assert not ua.rotary(q, k, pos, f)[0].requires_grad
+    frozen = ua.rotary(q.detach(), k, pos, f)
+    assert torch.autograd.grad(frozen[1].sum(), k)[0].shape == k.shape
 
 
 @pytest.mark.parametrize("device", ["cpu", CUDA])

@@ -399,6 +399,23 @@ def _native(*tensors) -> bool:
             and _lib.host() is not None)
 
 
+_status_ptr: dict[int, int] = {}
+
+
+def _native_call(t: torch.Tensor):
+    """(native host part, status word, stream) for a call on ``t``'s device; None: there is no native part, or the device is not the
+    current one. The part itself looks at the tensors."""
+    idx = t.get_device()
+    if idx < 0 or idx != torch._C._cuda_getDevice():
+        return None
+    host = _lib.host()
+    if host is None:
+        return None
+    if idx not in _status_ptr:
+        _status_ptr[idx] = status_buffer(t.device).data_ptr()
+    return host, _status_ptr[idx], torch._C._cuda_getCurrentRawStream(idx)
+
+
 def dense_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, softmax_scale: float | None = None):
     """(O, lse) of :func:`attn_fwd_dense`, in new tensors."""
     if _native(q, k, v):

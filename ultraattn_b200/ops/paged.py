@@ -28,7 +28,7 @@ import torch
 
 from .. import _lib
 from . import rotary as R
-from .attention import KERNEL_HEAD_DIM, _native, status_buffer
+from .attention import KERNEL_HEAD_DIM, _native_call, status_buffer
 
 MAX_REQUESTS = 8192
 _ATTN = struct.Struct("30q")          # struct UaPagedAttn of csrc/paged_args.h
@@ -84,10 +84,10 @@ def assign_pages(context_lens, new_lens, block_table, free_pages, free_count, *,
     ``free_count`` itself is not changed unless it is given as ``count_out`` too; else the pages left are in the result
     alone. All int32. A new token in front of position 0 (``new > context``) gets no slot. If the pages do not suffice, or a row of
     the table, or ``tokens``, nothing is assigned: every slot is -1, ``cu_new`` is 0 (and the error reported, see above)."""
-    if _native(block_table, context_lens, new_lens, free_pages, free_count):
-        with _lib.on_device(block_table):
-            r = _lib.host().assign_pages(context_lens, new_lens, block_table, free_pages, free_count, page_size, tokens, count_out, MAX_REQUESTS,
-                                         status_buffer(block_table.device).data_ptr(), _lib.stream_of(block_table))
+    native = _native_call(block_table)
+    if native is not None:
+        r = native[0].assign_pages(context_lens, new_lens, block_table, free_pages, free_count, page_size, tokens, count_out, MAX_REQUESTS, native[1],
+                                   native[2])
         if r is not None:
             _lib.LAUNCHES[0] += 1
             return PagedStep(*r)
@@ -142,10 +142,9 @@ def release_pages(ended, context_lens, block_table, free_pages, free_count, *, p
     onto the stack ``free_pages``, in the order of the requests; the table itself is left as it is. Returns the number
     of free pages, in ``count_out`` if given (``free_count`` itself may be). If the stack has no room for them (a page given
     back twice), nothing changes and the error is reported."""
-    if _native(block_table, ended, context_lens, free_pages, free_count):
-        with _lib.on_device(block_table):
-            r = _lib.host().release_pages(ended, context_lens, block_table, free_pages, free_count, page_size, count_out, MAX_REQUESTS,
-                                          status_buffer(block_table.device).data_ptr(), _lib.stream_of(block_table))
+    native = _native_call(block_table)
+    if native is not None:
+        r = native[0].release_pages(ended, context_lens, block_table, free_pages, free_count, page_size, count_out, MAX_REQUESTS, native[1], native[2])
         if r is not None:
             _lib.LAUNCHES[0] += 1
             return r
@@ -189,10 +188,9 @@ def rotary_append(q, k, v, pos, slots, k_cache, v_cache, inv_freq=None, *, inter
     fp32). A token whose slot is negative is not written to the cache. ``inv_freq``, ``interleaved``, ``magnitude`` as in
     :func:`ultraattn_b200.rotary`; without ``inv_freq`` nothing is turned. Returns the queries, in ``q_out`` if given (``q``
     itself: in place). Slots must differ: of two tokens with the same slot either may end up in it."""
-    if inv_freq is not None and q_out is None and _native(q, k, v, pos, slots, k_cache, v_cache, inv_freq):
-        with _lib.on_device(q):
-            r = _lib.host().rotary_append(q, k, v, pos, slots, k_cache, v_cache, inv_freq, interleaved, magnitude,
-                                          status_buffer(q.device).data_ptr(), _lib.stream_of(q))
+    native = _native_call(q) if inv_freq is not None and q_out is None else None
+    if native is not None:
+        r = native[0].rotary_append(q, k, v, pos, slots, k_cache, v_cache, inv_freq, interleaved, magnitude, native[1], native[2])
         if r is not None:
             _lib.LAUNCHES[0] += 1
             return r
@@ -288,11 +286,11 @@ def paged_attention(q, k_cache, v_cache, block_table, context_lens, cu_new, *, m
     ``o [tokens, heads, 128]`` bf16 and ``lse [heads, tokens]`` fp32, in ``out = (o, lse)`` if given; rows behind the
     last request are not written. A query that sees no key (``context < n``) gives 0 and -inf. What the cache holds in places that no
     query of a request sees (behind its last token, in pages before its window) does not matter, NaN included. Forward only."""
-    if out is None and window_size[1] in (0, -1) and _native(q, k_cache, v_cache, block_table, context_lens, cu_new):
-        with _lib.on_device(q):
-            r = _lib.host().paged_attention(q, k_cache, v_cache, block_table, context_lens, cu_new, q.shape[0] if most_new is None else most_new,
-                                            q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale, window_size[0], sink_tokens, MAX_REQUESTS,
-                                            status_buffer(q.device).data_ptr(), _lib.stream_of(q))
+    native = _native_call(q) if out is None and window_size[1] in (0, -1) else None
+    if native is not None:
+        r = native[0].paged_attention(q, k_cache, v_cache, block_table, context_lens, cu_new, q.shape[0] if most_new is None else most_new,
+                                      q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale, window_size[0], sink_tokens, MAX_REQUESTS,
+                                      native[1], native[2])
         if r is not None:
             _lib.LAUNCHES[0] += 2
             return r

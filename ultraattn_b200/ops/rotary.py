@@ -18,6 +18,7 @@ import struct
 import torch
 
 from .. import _lib
+from .attention import _native_call, status_buffer
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _MAX_PAIRS = 256
@@ -124,7 +125,6 @@ def part(src, dst, rotate=True, paged=False) -> tuple:
 
 def launch(parts, like, pos, inv_freq, interleaved, magnitude, inverse=False, slots=None, page_shift=0, n_slots=0) -> None:
     """``ua_rotary`` over the tokens of ``like``."""
-    from .attention import status_buffer
     batch, tokens = (1, like.shape[0]) if like.dim() == 3 else like.shape[:2]
     ps = (0, pos.stride(0)) if pos.dim() == 1 else pos.stride()
     pairs = 0 if inv_freq is None else inv_freq.shape[0]
@@ -170,30 +170,21 @@ def rotate(tensors, pos, inv_freq, *, interleaved: bool = False, magnitude: floa
     return dst
 
 
-def _rotate_pair(q, k, pos, inv_freq, interleaved, magnitude, inverse):
-    from .attention import _native, status_buffer
-    if _native(q, k, pos, inv_freq):
-        with _lib.on_device(q):
-            r = _lib.host().rotate_pair(q, k, pos, inv_freq, interleaved, magnitude, inverse, status_buffer(q.device).data_ptr(), _lib.stream_of(q))
-        if r is not None:
-            _lib.LAUNCHES[0] += 1
-            return r
-    return rotate((q, k), pos, inv_freq, interleaved=interleaved, magnitude=magnitude, inverse=inverse)
-
-
 class _Rotary(torch.autograd.Function):
+    """The gradient is the rotation the other way, by the same function: it has a gradient itself."""
+
     @staticmethod
-    def forward(ctx, q, k, pos, inv_freq, interleaved, magnitude):
+    def forward(ctx, q, k, pos, inv_freq, interleaved, magnitude, inverse):
         ctx.save_for_backward(pos, inv_freq)
-        ctx.form = (interleaved, magnitude)
-        return _rotate_pair(q, k, pos, inv_freq, interleaved, magnitude, False)
+        ctx.form = (interleaved, magnitude, inverse)
+        return rotate((q, k), pos, inv_freq, interleaved=interleaved, magnitude=magnitude, inverse=inverse)
 
     @staticmethod
     def backward(ctx, dq, dk):
         pos, inv_freq = ctx.saved_tensors
-        interleaved, magnitude = ctx.form
-        dq, dk = _rotate_pair(dq, dk, pos, inv_freq, interleaved, magnitude, True)
-        return dq, dk, None, None, None, None
+        interleaved, magnitude, inverse = ctx.form
+        dq, dk = _Rotary.apply(dq, dk, pos, inv_freq, interleaved, magnitude, not inverse)
+        return dq, dk, None, None, None, None, None
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False,
@@ -204,6 +195,12 @@ def rotary(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, inv_freq: torch.
     packed projection among them) with ``pos [tokens]``, or all of them with a leading batch axis; ``pos`` int32 or int64;
     ``inv_freq``, ``magnitude`` from :func:`rotary_frequencies`. bf16, fp16 or fp32 on CUDA, any float type on CPU; results and
     gradients are contiguous and of the inputs' type, computed in fp32."""
+    native = _native_call(q)
+    if native is not None:
+        r = native[0].rotate_pair(q, k, pos, inv_freq, interleaved, magnitude, native[1], native[2])
+        if r is not None:
+            _lib.LAUNCHES[0] += 1           # (the backward, which need not run, is not counted)
+            return r
     if q.dim() != k.dim() or q.shape[:-2] != k.shape[:-2]:
         raise ValueError(f"queries {tuple(q.shape)} and keys {tuple(k.shape)} have different tokens")
-    return _Rotary.apply(q, k, pos, inv_freq, bool(interleaved), float(magnitude))
+    return _Rotary.apply(q, k, pos, inv_freq, bool(interleaved), float(magnitude), False)
