@@ -1,0 +1,162 @@
+"""The model's serving step on the paged cache against its whole forward, and its general rotary embedding in training."""
+import pytest
+import torch
+
+import ultraattn_b200 as ua
+from ultraattn_b200 import patterns as P
+from ultraattn_b200.models.llama import LlamaConfig, LlamaModel, _QkvRotary, _split_heads
+from ultraattn_b200.ops import attention as A
+from ultraattn_b200.ops import gemm as G
+
+CUDA = pytest.param("cuda", marks=pytest.mark.gpu)
+FORMS = {
+    "plain": {},
+    "window": dict(sliding_window=24, sink_tokens=0),
+    "window and sinks": dict(sliding_window=24, sink_tokens=3),
+    "stretched": dict(rope_scaling="yarn", rope_factor=4.0, rope_original_context=32),
+    "part of the head, adjacent pairs": dict(rope_dim=64, rope_interleaved=True),
+}
+
+
+def _model(device, **form):
+    if device == "cuda" and not torch.cuda.is_available():
+        pytest.skip("needs a CUDA GPU")
+    # (weights of 0.1: at 0.02 all tokens come out nearly alike)
+    cfg = LlamaConfig(n_layers=2, hidden=256, n_heads=4, n_kv_heads=2, head_dim=128, ffn=512, vocab=512, init_std=0.1, **form)
+    return LlamaModel(cfg, device=torch.device(device), pattern=P.causal(1), seed=3)
+
+
+def _whole(model, ids):
+    """Logits behind the last token of one sequence, by the training forward."""
+    with torch.no_grad():
+        h = model.hidden_states(ids)
+        return G.gemm(h[-1:].contiguous(), model.p["lm_head"])[0]
+
+
+def _steps(model, sequences, plan, page, pages, graph=False):
+    """Serves ``sequences`` as ``plan`` says (new tokens of every request, step by step) and compares every step's logits with
+    the whole forward over what has been fed so far."""
+    dev, n = model.device, len(sequences)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    cache = model.paged_cache(pages, page)
+    for k, v in cache:
+        k.fill_(float("nan")), v.fill_(float("nan"))
+    table = torch.full((n, 16), -1, dtype=torch.int32, device=dev)
+    free, count = torch.randperm(pages, generator=torch.Generator().manual_seed(1)).to(torch.int32).to(dev), i32([pages])
+    fed = [0] * n
+    for new in plan:
+        ids = torch.cat([s[f:f + k] for s, f, k in zip(sequences, fed, new)] + [sequences[0][:2]])      # two rows of padding
+        fed = [f + k for f, k in zip(fed, new)]
+        context = i32(fed)
+        step = ua.paged.assign_pages(context, i32(new), table, free, count, page_size=page, tokens=len(ids), count_out=count)
+        logits = model.paged_logits(ids, cache, table, context, step, most_new=max(new))
+        for r in range(n):
+            if new[r] == 0:
+                continue
+            want = _whole(model, sequences[r][:fed[r]]).float()
+            got = logits[r].float()
+            # two layers of bf16 activations: each of some ten roundings is off by 2^-8 of its value at most, 2^-8 * sqrt(20) together if
+            # they are independent, 3 times that allowed; fp32 on the CPU
+            rel = float((got - want).norm() / want.norm())
+            assert rel < (3 * 20 ** 0.5 * 2.0 ** -8 if dev.type == "cuda" else 1e-4), (r, fed[r], rel)
+    left = ua.paged.release_pages(torch.ones(n, dtype=torch.bool, device=dev), i32(fed), table, free, count, page_size=page)
+    assert int(left) == pages and sorted(free.tolist()) == list(range(pages))
+    if dev.type == "cuda":
+        A.check_status(dev)
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+@pytest.mark.parametrize("form", FORMS)
+def test_serving_steps(device, form):
+    model = _model(device, **FORMS[form])
+    g = torch.Generator().manual_seed(2)
+    seqs = [torch.randint(0, 512, (90,), generator=g).to(model.device) for _ in range(3)]
+    plan = [[40, 0, 7], [1, 33, 1], [1, 1, 1], [17, 1, 0], [1, 1, 40], [1, 1, 1]]
+    _steps(model, seqs, plan, 16, 24)
+
+
+@pytest.mark.gpu
+def test_decoding_step_in_a_graph():
+    """One captured step, replayed while the requests grow over pages' ends: lengths, tokens and pages are data."""
+    model = _model("cuda")
+    dev, n, page, pages = model.device, 3, 16, 24
+    g = torch.Generator().manual_seed(4)
+    seqs = torch.randint(0, 512, (n, 60), generator=g).to(dev)
+    cache, table = model.paged_cache(pages, page), torch.full((n, 8), -1, dtype=torch.int32, device=dev)
+    free, count = torch.arange(pages, dtype=torch.int32, device=dev), torch.tensor([pages], dtype=torch.int32, device=dev)
+    context, one = torch.tensor([29, 13, 5], dtype=torch.int32, device=dev), torch.ones(n, dtype=torch.int32, device=dev)
+    fed = context.tolist()
+    step = ua.paged.assign_pages(context, context, table, free, count, page_size=page, tokens=sum(fed), count_out=count)
+    model.paged_logits(torch.cat([s[:f] for s, f in zip(seqs, fed)]), cache, table, context, step)
+    ids = torch.zeros(n, dtype=torch.long, device=dev)
+
+    def decode():
+        context.add_(1)
+        st = ua.paged.assign_pages(context, one, table, free, count, page_size=page, tokens=n, count_out=count)
+        return model.paged_logits(ids, cache, table, context, st, most_new=1)
+
+    saved = [x.clone() for x in (context, table, count)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        decode()                                        # (a warm-up outside the graph)
+    torch.cuda.current_stream().wait_stream(side)
+    for x, y in zip((context, table, count), saved):
+        x.copy_(y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        logits = decode()
+    for x, y in zip((context, table, count), saved):
+        x.copy_(y)
+    for i in range(8):
+        ids.copy_(torch.stack([s[f] for s, f in zip(seqs, fed)]))
+        graph.replay()
+        fed = [f + 1 for f in fed]
+        for r in range(n):
+            want = _whole(model, seqs[r][:fed[r]]).float()
+            assert float((logits[r].float() - want).norm() / want.norm()) < 3 * 20 ** 0.5 * 2.0 ** -8
+    assert context.tolist() == fed
+    A.check_status(dev)
+
+
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_projection_split_and_turned(device):
+    """_QkvRotary against autograd through views and ua.rotary."""
+    if device == "cuda" and not torch.cuda.is_available():
+        pytest.skip("needs a CUDA GPU")
+    dev = torch.device(device)
+    dtype = torch.bfloat16 if device == "cuda" else torch.float32
+    g = torch.Generator().manual_seed(7)
+    qkv = torch.randn(19, 8 * 64, generator=g).to(dtype).to(dev)
+    grads = [torch.randn(19, n, 64, generator=g).to(dtype).to(dev) for n in (4, 2, 2)]
+    pos = torch.arange(19, device=dev) * 333
+    f, m = ua.rotary_frequencies(48, scaling="yarn", factor=2.0, device=dev)
+    a, b = qkv.clone().requires_grad_(), qkv.clone().requires_grad_()
+    got = _QkvRotary.apply(a, f, m, True, pos, 4, 2, 64)
+    q, k, v = _split_heads(b, 4, 2, 64)
+    want = (*ua.rotary(q, k, pos, f, interleaved=True, magnitude=m), v)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    assert torch.equal(torch.autograd.grad(got, a, grads)[0], torch.autograd.grad(want, b, grads)[0])
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_training_with_the_general_embedding(device):
+    """All of the head in halves is what the plain path computes (from fp32 tables): same loss and gradients; a stretched one trains."""
+    ids = torch.randint(0, 512, (65,), generator=torch.Generator().manual_seed(8))
+    models = [_model(device), _model(device, rope_dim=128)]
+    assert models[1].cfg.general_rotary and not models[0].cfg.general_rotary
+    out = []
+    for m in models:
+        x = ids.to(m.device)
+        loss = m.loss(x[:-1], x[1:])
+        loss.backward()
+        out.append((float(loss.detach()), m.flat_grad.float().clone()))
+    # bf16: one rounding of q and k that falls the other way where the tables' angles are off by 2^-24 * 64; fp32 on the CPU
+    tol = 2.0 ** -7 if device == "cuda" else 1e-5
+    assert abs(out[0][0] - out[1][0]) < tol * abs(out[0][0])
+    assert float((out[0][1] - out[1][1]).norm() / out[0][1].norm()) < tol
+    m = _model(device, rope_scaling="bands", rope_factor=4.0, rope_original_context=16)
+    x = ids.to(m.device)
+    assert m.train_step(x[:-1], x[1:]) > 0 and torch.isfinite(m.flat.float()).all()

@@ -27,6 +27,7 @@ template <int ROWS> constexpr int PA_ITEM_TILES = ROWS <= 32 ? 1 : 3;
 // An item of fewer tiles is not cut: the border moves to its nearer end. Writing and merging the fp32 parts of 256 rows takes as long as
 // six to eight key tiles of them, those of 16 rows nothing.
 template <int ROWS> constexpr int PA_WHOLE = ROWS <= 32 ? 0 : ROWS == 128 ? 8 : 20;
+template <int ROWS> constexpr int PA_SNAP = ROWS <= 32 ? 0 : ROWS == 128 ? 3 : 6;     // nor are fewer tiles of an item cut off
 constexpr int PA_MIN_SHARE = 2;               // key tiles of a CTA at least
 
 // (Every block copies these into its shared memory before it waits for the kernel in front of it: parameters that have not been
@@ -67,6 +68,7 @@ static_assert(sizeof(PagedScalars) % 4 == 0 && sizeof(PagedScalars) <= 64 * 4, "
 // rows (1 - 3); 4: the part of one that began before (0 none, 1 goes on, 2 ends)
 constexpr int PA_DESC = 8;
 
+constexpr int PA_DEAL = 8;                    // see PagedWalk::start
 constexpr int PA_NO_PAGE = -0x7FFFFFFF;
 constexpr int PA_ITEMS = 3;                   // items in shared memory: the one before may still be written out
 
@@ -178,6 +180,7 @@ struct PagedWalk {
   int r, head, tile;
   int same;                  // a window: the weight of every item of the request (0: key tiles and PA_ITEM_TILES)
   PagedRequest<ROWS> q;
+  int deal = 0, dealt, deal_cta, deal_ctas;      // items dealt out whole (0: equal shares), rounds so far
   int ahead[3];              // cu_new[r + 1], cu_new[r + 2], context[r + 1]: a request's lengths are loaded while the one before is walked
 
   __device__ __forceinline__ void look_ahead(const PagedScalars& p) {
@@ -218,8 +221,28 @@ struct PagedWalk {
     before -= mine;
     // as many CTAs as have a share worth its start
     const long most = total / PA_MIN_SHARE;
-    const int ctas = static_cast<int>(most < 1 ? 1 : most < all_ctas ? most : all_ctas);
-    if (total == 0 || cta >= ctas) return false;
+    int ctas = static_cast<int>(most < 1 ? 1 : most < all_ctas ? most : all_ctas);
+    if (total == 0) return false;
+    if (ROWS == 256 && p.requests == 1) {
+      // One request. A chunk behind a long context: all items have about the same keys, and as many CTAs as give each the same number of equal
+      // parts walk them in step, so that a key tile comes out of DRAM once for all (512 queries behind 32768 keys, 64 items, on the
+      // device: 148 equal shares 265 us, 128 of them 260).
+      q = paged_request<ROWS>(p, 0, false);
+      const int items = p.kv_heads * q.row_tiles, whole = ctas / items * items;
+      if (5 * whole >= 4 * ctas) ctas = whole;
+      // A prompt: many items, the first of few keys. Whole ones dealt out from the longest on, every other round backwards, end as evenly, and
+      // nothing has to be merged (8192 tokens, 32 / 8 heads: 505 us in equal shares, 487 so).
+      PagedItem first;
+      if (p.left < 0 && items >= 2 * ctas && q.tiles(p, 0, first) <= PA_DEAL) {
+        deal = items;
+        dealt = 0;
+        deal_cta = cta;
+        deal_ctas = ctas;
+        r = 0;
+        return true;
+      }
+    }
+    if (cta >= ctas) return false;
     const auto border = [&](int k) -> long {            // total * k / ctas; (a 64-bit division is a hundred instructions)
       if (total >> 32) return total * k / ctas;
       const unsigned t = static_cast<unsigned>(total), d = t / ctas, rest = t % ctas;
@@ -263,13 +286,25 @@ struct PagedWalk {
   }
   // the next piece of this share; false: there is none. `part`: 0 whole item, 1 its beginning, 2 its middle, 3 its end
   __device__ __forceinline__ bool next(const PagedScalars& p, PagedItem& it, int& part) {
+    if (ROWS == 256 && deal > 0) {
+      const int i = dealt * deal_ctas + (dealt & 1 ? deal_ctas - 1 - deal_cta : deal_cta);
+      ++dealt;
+      if (i >= deal) return false;
+      it.total = q.tiles(p, q.row_tiles - 1 - i / p.kv_heads, it);
+      it.q_row = q.q_row;
+      it.kv_head = i % p.kv_heads;
+      it.past = q.past;
+      it.request = 0;
+      part = 0;
+      return true;
+    }
     while (r < p.requests && s < x1) {
       const int total = q.tiles(p, tile, it);
       const long e = s + (same > 0 ? same : PA_ITEM_TILES<ROWS> + total);
       const auto cut = [&](long x) -> int {
         if (total < PA_WHOLE<ROWS>) return 2 * (x - s) > e - s ? total : 0;
         const long t = x - s - PA_ITEM_TILES<ROWS>;
-        return x >= e || t > total ? total : t < 0 ? 0 : static_cast<int>(t);
+        return x >= e || t > total - PA_SNAP<ROWS> ? total : t < PA_SNAP<ROWS> ? 0 : static_cast<int>(t);
       };
       const int t0 = cut(x0), t1 = cut(x1);
       const bool valid = t1 > t0 || (total == 0 && x0 < e && e <= x1);

@@ -33,6 +33,8 @@ import torch.nn.functional as F
 from .. import api
 from ..ops import elementwise as E
 from ..ops import gemm as G
+from ..ops import paged
+from ..ops import rotary as R
 from ..patterns.blocks import BSA_Repr
 
 
@@ -50,10 +52,20 @@ class LlamaConfig:
     init_std: float = 0.02
     sliding_window: Optional[int] = None     # Mistral: every query sees itself and the sliding_window - 1 tokens before it
     sink_tokens: int = 0                     # with a sliding window: leading tokens that stay visible (streaming)
+    rope_scaling: Optional[str] = None       # stretched contexts: "linear", "ntk", "yarn", "bands" (ops/rotary.py)
+    rope_factor: float = 1.0
+    rope_original_context: int = 4096        # tokens that the angles were trained on
+    rope_dim: Optional[int] = None           # rotated elements of a head (default: all)
+    rope_interleaved: bool = False           # pairs (2 i, 2 i + 1) instead of (i, i + half)
 
     @property
     def kv_heads(self) -> int:
         return self.n_kv_heads or self.n_heads
+
+    @property
+    def general_rotary(self) -> bool:
+        """The rotary embedding is not the plain one of ``ops.elementwise.rope``."""
+        return self.rope_scaling is not None or self.rope_dim is not None or self.rope_interleaved
 
     @classmethod
     def llama2_7b(cls) -> "LlamaConfig":
@@ -183,6 +195,35 @@ class _QkvRope(torch.autograd.Function):
         E.rope(dk.contiguous(), cos, sin, pos, inverse=True, out=dqkv[:, nq:nq + nk].unflatten(1, (Hk, D)))
         dqkv[:, nq + nk:].unflatten(1, (Hk, D)).copy_(dv)
         return dqkv, None, None, None, None, None
+
+
+class _QkvRotary(torch.autograd.Function):
+    """:class:`_QkvRope` with the general rotary embedding (ops/rotary.py): q and k are turned from their column ranges in one
+    launch, and in the backward turned back into their ranges of dqkv. Any head dim."""
+
+    @staticmethod
+    def forward(ctx, qkv, inv_freq, magnitude, interleaved, pos, n_heads, n_kv_heads, head_dim):
+        ctx.save_for_backward(inv_freq, pos)
+        ctx.form = (magnitude, interleaved, n_heads, n_kv_heads, head_dim)
+        q, k, v = _split_heads(qkv, n_heads, n_kv_heads, head_dim)
+        q, k = R.rotate((q, k), pos, inv_freq, interleaved=interleaved, magnitude=magnitude)
+        return q, k, v
+
+    @staticmethod
+    def backward(ctx, dq, dk, dv):
+        inv_freq, pos = ctx.saved_tensors
+        magnitude, interleaved, n_heads, n_kv_heads, head_dim = ctx.form
+        dqkv = torch.empty(dq.shape[0], (n_heads + 2 * n_kv_heads) * head_dim, dtype=dq.dtype, device=dq.device)
+        q, k, v = _split_heads(dqkv, n_heads, n_kv_heads, head_dim)
+        R.rotate((dq, dk), pos, inv_freq, interleaved=interleaved, magnitude=magnitude, inverse=True, out=(q, k))
+        v.copy_(dv)
+        return dqkv, None, None, None, None, None, None, None
+
+
+def _split_heads(qkv, n_heads, n_kv_heads, head_dim):
+    """The q, k and v heads of a packed projection, as views."""
+    x = qkv.unflatten(1, (n_heads + 2 * n_kv_heads, head_dim))
+    return x[:, :n_heads], x[:, n_heads:n_heads + n_kv_heads], x[:, n_heads + n_kv_heads:]
 
 
 class _Swiglu(torch.autograd.Function):
@@ -324,6 +365,8 @@ class LlamaModel:
         if cfg.sliding_window is not None and (runtime is not None or (seq_algo != "halo" and group is not None)):
             raise NotImplementedError("a token-exact sliding window runs on one device or with seq_algo='halo' "
                                       "(contiguous shards); in the planner-driven runtimes express it as a block pattern")
+        if cfg.general_rotary and seq_algo == "ulysses" and group is not None:
+            raise NotImplementedError("the head-parallel projections turn q and k with the plain rotary embedding")
         if seq_algo == "halo":
             assert cfg.sliding_window is not None and not cfg.sink_tokens, \
                 "seq_algo='halo' is the strategy of a sliding window (without sink tokens)"
@@ -399,6 +442,7 @@ class LlamaModel:
         self.m = torch.zeros_like(self.master)
         self.v = torch.zeros_like(self.master)
         self.cos, self.sin = None, None
+        self._rotary = None
         self.max_pos = max_pos
         if seq_algo == "ulysses" and self.world > 1:
             from ..parallel.ulysses_fused import FusedUlyssesAttention
@@ -414,12 +458,24 @@ class LlamaModel:
             self.cos, self.sin = E.rope_tables(n_pos, self.cfg.head_dim, self.cfg.rope_base, self.device)
         return self.cos, self.sin
 
+    def _angles(self):
+        """(inv_freq, magnitude) of the rotary embedding."""
+        c = self.cfg
+        if self._rotary is None:
+            self._rotary = R.rotary_frequencies(c.rope_dim or c.head_dim, c.rope_base, scaling=c.rope_scaling, factor=c.rope_factor,
+                                                original_context=c.rope_original_context, device=self.device)
+        return self._rotary
+
     def _seg_qkv(self, x, li):
         c, p = self.cfg, self.p
         h = _RMSNorm.apply(x, p[f"l{li}.norm1"], c.eps)
         qkv = _Linear.apply(h, p[f"l{li}.wqkv"])
         T = x.shape[0]
         nq, nk = c.n_heads * c.head_dim, c.kv_heads * c.head_dim
+        if c.general_rotary:
+            inv_freq, magnitude = self._angles()
+            q, k, v = _QkvRotary.apply(qkv, inv_freq, magnitude, c.rope_interleaved, self._pos, c.n_heads, c.kv_heads, c.head_dim)
+            return q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)
         if qkv.is_cuda and c.head_dim == 128:
             cos, sin = self._tables(self._n_pos)
             q, k, v = _QkvRope.apply(qkv, cos, sin, self._pos, c.n_heads, c.kv_heads)
@@ -521,6 +577,38 @@ class LlamaModel:
             last = a + chunk >= h.shape[0]
             total = total + _ChunkLoss.apply(h[a:a + chunk], self.p["lm_head"], targets[a:a + chunk], last)
         return total / n_total
+
+    # ------------------------------- serving ----------------------------------------------------
+    def paged_cache(self, pages: int, page_size: int) -> list:
+        """An empty paged cache: ``(k, v)`` of every layer, ``[pages, page_size, kv_heads, head_dim]`` each."""
+        c = self.cfg
+        new = lambda: torch.empty(pages, page_size, c.kv_heads, c.head_dim, dtype=self.dtype, device=self.device)
+        return [(new(), new()) for _ in range(c.n_layers)]
+
+    @torch.no_grad()
+    def paged_logits(self, ids, cache, block_table, context_lens, step: paged.PagedStep, most_new: Optional[int] = None) -> torch.Tensor:
+        """One serving step on one device: the new tokens ``ids [tokens]`` of a batch of requests (prompts, chunks of them or a token
+        each, in the order and number that ``step`` was made for by ``ops.paged.assign_pages``) go into ``cache``, and the logits ``[requests,
+        vocab]`` behind the last new token of every request come back. A request without a new token gets those of some other row. Nothing
+        waits for the host. The window and the sinks of the configuration hold; a block pattern does not: causal."""
+        c, p = self.cfg, self.p
+        if self.world > 1:
+            raise NotImplementedError("paged serving runs on one device")
+        inv_freq, magnitude = self._angles()
+        window = self._window() or (-1, 0)
+        x = F.embedding(ids, p["embed"])
+        h, _ = E.rmsnorm_fwd(x, p["l0.norm1"], c.eps) if c.n_layers else (x, None)
+        for li, (kc, vc) in enumerate(cache):
+            q, k, v = _split_heads(G.gemm(h, p[f"l{li}.wqkv"]), c.n_heads, c.kv_heads, c.head_dim)
+            q = paged.rotary_append(q, k, v, step.pos, step.slots, kc, vc, inv_freq, interleaved=c.rope_interleaved, magnitude=magnitude)
+            o, _ = paged.paged_attention(q, kc, vc, block_table, context_lens, step.cu_new, most_new=most_new, window_size=window,
+                                         sink_tokens=c.sink_tokens)
+            x, h, _ = E.add_rmsnorm_fwd(x, G.gemm(o.reshape(x.shape[0], -1), p[f"l{li}.wo"]), p[f"l{li}.norm2"], c.eps)
+            f = G.gemm(E.swiglu_fwd(G.gemm(h, p[f"l{li}.wgu"])), p[f"l{li}.wdown"])
+            following = p[f"l{li + 1}.norm1"] if li + 1 < c.n_layers else p["norm_f"]
+            x, h, _ = E.add_rmsnorm_fwd(x, f, following, c.eps)
+        last = (step.cu_new[1:].long() - 1).clamp(min=0)
+        return G.gemm(h[last], p["lm_head"])
 
     # ------------------------------- optimizer --------------------------------------------------
     def optimizer_step(self) -> None:
