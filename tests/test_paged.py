@@ -478,6 +478,99 @@ def test_attention_bad_pages(device):
             A.check_status(dev)
 
 
+@pytest.mark.gpu
+def test_impossible_lengths():
+    """Lengths that cannot be (larger than the table, more new tokens than rows or than promised, running backwards): reported, the
+    requests are left alone and the others come out."""
+    dev = _dev("cuda")
+    q, kc, vc, table, ctx, cu, _, _ = _problem(dev, [100, 200, 50], [1, 30, 20], 4, 2, 16)
+    want, _ = ua.paged_attention(q, kc, vc, table, ctx, cu)
+
+    def check(ctx, cu, most_new, good):
+        o = torch.full_like(q, 7.0)
+        lse = torch.full((4, len(q)), 7.0, device=dev)
+        ua.paged_attention(q, kc, vc, table, ctx, cu, most_new=most_new, out=(o, lse))
+        torch.cuda.synchronize()
+        for a, b in good:
+            assert torch.equal(o[a:b], want[a:b])
+        with pytest.raises(RuntimeError, match="code=3"):
+            A.check_status(dev)
+        return o
+
+    for length in (10_000, 2 ** 31 - 1):
+        o = check(_i32([100, length, 50], dev), cu, None, [(0, 1), (31, 51)])
+        assert (o[1:31] == 7).all()
+    check(ctx, _i32([0, 1, 31, 52], dev), None, [(0, 1), (1, 31)])             # behind the last row
+    check(ctx, _i32([0, 1, -5, 51], dev), None, [(0, 1)])
+    o = check(ctx, cu, 20, [(0, 1), (31, 51)])                                   # 30 where 20 were promised
+    assert (o[1:31] == 7).all()
+
+
+@pytest.mark.gpu
+def test_cache_of_more_than_32_bits():
+    """Slots and pages behind 2^31 elements and 2^32 bytes of a cache."""
+    dev = _dev("cuda")
+    page, hk, pages = 64, 8, 34_000                      # 4.5 GB of keys
+    if torch.cuda.mem_get_info()[0] < 12e9:
+        pytest.skip("needs 12 GB")
+    kc, vc = (torch.empty(pages, page, hk, 128, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    g = torch.Generator().manual_seed(9)
+    context = 150
+    table = _i32([[pages - 1, pages - 2, 3]], dev)
+    k, v, q = (torch.randn(context, n, 128, generator=g).to(torch.bfloat16).to(dev) for n in (hk, hk, 16))
+    step = ua.paged.assign_pages(_i32([context], dev), _i32([context], dev), torch.full((1, 3), -1, dtype=torch.int32, device=dev),
+                                 table[0].flip(0).contiguous(), _i32([3], dev), page_size=page, tokens=context)
+    assert step.slots.max() == pages * page - 1
+    ua.paged.rotary_append(q, k, v, step.pos, step.slots, kc, vc)
+    assert torch.equal(kc[table[0].long()].view(-1, hk, 128)[:context], k)
+    o, lse = ua.paged_attention(q, kc, vc, table, _i32([context], dev), step.cu_new)
+    _close(o, lse, *_exact(q, k, v, context, context, 128 ** -0.5, -1, 0))
+    A.check_status(dev)
+
+
+@pytest.mark.gpu
+def test_attention_on_streams_and_threads():
+    """Two calls at once, each on a stream and a thread of its own, and one inside a graph: every one as if it were alone."""
+    import threading
+    dev = _dev("cuda")
+    problems = [_problem(dev, [3000 + 7 * i, 40, 900], [1, 1, 17 if i else 1], 8, 2, 32, seed=i) for i in range(2)]
+    want = [ua.paged_attention(*p[:6]) for p in problems]
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(s):
+                for _ in range(50):
+                    o, lse = ua.paged_attention(*problems[i][:6])
+                    if not (torch.equal(o, want[i][0]) and torch.equal(lse, want[i][1])):
+                        raise AssertionError(i)
+            s.synchronize()
+        except BaseException as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    torch.cuda.synchronize()
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    graphs = []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got[i] = ua.paged_attention(*problems[i][:6])
+        graphs.append(g)
+    for g in graphs * 3:
+        g.replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(got[i][0], want[i][0]) and torch.equal(got[i][1], want[i][1])
+    A.check_status(dev)
+
+
 @pytest.mark.parametrize("device", ["cpu", CUDA])
 def test_attention_refusals(device):
     dev = _dev(device)

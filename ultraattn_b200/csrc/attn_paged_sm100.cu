@@ -687,7 +687,9 @@ static PagedPlan plan_paged(const UaPagedAttn* a) {
   add(most <= PT ? PT : 2 * PT, below, most);
   return d;
 }
-static long part_floats(int rows, int ctas) { return static_cast<long>(ctas) * (2l * rows * (PD + 1) + PA_DESC); }
+// Workspace of a launch: parts, their lse (up to a whole number of 16 bytes), descriptions.
+static long part_lse_floats(int rows, int ctas) { return (2l * ctas * rows + 3) / 4 * 4; }
+static long part_floats(int rows, int ctas) { return 2l * ctas * rows * PD + part_lse_floats(rows, ctas) + static_cast<long>(ctas) * PA_DESC; }
 
 template <bool FEW>
 static int launch_paged(const PagedParams& p, int ctas, cudaStream_t stream) {
@@ -779,7 +781,7 @@ extern "C" int ua_attn_paged(const UaPagedAttn* a, float softmax_scale, float* w
     if (make_tmap_2byte(&p.tm_q, a->q, 3, q_dims, q_str, q_box)) return -1;
     c.part_o[i] = p.c.part_o = workspace;
     c.part_lse[i] = p.c.part_lse = workspace + 2l * ctas * l.part_rows * PD;
-    c.desc[i] = p.c.part_desc = reinterpret_cast<int*>(p.c.part_lse + 2l * ctas * l.part_rows);
+    c.desc[i] = p.c.part_desc = reinterpret_cast<int*>(p.c.part_lse + part_lse_floats(l.part_rows, ctas));
     c.part_rows[i] = l.part_rows;
     workspace += part_floats(l.part_rows, ctas);
     if (l.part_rows > most_part_rows) most_part_rows = l.part_rows;

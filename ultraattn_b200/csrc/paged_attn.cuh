@@ -159,10 +159,12 @@ __device__ __forceinline__ PagedRequest<ROWS> paged_request(const PagedScalars& 
   q.q_row = first;
   q.n = next - first;
   q.past = c - q.n;
-  const bool bad = first < 0 || next > p.tokens || q.n < 0;
+  // (a request that the table has no columns for is not begun: its length may be anything)
+  const bool narrow = c > static_cast<long>(p.columns) << p.page_shift;
+  const bool bad = first < 0 || next > p.tokens || q.n < 0 || (narrow && q.n > 0);
   const long rows = bad ? 0 : static_cast<long>(q.n) << p.pack_shift;
   const bool mine = rows > p.min_rows && rows <= p.max_rows;
-  if (report && (bad || rows > p.most_rows)) paged_error(p.status, bad ? 521 : 522, r);
+  if (report && (bad || rows > p.most_rows)) paged_error(p.status, narrow ? 523 : bad ? 521 : 522, r);
   q.row_tiles = mine ? static_cast<int>((rows + ROWS - 1) / ROWS) : 0;
   return q;
 }
