@@ -362,6 +362,14 @@ def test_attention(device, name, heads, kv, page):
 
 
 @pytest.mark.parametrize("device", ["cpu", CUDA])
+@pytest.mark.parametrize("name", ["decode short", "mixed", "chunks", "more new than context"])
+@pytest.mark.parametrize("heads,kv", [(24, 1), (64, 2), (64, 1), (100, 1), (128, 1)])
+def test_attention_wide_groups(device, name, heads, kv):
+    """Many query heads on a key/value head: 24 to 128 rows for a token."""
+    _check(_dev(device), *BATCHES[name], heads, kv, 64)
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
 @pytest.mark.parametrize("name", BATCHES)
 @pytest.mark.parametrize("left,sink,page", [(0, 0, 16), (63, 4, 16), (127, 0, 64), (128, 130, 128), (500, 1, 256), (10_000, 4, 32)])
 def test_attention_window(device, name, left, sink, page):

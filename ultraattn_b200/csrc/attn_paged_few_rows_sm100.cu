@@ -12,7 +12,11 @@
 
 namespace ua {
 
-constexpr int PF_THREADS = 352;
+// 32 rows take the registers of the warps that load and issue (see attn_paged_sm100.cu; without: 150 bytes of spills, and 48 requests of 4096
+// keys, 64 / 2 heads, take 54 us instead of 46).
+template <int N> constexpr int PF_THREADS = N == 16 ? 352 : 384;
+constexpr int PF_REGS_LAUNCH = 168, PF_REGS_LOAD = 72, PF_REGS_SOFTMAX = 216;
+static_assert(2 * PF_REGS_SOFTMAX + PF_REGS_LOAD <= 3 * PF_REGS_LAUNCH, "setmaxnreg may only redistribute the launch-time pool");
 constexpr int PF_TMA_WARP = 8;
 constexpr int PF_WALK_WARP = 10;
 constexpr int PF_MMA_WARP = 9;                // issues the products; owns the TMEM allocation
@@ -85,7 +89,7 @@ __device__ __forceinline__ float reduce_rows(float (&v)[N], int lane, Op op) {
 constexpr float PF_UNSEEN = 1e30f;            // minus the maximum of a row that has seen no key: any score is above it
 
 template <int N>
-__global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __grid_constant__ PagedParams maps) {
+__global__ void __launch_bounds__(PF_THREADS<N>, 1) attn_paged_few_kernel(const __grid_constant__ PagedParams maps) {
   using Smem = FewSmem<N>;
   constexpr int STAGES = Smem::STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -139,67 +143,71 @@ __global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __g
   };
   auto item_there = [&](uint32_t n) -> bool { return wait(&s.item_full[n % PA_ITEMS], (n / PA_ITEMS) & 1, 450) && s.item[n % PA_ITEMS].exists != 0; };
 
-  if (warp == PF_WALK_WARP) {
-    paged_walker<N>(s, wait);
-  } else if (warp == PF_TMA_WARP) {
-    paged_loader(maps, s, wait, item_there, [&](const PagedItem& it, uint32_t live) -> bool {
-      const uint32_t qb = live % Smem::QS;
-      if (!__all_sync(0xFFFFFFFFu, wait(&s.q_empty[qb], ((live / Smem::QS) & 1) ^ 1, 451))) return false;
-      if (lane == 0) mbar_arrive_expect_tx(&s.q_full[qb], N * PD * 2);
-      __syncwarp();
-      if (lane < 2) tma_load_3d(s.q[qb] + lane * (N * 128), &maps.tm_q, &s.q_full[qb], lane * 64, it.kv_head * p.group, it.q_row + it.tok0);
-      return true;
-    });
-  } else if (warp == PF_MMA_WARP) {
-    if (elect_one()) {
-      const uint32_t idesc_s = make_idesc_bf16(128, N, 0, 0);      // S^T = K Q^T, both K-major
-      const uint32_t idesc_o = make_idesc_bf16(128, N, 1, 0);      // O^T += V^T P^T: V with its head dim side by side, P^T with its keys
-      constexpr uint32_t HI = desc_hi_sw128(1024), HI_P = desc_hi_noswz(128);
-      constexpr uint32_t TILE16 = PA_TILE_BYTES >> 4;
-      const uint32_t k_desc = desc_lo(smem_u32(s.k[0]), 16), v_desc = desc_lo(smem_u32(s.v[0]), 16384);
-      const uint32_t q_desc = desc_lo(smem_u32(s.q[0]), 16), p_desc = desc_lo(smem_u32(s.p[0]), Smem::P_KEYS8);
-      bool ok = true;
-      uint32_t kv = 0, live = 0, phase = 0;
-      for (uint32_t n = 0; ok && item_there(n); ++n) {
-        const int total = s.item[n % PA_ITEMS].total;
-        mbar_arrive(&s.item_empty[n % PA_ITEMS]);
-        if (total == 0) continue;
+  if (warp >= 8) {
+    if constexpr (N > 16) reg_dealloc<PF_REGS_LOAD>();
+    if (warp == PF_WALK_WARP) {
+      paged_walker<N>(s, wait);
+    } else if (warp == PF_TMA_WARP) {
+      paged_loader(maps, s, wait, item_there, [&](const PagedItem& it, uint32_t live) -> bool {
         const uint32_t qb = live % Smem::QS;
-        if (!wait(&s.q_full[qb], (live / Smem::QS) & 1, 452)) break;
-        // key tile i belongs to group i & 1; its scores are issued two tiles ahead
-        auto scores = [&](int i) -> bool {
-          const uint32_t g = kv + i;
-          if (!wait(&s.k_full[g % STAGES], (g / STAGES) & 1, 453)) return false;
-          tc_fence_after_sync();
+        if (!__all_sync(0xFFFFFFFFu, wait(&s.q_empty[qb], ((live / Smem::QS) & 1) ^ 1, 451))) return false;
+        if (lane == 0) mbar_arrive_expect_tx(&s.q_full[qb], N * PD * 2);
+        __syncwarp();
+        if (lane < 2) tma_load_3d(s.q[qb] + lane * (N * 128), &maps.tm_q, &s.q_full[qb], lane * 64, it.kv_head * p.group, it.q_row + it.tok0);
+        return true;
+      });
+    } else if (warp == PF_MMA_WARP) {
+      if (elect_one()) {
+        const uint32_t idesc_s = make_idesc_bf16(128, N, 0, 0);      // S^T = K Q^T, both K-major
+        const uint32_t idesc_o = make_idesc_bf16(128, N, 1, 0);      // O^T += V^T P^T: V with its head dim side by side, P^T with its keys
+        constexpr uint32_t HI = desc_hi_sw128(1024), HI_P = desc_hi_noswz(128);
+        constexpr uint32_t TILE16 = PA_TILE_BYTES >> 4;
+        const uint32_t k_desc = desc_lo(smem_u32(s.k[0]), 16), v_desc = desc_lo(smem_u32(s.v[0]), 16384);
+        const uint32_t q_desc = desc_lo(smem_u32(s.q[0]), 16), p_desc = desc_lo(smem_u32(s.p[0]), Smem::P_KEYS8);
+        bool ok = true;
+        uint32_t kv = 0, live = 0, phase = 0;
+        for (uint32_t n = 0; ok && item_there(n); ++n) {
+          const int total = s.item[n % PA_ITEMS].total;
+          mbar_arrive(&s.item_empty[n % PA_ITEMS]);
+          if (total == 0) continue;
+          const uint32_t qb = live % Smem::QS;
+          if (!wait(&s.q_full[qb], (live / Smem::QS) & 1, 452)) break;
+          // key tile i belongs to group i & 1; its scores are issued two tiles ahead
+          auto scores = [&](int i) -> bool {
+            const uint32_t g = kv + i;
+            if (!wait(&s.k_full[g % STAGES], (g / STAGES) & 1, 453)) return false;
+            tc_fence_after_sync();
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            umma_ss_lo<HI, HI>(tmem_base + (i & 1) * N, k_desc + (g % STAGES) * TILE16 + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
-                               q_desc + ((qb * (N * 256) + (kk >> 2) * (N * 128) + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
-          tc_commit(&s.s_full[i & 1]);
-          tc_commit(&s.k_empty[g % STAGES]);
-          if (i + 1 == total) tc_commit(&s.q_empty[qb]);
-          return true;
-        };
-        ok = scores(0) && (total < 2 || scores(1));
-        for (int i = 0; i < total && ok; ++i) {
-          const int w = i & 1, st = (kv + i) % STAGES;
-          ok = wait(&s.v_full[st], ((kv + i) / STAGES) & 1, 454) && wait(&s.p_full[w], (phase >> w) & 1, 455);
-          if (!ok) break;
-          phase ^= 1u << w;
-          tc_fence_after_sync();
+            for (int kk = 0; kk < 8; ++kk)
+              umma_ss_lo<HI, HI>(tmem_base + (i & 1) * N, k_desc + (g % STAGES) * TILE16 + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+                                 q_desc + ((qb * (N * 256) + (kk >> 2) * (N * 128) + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+            tc_commit(&s.s_full[i & 1]);
+            tc_commit(&s.k_empty[g % STAGES]);
+            if (i + 1 == total) tc_commit(&s.q_empty[qb]);
+            return true;
+          };
+          ok = scores(0) && (total < 2 || scores(1));
+          for (int i = 0; i < total && ok; ++i) {
+            const int w = i & 1, st = (kv + i) % STAGES;
+            ok = wait(&s.v_full[st], ((kv + i) / STAGES) & 1, 454) && wait(&s.p_full[w], (phase >> w) & 1, 455);
+            if (!ok) break;
+            phase ^= 1u << w;
+            tc_fence_after_sync();
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)          // 16 keys: two of P's key groups
-            umma_ss_lo<HI, HI_P>(tmem_base + (2 + w) * N, v_desc + st * TILE16 + ((kk * 2048) >> 4),
-                                 p_desc + ((w * Smem::P_BYTES + kk * 2 * Smem::P_KEYS8) >> 4), idesc_o, (i >= 2 || kk > 0) ? 1u : 0u);
-          tc_commit(&s.pv_done[w]);
-          tc_commit(&s.v_empty[st]);
-          if (i + 2 < total) ok = scores(i + 2);
+            for (int kk = 0; kk < 8; ++kk)          // 16 keys: two of P's key groups
+              umma_ss_lo<HI, HI_P>(tmem_base + (2 + w) * N, v_desc + st * TILE16 + ((kk * 2048) >> 4),
+                                   p_desc + ((w * Smem::P_BYTES + kk * 2 * Smem::P_KEYS8) >> 4), idesc_o, (i >= 2 || kk > 0) ? 1u : 0u);
+            tc_commit(&s.pv_done[w]);
+            tc_commit(&s.v_empty[st]);
+            if (i + 2 < total) ok = scores(i + 2);
+          }
+          kv += total;
+          ++live;
         }
-        kv += total;
-        ++live;
       }
     }
   } else {
+    if constexpr (N > 16) reg_alloc<PF_REGS_SOFTMAX>();
     // =============================== softmax + epilogue: a lane is a key, then a head-dim element ===============================
     const int w = warp >> 2, quad = warp & 3;
     const int key_lane = quad * 32 + lane;
@@ -393,7 +401,7 @@ static int launch_few(const PagedParams& p, int ctas, cudaStream_t stream) {
     UA_CUDA(cudaFuncSetAttribute(attn_paged_few_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes));
     if (dev < 64) smem_set[dev] = 1;
   }
-  UA_CUDA(launch_kernel(attn_paged_few_kernel<N>, ctas, PF_THREADS, smem_bytes, stream, true, p));
+  UA_CUDA(launch_kernel(attn_paged_few_kernel<N>, ctas, PF_THREADS<N>, smem_bytes, stream, true, p));
   return 0;
 }
 
