@@ -7,18 +7,21 @@
 // vote of the four warps per tile), the row sums stay spread over the lanes until the item's end, and O^T is N columns of tensor
 // memory. Bound by reading the keys and values (64 KB a tile, three tiles in flight).
 //
-// Two groups of four warps take the key tiles in turn, each with its own S^T, P^T and O^T; one warp loads, one issues the products.
+// Two groups of four warps take the key tiles in turn, each with its own S^T, P^T and O^T; one warp loads keys, one values, one
+// issues the products, one walks the share. (A share for each group, so that one goes on while the other ends an item: the products are
+// issued in one order and wait for each other all the same, 95.7 -> 113 us for 48 requests of 20 to 16000 keys.)
 #include "paged_attn.cuh"
 
 namespace ua {
 
 // 32 rows take the registers of the warps that load and issue (see attn_paged_sm100.cu; without: 150 bytes of spills, and 48 requests of 4096
 // keys, 64 / 2 heads, take 54 us instead of 46).
-template <int N> constexpr int PF_THREADS = N == 16 ? 352 : 384;
+constexpr int PF_THREADS = 384;
 constexpr int PF_REGS_LAUNCH = 168, PF_REGS_LOAD = 72, PF_REGS_SOFTMAX = 216;
 static_assert(2 * PF_REGS_SOFTMAX + PF_REGS_LOAD <= 3 * PF_REGS_LAUNCH, "setmaxnreg may only redistribute the launch-time pool");
 constexpr int PF_TMA_WARP = 8;
 constexpr int PF_WALK_WARP = 10;
+constexpr int PF_VALUE_WARP = 11;             // loads V (PF_TMA_WARP: K and Q)
 constexpr int PF_MMA_WARP = 9;                // issues the products; owns the TMEM allocation
 
 template <int N>
@@ -89,7 +92,7 @@ __device__ __forceinline__ float reduce_rows(float (&v)[N], int lane, Op op) {
 constexpr float PF_UNSEEN = 1e30f;            // minus the maximum of a row that has seen no key: any score is above it
 
 template <int N>
-__global__ void __launch_bounds__(PF_THREADS<N>, 1) attn_paged_few_kernel(const __grid_constant__ PagedParams maps) {
+__global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __grid_constant__ PagedParams maps) {
   using Smem = FewSmem<N>;
   constexpr int STAGES = Smem::STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(PF_THREADS<N>, 1) attn_paged_few_kernel(const 
     }
     for (int i = 0; i < PA_ITEMS; ++i) {
       mbar_init(&s.item_full[i], 1);
-      mbar_init(&s.item_empty[i], 2 + 8);       // loader, issuer, softmax warps
+      mbar_init(&s.item_empty[i], 3 + 8);       // loaders, issuer, softmax warps
     }
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&s.k_full[i], 1);
@@ -148,7 +151,7 @@ __global__ void __launch_bounds__(PF_THREADS<N>, 1) attn_paged_few_kernel(const 
     if (warp == PF_WALK_WARP) {
       paged_walker<N>(s, wait);
     } else if (warp == PF_TMA_WARP) {
-      paged_loader(maps, s, wait, item_there, [&](const PagedItem& it, uint32_t live) -> bool {
+      paged_loader<true, false>(maps, s, wait, item_there, [&](const PagedItem& it, uint32_t live) -> bool {
         const uint32_t qb = live % Smem::QS;
         if (!__all_sync(0xFFFFFFFFu, wait(&s.q_empty[qb], ((live / Smem::QS) & 1) ^ 1, 451))) return false;
         if (lane == 0) mbar_arrive_expect_tx(&s.q_full[qb], N * PD * 2);
@@ -156,6 +159,8 @@ __global__ void __launch_bounds__(PF_THREADS<N>, 1) attn_paged_few_kernel(const 
         if (lane < 2) tma_load_3d(s.q[qb] + lane * (N * 128), &maps.tm_q, &s.q_full[qb], lane * 64, it.kv_head * p.group, it.q_row + it.tok0);
         return true;
       });
+    } else if (warp == PF_VALUE_WARP) {
+      paged_loader<false, true>(maps, s, wait, item_there, [](const PagedItem&, uint32_t) { return true; });
     } else if (warp == PF_MMA_WARP) {
       if (elect_one()) {
         const uint32_t idesc_s = make_idesc_bf16(128, N, 0, 0);      // S^T = K Q^T, both K-major
@@ -365,12 +370,14 @@ __global__ void __launch_bounds__(PF_THREADS<N>, 1) attn_paged_few_kernel(const 
                                    : reinterpret_cast<uintptr_t>(p.o + tok * p.o_token + head * p.o_head + key_lane - lane);
 #pragma unroll
         for (int y = 0; y < N; ++y) {
-          if (!((rows >> y) & 1u)) continue;
+          if ((rows >> y) == 0) break;
           const float g0 = __shfl_sync(0xFFFFFFFFu, f0, y), g1 = __shfl_sync(0xFFFFFFFFu, f1, y);
           const uintptr_t to = __shfl_sync(0xFFFFFFFFu, static_cast<unsigned long long>(dst), y);
           const float o = (g0 != 0.f ? o0[y] * g0 : 0.f) + (g1 != 0.f ? o1[y] * g1 : 0.f);
-          if (part) reinterpret_cast<float*>(to)[lane] = o;
-          else reinterpret_cast<__nv_bfloat16*>(to)[lane] = __float2bfloat16_rn(o);
+          if ((rows >> y) & 1u) {
+            if (part) reinterpret_cast<float*>(to)[lane] = o;
+            else reinterpret_cast<__nv_bfloat16*>(to)[lane] = __float2bfloat16_rn(o);
+          }
         }
         tc_fence_before_sync();
         mbar_arrive_warp(&s.merged);
@@ -401,7 +408,7 @@ static int launch_few(const PagedParams& p, int ctas, cudaStream_t stream) {
     UA_CUDA(cudaFuncSetAttribute(attn_paged_few_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes));
     if (dev < 64) smem_set[dev] = 1;
   }
-  UA_CUDA(launch_kernel(attn_paged_few_kernel<N>, ctas, PF_THREADS<N>, smem_bytes, stream, true, p));
+  UA_CUDA(launch_kernel(attn_paged_few_kernel<N>, ctas, PF_THREADS, smem_bytes, stream, true, p));
   return 0;
 }
 

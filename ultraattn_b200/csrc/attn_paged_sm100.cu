@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
       // =============================== loader =================================
       const int boxes = FEW ? 2 : 4;
       const uint32_t bytes = FEW && p.two_q ? PA_TILE_BYTES / 2 : boxes * (PA_TILE_BYTES / 2);
-      paged_loader(maps, s, wait, item_there, [&](const PagedItem& it, uint32_t live) -> bool {
+      paged_loader<true, true>(maps, s, wait, item_there, [&](const PagedItem& it, uint32_t live) -> bool {
         const uint32_t qb = p.two_q ? live & 1 : 0, use = p.two_q ? live >> 1 : live;
         if (!__all_sync(0xFFFFFFFFu, wait(&s.q_empty[qb], (use & 1) ^ 1, 402))) return false;
         if (lane == 0) mbar_arrive_expect_tx(&s.q_full[qb], bytes);

@@ -22,8 +22,9 @@ namespace ua {
 constexpr int PD = 128;                       // head dim
 constexpr int PT = 128;                       // keys of a tile
 constexpr int PA_TILE_BYTES = PT * PD * 2;    // [2 d-halves][128 rows][128 B]
-// What the start and the end of an item cost, in key tiles of its form (a share's border is not put into them).
-template <int ROWS> constexpr int PA_ITEM_TILES = ROWS <= 32 ? 1 : 3;
+// What the start and the end of an item cost, in key tiles of its form (a share's border is not put into them). Up to 32 rows, 200 requests of
+// 20 to 2000 keys, 32 / 8 heads: 1 126 us, 3 97, 4 90, 5 99; 48 of 20 to 16000 94 to 96 with each.
+template <int ROWS> constexpr int PA_ITEM_TILES = ROWS <= 32 ? 4 : 3;
 // An item of fewer tiles is not cut: the border moves to its nearer end. Writing and merging the fp32 parts of 256 rows takes as long as
 // six to eight key tiles of them, those of 16 rows nothing.
 template <int ROWS> constexpr int PA_WHOLE = ROWS <= 32 ? 0 : ROWS == 128 ? 8 : 20;
@@ -209,8 +210,20 @@ struct PagedWalk {
     const int r0 = min(p.requests, lane * per), r1 = min(p.requests, r0 + per);
     long mine = 0;
     PagedRequest<ROWS> mine_last{};
+    int first = 0, upto = 0, context = 0;
+    if (r0 < r1) {
+      first = p.cu_new[r0];
+      upto = p.cu_new[r0 + 1];
+      context = p.context[r0];
+    }
     for (int i = r0; i < r1; ++i) {
-      mine_last = paged_request<ROWS>(p, i, cta == 0);
+      const int f = first, u = upto, c = context;
+      if (i + 1 < r1) {                       // (the next one's are on their way meanwhile)
+        first = u;
+        upto = p.cu_new[i + 2];
+        context = p.context[i + 1];
+      }
+      mine_last = paged_request<ROWS>(p, i, f, u, c, cta == 0);
       if (mine_last.row_tiles > 0) mine += p.kv_heads * mine_last.weight(p, mine_last.row_tiles);
     }
     long before = mine;
@@ -420,9 +433,10 @@ __device__ __forceinline__ void paged_walker(Smem& s, Wait wait) {
   }
 }
 
-// The loader's warp: keys and values, page by page (a TMA box is a page, or 128 tokens of a larger one). load_q(item, live) loads the
-// queries of the live-th item that has keys.
-template <typename Smem, typename Wait, typename There, typename LoadQ>
+// A loader's warp: keys and values, page by page (a TMA box is a page, or 128 tokens of a larger one). load_q(item, live) loads the
+// queries of the live-th item that has keys. KEYS, VALUES: one warp for both, or one for each (what a tile takes to issue is a chain of
+// 1000 clocks; 33 requests behind a window of 4096, 28 / 4 heads, pages of 16: one warp 24.9 us, two 22.3).
+template <bool KEYS, bool VALUES, typename Smem, typename Wait, typename There, typename LoadQ>
 __device__ __forceinline__ void paged_loader(const PagedParams& maps, Smem& s, Wait wait, There item_there, LoadQ load_q) {
   const PagedScalars& p = s.c;
   constexpr int STAGES = Smem::STAGES;
@@ -455,23 +469,27 @@ __device__ __forceinline__ void paged_loader(const PagedParams& maps, Smem& s, W
       const int st = j % STAGES;
       const uint32_t ph = (j / STAGES) & 1;
       const unsigned there = __ballot_sync(0xFFFFFFFFu, page >= 0 && page < p.pages);
-      if (page != PA_NO_PAGE && !((there >> lane) & 1u)) paged_error(p.status, 520, it.request);
+      if (KEYS && page != PA_NO_PAGE && !((there >> lane) & 1u)) paged_error(p.status, 520, it.request);
       int pages[8];
 #pragma unroll
       for (int b = 0; b < 8; ++b) pages[b] = __shfl_sync(0xFFFFFFFFu, page, b);
-      ok = __all_sync(0xFFFFFFFFu, wait(&s.k_empty[st], ph ^ 1, 400));
-      if (!ok) break;
-      load_tile(s.k[st], &maps.tm_k, &s.k_full[st], there, pages, head, off);
-      if (i == 0) {
-        // Q, behind the first keys: its room is free when the scores of the item before (of the one before that, where there are
-        // two) are complete, later than that of a key tile
-        ok = load_q(it, live);
+      if (KEYS) {
+        ok = __all_sync(0xFFFFFFFFu, wait(&s.k_empty[st], ph ^ 1, 400));
         if (!ok) break;
-        ++live;
+        load_tile(s.k[st], &maps.tm_k, &s.k_full[st], there, pages, head, off);
+        if (i == 0) {
+          // Q, behind the first keys: its room is free when the scores of the item before (of the one before that, where there are
+          // two) are complete, later than that of a key tile
+          ok = load_q(it, live);
+          if (!ok) break;
+          ++live;
+        }
       }
-      ok = __all_sync(0xFFFFFFFFu, wait(&s.v_empty[st], ph ^ 1, 401));
-      if (!ok) break;
-      load_tile(s.v[st], &maps.tm_v, &s.v_full[st], there, pages, head, off);
+      if (VALUES) {
+        ok = __all_sync(0xFFFFFFFFu, wait(&s.v_empty[st], ph ^ 1, 401));
+        if (!ok) break;
+        load_tile(s.v[st], &maps.tm_v, &s.v_full[st], there, pages, head, off);
+      }
       page = next_page;
     }
     __syncwarp();
