@@ -445,6 +445,55 @@ def test_attention_large_scores(device):
     _check(_dev(device), [700, 260], [1, 260], 8, 2, 64, scale_q=4.0)
 
 
+# (context, new, query heads of one key/value head): items of 16, 32, 128 and 256 rows; short ones, and long ones in parts
+NAN_BATCHES = [([40, 9000], [1, 1], 4), ([40, 9000], [1, 1], 16), ([40, 9000], [1, 20], 4), ([100, 9000], [70, 90], 4)]
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+@pytest.mark.parametrize("value", [NAN, math.inf])
+@pytest.mark.parametrize("context,new,heads", NAN_BATCHES)
+def test_attention_of_a_nan(device, context, new, heads, value):
+    """A row with a NaN among the scores that it sees is NaN, not 0; the others are what they are."""
+    dev = _dev(device)
+    q, kc, vc, table, ctx, cu, keys, values = _problem(dev, context, new, heads, 1, 64)
+    exact = [_exact(x, kk, vv, c, n, 128 ** -0.5, -1, 0) for x, kk, vv, c, n in zip(q.split(new), keys, values, context, new)]
+    want, want_lse, weight = torch.cat([x[0] for x in exact]), torch.cat([x[1] for x in exact], 1), torch.cat([x[2] for x in exact])
+    # one head of one query of the long request (an infinity: one score of +inf or -inf, a NaN with the next one)
+    q2 = q.clone()
+    q2[-1, 1, :2] = value
+    o, lse = ua.paged_attention(q2, kc, vc, table, ctx, cu)
+    assert o[-1, 1].isnan().all() and (math.isinf(value) or lse[1, -1].isnan())
+    rest = torch.ones(q.shape[:2], dtype=torch.bool, device=dev)
+    rest[-1, 1] = False
+    _close(o[rest], lse.t()[rest], want[rest], want_lse.t()[rest], weight[rest])
+    # a key of the short request: position 0 is seen by all of its rows
+    kc[table[0, 0].long(), 0, 0, 5] = NAN
+    o, lse = ua.paged_attention(q, kc, vc, table, ctx, cu)
+    a = new[0]
+    assert o[:a].isnan().all() and lse[:, :a].isnan().all()
+    _close(o[a:], lse[:, a:], want[a:], want_lse[:, a:], weight[a:])
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+@pytest.mark.parametrize("context,new,heads", NAN_BATCHES)
+def test_attention_far_below_zero(device, context, new, heads):
+    """Scores of -1e32 and less: still seen, and the first key (of -1e32, the others -2e32) has all the weight."""
+    dev = _dev(device)
+    q, kc, vc, table, ctx, cu, _, _ = _problem(dev, context, new, heads, 1, 64)
+    q.fill_(-2.0 ** 50)
+    for r, c in enumerate(context):
+        j = torch.arange(c, device=dev)
+        kc[table[r, j // 64].long(), j % 64] = 2.0 ** 54
+        kc[table[r, 0].long(), 0] = 2.0 ** 53
+    o, lse = ua.paged_attention(q, kc, vc, table, ctx, cu)
+    score = -2.0 ** 103 * 128 * 128 ** -0.5
+    for r in range(2):
+        first = vc[table[r, 0].long(), 0, 0]
+        assert torch.equal(o[int(cu[r]):int(cu[r + 1])], first.expand(new[r], heads, 128))
+    # (the scale and log2 e are rounded to fp32, and so are two products and a sum)
+    assert ((lse.double() / score - 1).abs() <= 6 * 2.0 ** -24).all()
+
+
 @pytest.mark.parametrize("device", ["cpu", CUDA])
 def test_attention_shared_pages(device):
     """Two requests that name the same pages for a common beginning."""

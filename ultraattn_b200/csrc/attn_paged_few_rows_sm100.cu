@@ -89,7 +89,7 @@ __device__ __forceinline__ float reduce_rows(float (&v)[N], int lane, Op op) {
   return N == 16 ? op(v[0], __shfl_xor_sync(0xFFFFFFFFu, v[0], 1)) : v[0];
 }
 
-constexpr float PF_UNSEEN = 1e30f;            // minus the maximum of a row that has seen no key: any score is above it
+constexpr float PF_UNSEEN = 3e38f;            // minus the maximum of a row that has seen no key: any score is above it
 
 template <int N>
 __global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __grid_constant__ PagedParams maps) {
@@ -353,17 +353,18 @@ __global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __g
         const bool in0 = m0 > -INFINITY, in1 = m1 > -INFINITY;
         const float sum = (in0 || l0 != l0 ? a0 * l0 : 0.f) + (in1 || l1 != l1 ? a1 * l1 : 0.f);
         const bool seen = sum > 0.f && m > -INFINITY;
-        const float lse = seen ? (m + __log2f(sum)) * 0.6931471805599453f : -INFINITY;
+        const bool bad = sum != sum;                 // a NaN among the scores that the row sees
+        const float lse = seen ? (m + __log2f(sum)) * 0.6931471805599453f : bad ? sum : -INFINITY;
         // (0: what tensor memory holds of a group without a key is not used)
         const float inv = __fdividef(1.f, sum);
-        const float f0 = seen && in0 ? a0 * inv : 0.f, f1 = seen && in1 ? a1 * inv : 0.f;
+        const float f0 = seen && in0 ? a0 * inv : bad ? sum : 0.f, f1 = seen && in1 ? a1 * inv : 0.f;
         long tok;
         int head;
         const bool valid = paged_row(p, it, x, tok, head) && lane < N;
         const long prow = static_cast<long>(it.slot) * p.part_rows + x;
         const unsigned rows = __ballot_sync(0xFFFFFFFFu, valid);
         if (valid && quad == 0) {
-          if (part) p.part_lse[prow] = sum != sum ? sum : lse;           // (a NaN score: see combine_parts_kernel)
+          if (part) p.part_lse[prow] = lse;
           else p.lse[head * p.lse_head + tok] = lse;
         }
         const uintptr_t dst = part ? reinterpret_cast<uintptr_t>(p.part_o + prow * PD + key_lane - lane)

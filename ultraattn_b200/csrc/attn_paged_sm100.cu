@@ -60,12 +60,14 @@ __device__ __forceinline__ void paged_epilogue(const PagedScalars& p, PagedSmem<
   if (any && l > 0.f && m > -INFINITY) {
     lse = (m + log2f(l)) * 0.6931471805599453f;
     f = 1.0f / l;
+  } else if (any && l != l) {            // a NaN among the scores that the row sees
+    lse = f = l;
   }
   long tok;
   int head;
   const bool valid = paged_row(p, it, x, tok, head);
   if (part) {
-    if (x < p.part_rows) p.part_lse[static_cast<long>(it.slot) * p.part_rows + x] = any && l != l ? l : lse;   // (a NaN score: see combine_parts)
+    if (x < p.part_rows) p.part_lse[static_cast<long>(it.slot) * p.part_rows + x] = lse;
   } else if (valid) {
     p.lse[head * p.lse_head + tok] = lse;
   }
@@ -130,7 +132,8 @@ __device__ __forceinline__ void paged_few_epilogue(const PagedScalars& p, PagedS
   const float a0 = fast_exp2(m0 - m), a1 = fast_exp2(other.x - m);
   const float l = (m0 > -INFINITY || l0 != l0 ? a0 * l0 : 0.f) + (other.x > -INFINITY || other.y != other.y ? a1 * other.y : 0.f);
   const bool live = l > 0.f && m > -INFINITY, use0 = live && m0 > -INFINITY, use1 = live && other.x > -INFINITY;
-  const float lse = live ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  const float bad = l != l ? l : 0.f;           // a NaN among the scores that the row sees
+  const float lse = live ? (m + log2f(l)) * 0.6931471805599453f : l != l ? l : -INFINITY;
   const float f0 = a0 / l, f1 = a1 / l;
   const bool part = it.slot >= 0;
   long tok;
@@ -138,7 +141,7 @@ __device__ __forceinline__ void paged_few_epilogue(const PagedScalars& p, PagedS
   const bool valid = paged_row(p, it, x, tok, head);
   const long prow = static_cast<long>(it.slot) * p.part_rows + x;
   if (valid) {
-    if (part) p.part_lse[prow] = l != l ? l : lse;
+    if (part) p.part_lse[prow] = lse;
     else p.lse[head * p.lse_head + tok] = lse;
   }
   __nv_bfloat16* optr = p.o + tok * p.o_token + head * p.o_head;
@@ -152,7 +155,7 @@ __device__ __forceinline__ void paged_few_epilogue(const PagedScalars& p, PagedS
     float f[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      f[i] = (use0 ? __uint_as_float(u[i]) * f0 : 0.f) + (use1 ? __uint_as_float(v[i]) * f1 : 0.f);
+      f[i] = (use0 ? __uint_as_float(u[i]) * f0 : bad) + (use1 ? __uint_as_float(v[i]) * f1 : bad);
     if (part) {
 #pragma unroll
       for (int q = 0; q < 8; ++q)
@@ -595,7 +598,7 @@ __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constan
   auto row_of = [&](int i, int x) -> long { return (i == 0 ? 2 * first + 1 : 2 * (first + i)) * part_rows + x; };
   // lane i: the lse of part i (and of parts 32 + i ..), then its weight; the parts themselves in one go behind that
   float mx[4];
-  bool bad[4];                         // a NaN score: O = 0 and lse = -inf, as in an item that is not cut
+  bool bad[4];                         // a NaN score, in O and lse as in an item that is not cut
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     mx[k] = -INFINITY;
@@ -614,7 +617,8 @@ __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constan
   for (int k = 0; k < 4; ++k) {
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xFFFFFFFFu, mx[k], s));
-    if (__any_sync(0xFFFFFFFFu, bad[k])) mx[k] = -INFINITY;
+    bad[k] = __any_sync(0xFFFFFFFFu, bad[k]);
+    if (bad[k]) mx[k] = -INFINITY;
     tot[k] = 0.f;
     acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
@@ -647,14 +651,14 @@ __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constan
   for (int k = 0; k < 4; ++k) {
     const int x = x0 + 8 * k, h = x & ((1 << p.pack_shift) - 1);
     if (x >= d.w || h >= p.group) continue;
-    const float inv = tot[k] > 0.f ? 1.f / tot[k] : 0.f;
+    const float inv = bad[k] ? NAN : tot[k] > 0.f ? 1.f / tot[k] : 0.f;
     const long tok = d.y + (x >> p.pack_shift);
     const int head = d.z + h;
     uint2 o;
     o.x = pack_bf16x2(acc[k].x * inv, acc[k].y * inv);
     o.y = pack_bf16x2(acc[k].z * inv, acc[k].w * inv);
     *reinterpret_cast<uint2*>(p.o + tok * p.o_token + head * p.o_head + lane * 4) = o;
-    if (lane == 0) p.lse[head * p.lse_head + tok] = tot[k] > 0.f ? mx[k] + __logf(tot[k]) : -INFINITY;
+    if (lane == 0) p.lse[head * p.lse_head + tok] = bad[k] ? NAN : tot[k] > 0.f ? mx[k] + __logf(tot[k]) : -INFINITY;
   }
 }
 
