@@ -173,6 +173,8 @@ def test_page_refusals(device):
         lambda: ua.paged.assign_pages(c, c, t, f, n, page_size=24, tokens=2),
         lambda: ua.paged.assign_pages(c, c, t, f, n, page_size=0, tokens=2),
         lambda: ua.paged.assign_pages(c, c, t, f, n, page_size=16, tokens=-1),
+        lambda: ua.paged.assign_pages(c, c, t, f, n, page_size=16, tokens=(1 << 30) + 1),
+        lambda: ua.paged.assign_pages(c, c, t, f, n, page_size=1 << 31, tokens=2),
         lambda: ua.paged.assign_pages(c.long(), c, t, f, n, **ok),
         lambda: ua.paged.assign_pages(c[:1], c, t, f, n, **ok),
         lambda: ua.paged.assign_pages(c, c, t.t(), f, n, **ok),
@@ -186,6 +188,15 @@ def test_page_refusals(device):
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_pages_whose_slots_have_no_number(device):
+    """Page 2^27 of 16 tokens: its slots do not fit 32 bits. The tokens get none, instead of another page's."""
+    dev = _dev(device)
+    table, stack = _i32([[-7, -7]], dev), _i32([1 << 27, 5], dev)
+    step = ua.paged.assign_pages(_i32([20], dev), _i32([20], dev), table, stack, _i32([2], dev), page_size=16, tokens=20)
+    assert table.tolist() == [[5, 1 << 27]] and step.slots.tolist() == [80 + j for j in range(16)] + [-1] * 4
 
 
 # ------------------------------------------------------------------------------------------------
@@ -492,6 +503,35 @@ def test_attention_far_below_zero(device, context, new, heads):
         assert torch.equal(o[int(cu[r]):int(cu[r + 1])], first.expand(new[r], heads, 128))
     # (the scale and log2 e are rounded to fp32, and so are two products and a sum)
     assert ((lse.double() / score - 1).abs() <= 6 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_attention_of_nothing(device):
+    """No heads, no tokens, no requests; a bound of no new tokens, which one token may exceed unnoticed and no result is lost."""
+    dev = _dev(device)
+    q, kc, vc, table, ctx, cu, _, _ = _problem(dev, [300, 20], [1, 1], 8, 2, 16)
+    o, lse = ua.paged_attention(q[:, :0], kc, vc, table, ctx, cu)
+    assert o.shape == (2, 0, 128) and lse.shape == (0, 2)
+    o, lse = ua.paged_attention(q[:0], kc, vc, table, ctx, torch.zeros_like(cu))
+    assert o.shape == (0, 8, 128) and lse.shape == (8, 0)
+    o, lse = ua.paged_attention(q, kc, vc, table[:0], ctx[:0], cu[:1])
+    assert o.shape == q.shape
+    want, got = (ua.paged_attention(q, kc, vc, table, ctx, cu, most_new=n) for n in (1, 0))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_context_of_all_32_bits():
+    """A table may name one page again and again: a length that the positions' arithmetic has no room for is refused."""
+    dev = _dev("cuda")
+    cache = torch.zeros(1, 1 << 24, 1, 128, dtype=torch.bfloat16, device=dev)
+    q = torch.randn(2, 1, 128, device=dev).bfloat16()
+    table = torch.zeros(2, 128, dtype=torch.int32, device=dev)
+    for most in (1, None):
+        o, lse = ua.paged_attention(q, cache, cache, table, _i32([0x7FFFFFFF, 3], dev), _i32([0, 1, 2], dev), most_new=most)
+        with pytest.raises(RuntimeError, match="code=3"):
+            A.check_status(dev)
+        assert (o[1] == 0).all() and (lse[0, 1] - math.log(3)).abs() < 1e-6
 
 
 @pytest.mark.parametrize("device", ["cpu", CUDA])

@@ -209,6 +209,15 @@ def test_views_and_out(device):
         assert R.rotate((e,), pos[:shape[0]], f)[0].shape == e.shape
 
 
+@pytest.mark.gpu
+def test_more_heads_than_indexes():
+    dev = torch.device("cuda", 0)
+    f = torch.ones(1, dtype=torch.float64, device=dev)
+    many = torch.ones(1, 1, 2, device=dev).expand(1, (1 << 24) + 1, 2)
+    with pytest.raises(RuntimeError, match="heads"):
+        ua.rotary(many, many[:, :1], torch.zeros(1, dtype=torch.int32, device=dev), f)
+
+
 @pytest.mark.parametrize("device", ["cpu", CUDA])
 def test_refusals(device):
     dev = _dev(device)

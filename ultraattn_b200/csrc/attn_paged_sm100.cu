@@ -672,7 +672,7 @@ static PagedPlan plan_paged(const UaPagedAttn* a) {
   PagedPlan d{};
   const long group = a->heads / a->kv_heads;
   while ((1l << d.pack_shift) < group) ++d.pack_shift;
-  const long most = a->most_new << d.pack_shift;
+  const long most = (a->most_new > 0 ? a->most_new : 1) << d.pack_shift;       // (a bound of no tokens: the lengths are looked at all the same)
   auto add = [&](int form, int min_rows, long max_rows) {
     d.launch[d.n++] = {form, min_rows, static_cast<int>(max_rows < 0x7FFFFFFF ? max_rows : 0x7FFFFFFF),
                        static_cast<int>(max_rows < form ? max_rows : form)};
@@ -718,7 +718,7 @@ using namespace ua;
 
 // Floats of workspace that ua_attn_paged needs.
 extern "C" long ua_attn_paged_workspace(const UaPagedAttn* a) {
-  if (a->kv_heads <= 0 || a->heads % a->kv_heads != 0) return 0;
+  if (a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads != 0) return 0;
   const PagedPlan d = plan_paged(a);
   long n = 0;
   for (int i = 0; i < d.n; ++i) n += part_floats(d.launch[i].part_rows, sm_count());
@@ -726,7 +726,7 @@ extern "C" long ua_attn_paged_workspace(const UaPagedAttn* a) {
 }
 
 extern "C" int ua_attn_paged(const UaPagedAttn* a, float softmax_scale, float* workspace, int* status, cudaStream_t stream) {
-  if (a->tokens <= 0 || a->requests <= 0 || a->most_new <= 0) return 0;
+  if (a->tokens <= 0 || a->heads <= 0 || a->requests <= 0) return 0;
   if (a->kv_heads <= 0 || a->heads % a->kv_heads != 0)
     UA_FAIL("ua_attn_paged: %ld query heads do not divide into %ld key/value heads", a->heads, a->kv_heads);
   if (a->heads / a->kv_heads > PT) UA_FAIL("ua_attn_paged: %ld query heads for a key/value head (%d at most)", a->heads / a->kv_heads, PT);

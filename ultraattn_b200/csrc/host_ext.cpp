@@ -240,7 +240,7 @@ py::object rotary_append(py::handle qh, py::handle kh, py::handle vh, py::handle
   for (const Tensor* t : {&k, &v, &k_cache, &v_cache})
     if (t->scalar_type() != q.scalar_type() || t->device() != dev || t->size(t->dim() - 1) != dim || t->stride(t->dim() - 1) != 1) return py::none();
   if (T == 0 || rotary_type(q) < 0 || sh < 0 || q.stride(2) != 1 || k.sizes() != v.sizes() || k.size(0) != T || k_cache.sizes() != v_cache.sizes() ||
-      k_cache.size(2) != k.size(1) || !is_int(slots, dev, T) || pos.dim() != 1 || !angles_fit(q, pos, inv_freq))
+      k_cache.size(2) != k.size(1) || k_cache.size(0) << sh > int64_t{1} << 31 || !is_int(slots, dev, T) || pos.dim() != 1 || !angles_fit(q, pos, inv_freq))
     return py::none();
   const Tensor out = at::empty(q.sizes(), q.options());
   UaRotary a{};
@@ -269,7 +269,7 @@ py::object assign_pages(py::handle ch, py::handle nh, py::handle th, py::handle 
   const at::Device dev = table.device();
   const int sh = log2_of(page_size);
   const int64_t n = table.dim() == 2 ? table.size(0) : -1;
-  if (!dev.is_cuda() || sh < 0 || tokens < 0 || n < 0 || n > most_requests || !is_table(table, dev) || !is_int(context, dev, n) || !is_int(fresh, dev, n) ||
+  if (!dev.is_cuda() || sh < 0 || sh > 30 || tokens < 0 || tokens > 1 << 30 || n < 0 || n > most_requests || !is_table(table, dev) || !is_int(context, dev, n) || !is_int(fresh, dev, n) ||
       free_pages.dim() != 1 || !is_int(free_pages, dev, free_pages.size(0)) || !is_int(count, dev, 1) || (count_out && !is_int(*count_out, dev, 1)))
     return py::none();
   const auto opt = table.options();
@@ -294,7 +294,7 @@ py::object release_pages(py::handle eh, py::handle ch, py::handle th, py::handle
   const at::Device dev = table.device();
   const int sh = log2_of(page_size);
   const int64_t n = table.dim() == 2 ? table.size(0) : -1;
-  if (!dev.is_cuda() || sh < 0 || n < 0 || n > most_requests || !is_table(table, dev) || !is_int(context, dev, n) || free_pages.dim() != 1 ||
+  if (!dev.is_cuda() || sh < 0 || sh > 30 || n < 0 || n > most_requests || !is_table(table, dev) || !is_int(context, dev, n) || free_pages.dim() != 1 ||
       !is_int(free_pages, dev, free_pages.size(0)) || !is_int(count, dev, 1) || (count_out && !is_int(*count_out, dev, 1)) ||
       ended.scalar_type() != at::kBool || ended.device() != dev || ended.dim() != 1 || ended.size(0) != n || !ended.is_contiguous())
     return py::none();
@@ -325,7 +325,7 @@ py::object paged_attention(py::handle qh, py::handle kh, py::handle vh, py::hand
     for (int64_t i = 0; i < d; ++i)
       if (t->stride(i) % 8 != 0) return py::none();
   }
-  if (kc.sizes() != vc.sizes() || sh < 4 || hk == 0 || H % hk != 0 || H / hk > 128 || n > most_requests || !is_table(table, dev) || !is_int(context, dev, n) ||
+  if (kc.sizes() != vc.sizes() || sh < 4 || hk == 0 || H == 0 || H % hk != 0 || H / hk > 128 || n > most_requests || !is_table(table, dev) || !is_int(context, dev, n) ||
       !is_int(cu, dev, n + 1) || most_new < 0 || !(scale > 0.0 && scale < 1e30) || sink < 0 || (sink > 0 && left < 0))
     return py::none();
   const Tensor o = at::empty(q.sizes(), q.options());

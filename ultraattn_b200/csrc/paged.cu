@@ -20,6 +20,7 @@ namespace ua {
 constexpr int PAGES_THREADS = 1024;
 constexpr int PAGES_CLUSTER = 8;
 constexpr int PAGES_MAX_REQUESTS = 8192;
+constexpr int PAGES_MAX_TOKENS = 1 << 30;
 
 struct PagesParams {
   const int* context;        // [requests] tokens of a request, the new ones among them
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(PAGES_THREADS) assign_pages_kernel(const __gri
       if (at >= 0) {
         const int col = at >> sh, held = pages_of(past, sh);
         const int page = col >= held ? p.free_pages[count - 1 - (first[r] + col - held)] : p.table[r * p.table_stride + col];
-        if (page >= 0) slot = (page << sh) + (at & ((1 << sh) - 1));
+        if (page >= 0 && page <= 0x7FFFFFFF >> sh) slot = (page << sh) + (at & ((1 << sh) - 1));
       }
     }
     p.pos[t] = at;
@@ -250,6 +251,7 @@ extern "C" int ua_assign_pages(const int* context, const int* fresh, int request
                                const int* free_pages, int pool, const int* count_in, int* count_out, int page_shift, int tokens, int* cu,
                                int* pos, int* slots, int* status, cudaStream_t stream) {
   if (requests < 0 || requests > PAGES_MAX_REQUESTS) UA_FAIL("ua_assign_pages: %d requests (%d at most)", requests, PAGES_MAX_REQUESTS);
+  if (tokens < 0 || tokens > PAGES_MAX_TOKENS || page_shift < 0 || page_shift > 30) UA_FAIL("ua_assign_pages: %d tokens, pages of 2^%d", tokens, page_shift);
   PagesParams p{context, fresh, nullptr, requests, table, table_stride, columns, const_cast<int*>(free_pages), pool, count_in, count_out,
                 page_shift, tokens, cu, pos, slots, status};
   return launch_pages(assign_pages_kernel, p, tokens, (3 * requests + 2) * 4, stream);

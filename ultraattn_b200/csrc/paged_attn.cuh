@@ -29,6 +29,7 @@ template <int ROWS> constexpr int PA_ITEM_TILES = ROWS <= 32 ? 4 : 3;
 // six to eight key tiles of them, those of 16 rows nothing.
 template <int ROWS> constexpr int PA_WHOLE = ROWS <= 32 ? 0 : ROWS == 128 ? 8 : 20;
 template <int ROWS> constexpr int PA_SNAP = ROWS <= 32 ? 0 : ROWS == 128 ? 3 : 6;     // nor are fewer tiles of an item cut off
+constexpr long PA_MAX_KEYS = 0x7FFF0000;      // of a request: positions and tiles are counted in 32 bits
 constexpr int PA_MIN_SHARE = 2;               // key tiles of a CTA at least
 
 // (Every block copies these into its shared memory before it waits for the kernel in front of it: parameters that have not been
@@ -161,7 +162,7 @@ __device__ __forceinline__ PagedRequest<ROWS> paged_request(const PagedScalars& 
   q.n = next - first;
   q.past = c - q.n;
   // (a request that the table has no columns for is not begun: its length may be anything)
-  const bool narrow = c > static_cast<long>(p.columns) << p.page_shift;
+  const bool narrow = c > min(static_cast<long>(p.columns) << p.page_shift, PA_MAX_KEYS);
   const bool bad = first < 0 || next > p.tokens || q.n < 0 || (narrow && q.n > 0);
   const long rows = bad ? 0 : static_cast<long>(q.n) << p.pack_shift;
   const bool mine = rows > p.min_rows && rows <= p.max_rows;

@@ -300,6 +300,11 @@ extern "C" int ua_rotary(const UaRotary* a, float magnitude, int* status, cudaSt
   if (a->pairs < 0 || a->pairs > ROT_MAX_PAIRS || 2 * a->pairs > a->dim)
     UA_FAIL("ua_rotary: %ld pairs in heads of %ld elements (%d pairs at most)", a->pairs, a->dim, ROT_MAX_PAIRS);
   if (a->batch <= 0 || a->per_batch <= 0 || a->n_parts == 0) return 0;
+  const long most = 1l << 24;                  // (32-bit indexes)
+  if (a->per_batch > 0x7FFFFFFF || a->batch * a->per_batch > 1l << 33 || a->dim > most) UA_FAIL("ua_rotary: %ld tokens, heads of %ld elements", a->batch * a->per_batch, a->dim);
+  for (int i = 0; i < a->n_parts; ++i)
+    if (a->part[i].heads > most) UA_FAIL("ua_rotary: %ld heads", a->part[i].heads);
+  if (a->n_slots > 1l << 31) UA_FAIL("ua_rotary: a cache of %ld slots (their numbers are 32 bits wide)", a->n_slots);
   if (a->pairs > 0 && (!a->part[0].rotate || a->part[0].paged)) UA_FAIL("ua_rotary: the first tensor has to be a turned one outside the cache");
   RotParams p;
   memset(&p, 0, sizeof(p));

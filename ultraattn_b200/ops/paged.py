@@ -31,6 +31,7 @@ from . import rotary as R
 from .attention import KERNEL_HEAD_DIM, _native_call, status_buffer
 
 MAX_REQUESTS = 8192
+MAX_TOKENS = 1 << 30                  # of a step
 _ATTN = struct.Struct("30q")          # struct UaPagedAttn of csrc/paged_args.h
 
 
@@ -43,8 +44,8 @@ class PagedStep(NamedTuple):
 
 
 def _shift(page_size: int) -> int:
-    if page_size < 1 or page_size & (page_size - 1):
-        raise ValueError(f"the page size must be a power of two, not {page_size}")
+    if page_size < 1 or page_size & (page_size - 1) or page_size > 1 << 30:
+        raise ValueError(f"the page size must be a power of two up to 2^30, not {page_size}")
     return page_size.bit_length() - 1
 
 
@@ -93,8 +94,8 @@ def assign_pages(context_lens, new_lens, block_table, free_pages, free_count, *,
             return PagedStep(*r)
     sh = _shift(page_size)
     _check_pool(dict(context_lens=context_lens, new_lens=new_lens), block_table, free_pages, free_count, count_out)
-    if tokens < 0:
-        raise ValueError("tokens must not be negative")
+    if not 0 <= tokens <= MAX_TOKENS:
+        raise ValueError(f"tokens must be 0 to {MAX_TOKENS}, not {tokens}")
     dev, n = block_table.device, block_table.shape[0]
     if not block_table.is_cuda:
         return _assign_reference(context_lens, new_lens, block_table, free_pages, free_count, page_size, tokens, count_out)
@@ -125,8 +126,8 @@ def _assign_reference(context, new, table, free, count_in, page_size, tokens, co
             table[r, j] = free[count]
         at = list(range(c - k, c))
         pos += at
-        slots += [int(table[r, p // page_size]) * page_size + p % page_size if p >= 0 and table[r, p // page_size] >= 0 else -1
-                  for p in at]
+        slots += [int(table[r, p // page_size]) * page_size + p % page_size
+                  if p >= 0 and 0 <= int(table[r, p // page_size]) <= 0x7FFFFFFF // page_size else -1 for p in at]
         cu.append(cu[-1] + k)
     i32 = lambda x: torch.tensor(x, dtype=torch.int32)
     left = i32([count])
@@ -209,6 +210,8 @@ def rotary_append(q, k, v, pos, slots, k_cache, v_cache, inv_freq=None, *, inter
                               (dim > 1 and q_out.stride(-1) != 1)):
         raise ValueError("q_out must match q")
     n_slots = k_cache.shape[0] << sh
+    if n_slots > 1 << 31:
+        raise ValueError(f"slots are 32-bit numbers: at most 2^31 of them, not {n_slots}")
     if not q.is_cuda:
         turn = (lambda x: R.rotate_reference(x, pos, inv_freq, interleaved, magnitude)) if inv_freq is not None else (lambda x: x)
         if T and int(slots.max()) >= n_slots:
@@ -342,6 +345,8 @@ def paged_attention(q, k_cache, v_cache, block_table, context_lens, cu_new, *, m
         o, lse = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(H, T, dtype=torch.float32, device=q.device)
     elif o.stride(2) != 1 or o.stride(0) % 8 or o.stride(1) % 8 or o.data_ptr() % 16 or (T > 1 and lse.stride(1) != 1):
         raise ValueError("the rows of o start on 16 bytes, the tokens of lse lie side by side")
+    if H == 0:
+        return o, lse
     if H // hk > 128:
         raise ValueError(f"at most 128 query heads share a key/value head, not {H // hk}")
     block = _ATTN.pack(q.data_ptr(), T, H, q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), pages, hk,
