@@ -209,6 +209,51 @@ def test_views_and_out(device):
         assert R.rotate((e,), pos[:shape[0]], f)[0].shape == e.shape
 
 
+def _captured_gradients(q, k, pos, f):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, b = ua.rotary(q, k, pos, f)
+        grads = torch.autograd.grad((a, b), (q, k), (a.detach(), b.detach()))
+    return graph, grads
+
+
+@pytest.mark.gpu
+def test_gradients_in_a_graph():
+    """Captured behind eager calls of the same leaves whose graphs are gone, or live on a side stream, and replayed with other values.
+    A = m R is a rotation times the magnitude 1, so that A^T (A x) = x."""
+    dev = torch.device("cuda", 0)
+    q, k = (torch.randn(9, h, 64, device=dev, requires_grad=True) for h in (4, 2))
+    pos, f = torch.arange(9, dtype=torch.int32, device=dev), ua.rotary_frequencies(64, device=dev)[0]
+    torch.autograd.grad(ua.rotary(q, k, pos, f)[0].sum(), q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = ua.rotary(q, k, pos, f)
+    torch.cuda.synchronize()
+    graph, grads = _captured_gradients(q, k, pos, f)
+    for _ in range(2):
+        with torch.no_grad():
+            q.normal_(), k.normal_(), pos.random_(0, 1000)
+        graph.replay()
+        for g, x in zip(grads, (q, k)):
+            assert (g - x).abs().max() <= 16 * 2.0 ** -24 * 6         # (two rotations: four products and sums, angles to 2^-22; |x| < 6)
+    assert alive[0].grad_fn is not None
+
+
+@pytest.mark.gpu
+def test_captured_gradients_of_a_living_graph():
+    """A graph of the same leaves from the default stream still lives: refused, and the process goes on."""
+    dev = torch.device("cuda", 0)
+    q, k = (torch.randn(9, h, 64, device=dev, requires_grad=True) for h in (4, 2))
+    pos, f = torch.arange(9, dtype=torch.int32, device=dev), ua.rotary_frequencies(64, device=dev)[0]
+    alive = ua.rotary(q, k, pos, f)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="captured backward pass"):
+        _captured_gradients(q, k, pos, f)
+    dq, _ = torch.autograd.grad(alive, (q, k), (alive[0].detach(), alive[1].detach()))
+    assert (dq - q).abs().max() <= 16 * 2.0 ** -24 * 6
+
+
 @pytest.mark.gpu
 def test_more_heads_than_indexes():
     dev = torch.device("cuda", 0)

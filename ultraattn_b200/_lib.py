@@ -75,6 +75,7 @@ def _declare(lib):
         "ua_rmsnorm_bwd_res": [vp, vp, vp, vp, vp, vp, vp, i, i, vp],
         "ua_rope": [vp, vp, vp, vp, vp, l, i, l, l, i, vp],
         "ua_rotary": [c_char_p, f, vp, vp],                          # packed blocks: see ops/rotary.py, ops/paged.py
+        "ua_stream_capturing": [vp],
         "ua_attn_paged": [c_char_p, f, vp, vp, vp],
         "ua_attn_paged_workspace": [c_char_p],
         "ua_assign_pages": [vp, vp, i, vp, l, i, vp, i, vp, vp, i, i, vp, vp, vp, vp, vp],
@@ -143,7 +144,8 @@ def host():
             address = lambda name: ctypes.cast(getattr(lib, name), c_void_p).value
             mod.init(address("ua_attn_fwd_dense_parts"), address("ua_attn_fwd_dense"), address("ua_attn_bwd_local"),
                      address("ua_last_error"))
-            mod.init_paged(*map(address, ("ua_rotary", "ua_attn_paged_workspace", "ua_attn_paged", "ua_assign_pages", "ua_release_pages")))
+            mod.init_paged(*map(address, ("ua_rotary", "ua_attn_paged_workspace", "ua_attn_paged", "ua_assign_pages", "ua_release_pages",
+                                            "ua_stream_capturing")))
         _host.append(mod)
     return _host[0]
 

@@ -8,6 +8,7 @@
 //
 // The library is not linked; its entry points are handed over as addresses (init).
 #include <ATen/ATen.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -25,14 +26,16 @@ int (*rotary_launch)(const UaRotary*, float, int*, void*);
 long (*paged_workspace)(const UaPagedAttn*);
 int (*paged_attn)(const UaPagedAttn*, float, float*, int*, void*);
 int (*pages_assign)(const int*, const int*, int, int*, long, int, const int*, int, const int*, int*, int, int, int*, int*, int*, int*, void*);
+int (*stream_capturing)(void*);
 int (*pages_release)(const unsigned char*, const int*, int, const int*, long, int, int*, int, const int*, int*, int, int*, void*);
 
-void init_paged(uintptr_t rotary, uintptr_t workspace, uintptr_t attn, uintptr_t assign, uintptr_t release) {
+void init_paged(uintptr_t rotary, uintptr_t workspace, uintptr_t attn, uintptr_t assign, uintptr_t release, uintptr_t capturing) {
   rotary_launch = reinterpret_cast<decltype(rotary_launch)>(rotary);
   paged_workspace = reinterpret_cast<decltype(paged_workspace)>(workspace);
   paged_attn = reinterpret_cast<decltype(paged_attn)>(attn);
   pages_assign = reinterpret_cast<decltype(pages_assign)>(assign);
   pages_release = reinterpret_cast<decltype(pages_release)>(release);
+  stream_capturing = reinterpret_cast<decltype(stream_capturing)>(capturing);
 }
 
 void init(uintptr_t parts, uintptr_t dense, uintptr_t local, uintptr_t error) {
@@ -193,6 +196,22 @@ std::vector<Tensor> turn_pair(const Tensor& q, const Tensor& k, const Tensor& po
   return {q2, k2};
 }
 
+// A gradient that leaves a captured backward pass for a node of the default stream (the leaf of an eager graph that still lives) has that
+// stream wait for a captured one, which the engine does not survive. Refused in time.
+void refuse_leaving_capture(const at::Device& dev, void* stream) {
+  const auto node = torch::autograd::get_current_node();
+  if (stream == nullptr || !node) return;
+  const c10::Stream outside = c10::impl::VirtualGuardImpl(dev.type()).getDefaultStream(dev);
+  for (const torch::autograd::Edge& e : node->next_edges()) {
+    if (!e.function) continue;
+    const auto to = e.function->stream();
+    if (to && *to == outside && stream_capturing(stream))
+      throw std::runtime_error(
+          "rotary: the captured backward pass leads to a tensor that was used on the default stream before, by a graph that still lives; delete "
+          "that graph or run it on a side stream");
+  }
+}
+
 // The rotation with its gradient, the rotation the other way (which has a gradient in the same manner). In Python the forward took 29 us of
 // the host and the backward 86, on the engine's thread; 8192 tokens, there and back, take 60 on the device. The stream is the forward's,
 // on which the engine runs the backward too.
@@ -206,6 +225,7 @@ struct RotaryPair : torch::autograd::Function<RotaryPair> {
   static std::vector<Tensor> backward(torch::autograd::AutogradContext* ctx, std::vector<Tensor> grads) {
     const auto saved = ctx->get_saved_variables();
     const auto form = ctx->saved_data["form"].to<std::tuple<bool, double, bool, int64_t, int64_t>>();
+    refuse_leaving_capture(grads[0].device(), stream_ptr(std::get<4>(form)));
     for (Tensor& g : grads)
       if (g.stride(-1) != 1) g = g.contiguous();
     std::vector<Tensor> d;

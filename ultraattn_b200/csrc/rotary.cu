@@ -294,6 +294,12 @@ static int launch_rotary(const RotParams& p, bool wide, unsigned grid, cudaStrea
 
 using namespace ua;
 
+// 1: `stream` is being captured into a graph.
+extern "C" int ua_stream_capturing(cudaStream_t stream) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  return cudaStreamIsCapturing(stream, &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
+}
+
 extern "C" int ua_rotary(const UaRotary* a, float magnitude, int* status, cudaStream_t stream) {
   const int size = a->dtype == 2 ? 4 : 2, V = 16 / size;
   if (a->n_parts < 0 || a->n_parts > 3) UA_FAIL("ua_rotary: %ld tensors (3 at most)", a->n_parts);
