@@ -254,6 +254,29 @@ def test_captured_gradients_of_a_living_graph():
     assert (dq - q).abs().max() <= 16 * 2.0 ** -24 * 6
 
 
+@pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_gradients_again(device):
+    """Twice with and without keeping the graph, of one input alone, of positions changed in between, in forward mode (there is none)."""
+    dev = _dev(device)
+    q, k = (torch.randn(9, h, 64, device=dev, requires_grad=True) for h in (4, 2))
+    pos, f = torch.arange(9, dtype=torch.int32, device=dev), ua.rotary_frequencies(64, device=dev)[0]
+    a, b = ua.rotary(q, k, pos, f)
+    first = torch.autograd.grad((a, b), (q, k), (q, k), retain_graph=True)
+    again = torch.autograd.grad((a, b), (q, k), (q, k))
+    assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad((a, b), (q, k), (q, k))
+    a, b = ua.rotary(q.detach(), k, pos, f)
+    dk, = torch.autograd.grad((a, b), k, (q, k))
+    assert torch.equal(dk, first[1])
+    a, b = ua.rotary(q, k, pos, f)
+    pos += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad((a, b), (q, k), (q, k))
+    with torch.autograd.forward_ad.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        ua.rotary(torch.autograd.forward_ad.make_dual(q.detach(), q.detach()), k, pos, f)
+
+
 @pytest.mark.gpu
 def test_more_heads_than_indexes():
     dev = torch.device("cuda", 0)

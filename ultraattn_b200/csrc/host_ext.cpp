@@ -9,8 +9,10 @@
 // The library is not linked; its entry points are handed over as addresses (init).
 #include <ATen/ATen.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "arg_blocks.h"
@@ -183,26 +185,65 @@ bool turns_pair(const Tensor& q, const Tensor& k) {
          (d == 2 || q.size(1) == k.size(1));
 }
 
-// (q', k') in new tensors
-std::vector<Tensor> turn_pair(const Tensor& q, const Tensor& k, const Tensor& pos, const Tensor& inv_freq, bool interleaved, double magnitude, bool inverse,
-                              int64_t status, int64_t stream) {
-  const Tensor q2 = at::empty(q.sizes(), q.options()), k2 = at::empty(k.sizes(), k.options());
+// (q', k') in new tensors (undefined: left out)
+std::vector<Tensor> turn_pair(const std::vector<Tensor>& x, const Tensor& pos, const Tensor& inv_freq, bool interleaved, double magnitude, bool inverse,
+                              int* status, void* stream) {
+  std::vector<Tensor> y(2);
   UaRotary a{};
-  a.part[0] = rot_part(q, q2, true, false);
-  a.part[1] = rot_part(k, k2, true, false);
-  a.n_parts = 2;
-  rotary_common(a, q, pos, &inv_freq, interleaved, inverse);
-  check(rotary_launch(&a, static_cast<float>(magnitude), reinterpret_cast<int*>(status), stream_ptr(stream)), "ua_rotary");
-  return {q2, k2};
+  for (int i = 0; i < 2; ++i) {
+    if (!x[i].defined()) continue;
+    y[i] = at::empty(x[i].sizes(), x[i].options());
+    a.part[a.n_parts++] = rot_part(x[i], y[i], true, false);
+  }
+  if (a.n_parts == 0) return y;
+  rotary_common(a, x[0].defined() ? x[0] : x[1], pos, &inv_freq, interleaved, inverse);
+  check(rotary_launch(&a, static_cast<float>(magnitude), status, stream), "ua_rotary");
+  return y;
+}
+
+// The gradient of the rotation, the rotation the other way (which has a gradient in the same manner), of those inputs that need one. A call there
+// and back takes 69 us of the host (a product with 2.0: 52, the engine's hand-over to its thread; in Python 115); 8192 tokens take 59 on the
+// device. The stream is the forward's, on which the engine runs the backward too.
+struct RotaryBackward : torch::autograd::Node {
+  torch::autograd::SavedVariable pos, inv_freq;
+  bool interleaved, inverse;
+  double magnitude;
+  int* status;
+  void* stream;
+
+  std::string name() const override { return "RotaryBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    pos.reset_data();
+    inv_freq.reset_data();
+  }
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override;
+};
+
+std::vector<Tensor> turn_with_gradient(const std::vector<Tensor>& x, const Tensor& pos, const Tensor& inv_freq, bool interleaved, double magnitude, bool inverse,
+                                       int* status, void* stream) {
+  std::vector<Tensor> y = turn_pair(x, pos, inv_freq, interleaved, magnitude, inverse, status, stream);
+  if (c10::GradMode::is_enabled() && ((x[0].defined() && x[0].requires_grad()) || (x[1].defined() && x[1].requires_grad()))) {
+    const std::shared_ptr<RotaryBackward> node(new RotaryBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x[0], x[1]));
+    node->pos = torch::autograd::SavedVariable(pos, false);
+    node->inv_freq = torch::autograd::SavedVariable(inv_freq, false);
+    node->interleaved = interleaved;
+    node->inverse = inverse;
+    node->magnitude = magnitude;
+    node->status = status;
+    node->stream = stream;
+    torch::autograd::set_history(y, node);
+  }
+  return y;
 }
 
 // A gradient that leaves a captured backward pass for a node of the default stream (the leaf of an eager graph that still lives) has that
 // stream wait for a captured one, which the engine does not survive. Refused in time.
-void refuse_leaving_capture(const at::Device& dev, void* stream) {
-  const auto node = torch::autograd::get_current_node();
-  if (stream == nullptr || !node) return;
+void refuse_leaving_capture(const torch::autograd::Node& node, const at::Device& dev, void* stream) {
+  if (stream == nullptr) return;
   const c10::Stream outside = c10::impl::VirtualGuardImpl(dev.type()).getDefaultStream(dev);
-  for (const torch::autograd::Edge& e : node->next_edges()) {
+  for (const torch::autograd::Edge& e : node.next_edges()) {
     if (!e.function) continue;
     const auto to = e.function->stream();
     if (to && *to == outside && stream_capturing(stream))
@@ -212,38 +253,24 @@ void refuse_leaving_capture(const at::Device& dev, void* stream) {
   }
 }
 
-// The rotation with its gradient, the rotation the other way (which has a gradient in the same manner). In Python the forward took 29 us of
-// the host and the backward 86, on the engine's thread; 8192 tokens, there and back, take 60 on the device. The stream is the forward's,
-// on which the engine runs the backward too.
-struct RotaryPair : torch::autograd::Function<RotaryPair> {
-  static std::vector<Tensor> forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& pos, const Tensor& inv_freq,
-                                     bool interleaved, double magnitude, bool inverse, int64_t status, int64_t stream) {
-    ctx->save_for_backward({pos, inv_freq});
-    ctx->saved_data["form"] = c10::IValue(std::tuple<bool, double, bool, int64_t, int64_t>(interleaved, magnitude, inverse, status, stream));
-    return turn_pair(q, k, pos, inv_freq, interleaved, magnitude, inverse, status, stream);
-  }
-  static std::vector<Tensor> backward(torch::autograd::AutogradContext* ctx, std::vector<Tensor> grads) {
-    const auto saved = ctx->get_saved_variables();
-    const auto form = ctx->saved_data["form"].to<std::tuple<bool, double, bool, int64_t, int64_t>>();
-    refuse_leaving_capture(grads[0].device(), stream_ptr(std::get<4>(form)));
-    for (Tensor& g : grads)
-      if (g.stride(-1) != 1) g = g.contiguous();
-    std::vector<Tensor> d;
-    if (c10::GradMode::is_enabled())
-      d = apply(grads[0], grads[1], saved[0], saved[1], std::get<0>(form), std::get<1>(form), !std::get<2>(form), std::get<3>(form), std::get<4>(form));
-    else
-      d = turn_pair(grads[0], grads[1], saved[0], saved[1], std::get<0>(form), std::get<1>(form), !std::get<2>(form), std::get<3>(form), std::get<4>(form));
-    return {d[0], d[1], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
-  }
-};
+torch::autograd::variable_list RotaryBackward::apply(torch::autograd::variable_list&& grads) {
+  std::lock_guard<std::mutex> lock(mutex_);
+  const Tensor p = pos.unpack(), f = inv_freq.unpack();
+  refuse_leaving_capture(*this, f.device(), stream);
+  std::vector<Tensor> g(2);
+  for (int i = 0; i < 2; ++i)
+    if (grads[i].defined() && task_should_compute_output(i)) g[i] = grads[i].stride(-1) == 1 ? grads[i] : grads[i].contiguous();
+  return turn_with_gradient(g, p, f, interleaved, magnitude, !inverse, status, stream);
+}
 
 py::object rotate_pair(py::handle qh, py::handle kh, py::handle ph, py::handle fh, bool interleaved, double magnitude, uintptr_t status, uintptr_t stream) {
   const Plain x{qh, kh, ph, fh};
   if (!x.ok || !turns_pair(x.t[0], x.t[1]) || !angles_fit(x.t[0], x.t[2], x.t[3])) return py::none();
+  if (x.t[0]._fw_grad(0).defined() || x.t[1]._fw_grad(0).defined()) return py::none();        // (forward mode: refused in Python)
   std::vector<Tensor> r;
   {
     py::gil_scoped_release nogil;
-    r = RotaryPair::apply(x.t[0], x.t[1], x.t[2], x.t[3], interleaved, magnitude, false, static_cast<int64_t>(status), static_cast<int64_t>(stream));
+    r = turn_with_gradient({x.t[0], x.t[1]}, x.t[2], x.t[3], interleaved, magnitude, false, reinterpret_cast<int*>(status), stream_ptr(stream));
   }
   return py::make_tuple(r[0], r[1]);
 }
