@@ -560,8 +560,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
 }
 
 // The parts of a cut item, in the order of its keys: O = sum_i w_i O_i with w_i = exp(lse_i - lse), fp32, 4 elements of a row per lane.
-// Block (x, y, z): rows 32 y .. of the item that begins in CTA x of launch z and goes on behind it, if there is one. Latency of the chain
-// description -> lse -> parts and the parts' bytes (mostly in L2): a warp has four rows under way, so that all blocks are there at once.
+// Block (x, y, z): rows 8 ROWS y .. of the item that begins in CTA x of launch z and goes on behind it, if there is one. Latency: a kernel's
+// boundary (1.3 us), instructions that are not in the cache, loads one behind the other, the parts' bytes (mostly in L2).
+//   ROWS 1  items of up to 32 rows: little code, and what may be asked for is loaded together with the description. One request of 1500 keys, in all:
+//           11.8 us with ROWS 4, 11.1 with 1, 10.2 with the loads at once; 33 behind a window of 4096 23.4, 23.0, 22.4
+//   ROWS 4  others: a warp has four rows under way, so that all blocks are there at once
 struct CombineParams {
   const float* part_o[2];
   const float* part_lse[2];
@@ -574,8 +577,12 @@ struct CombineParams {
   float* lse;
   long lse_head;
 };
-constexpr int COMBINE_ROWS = 32;       // rows of a block
-__global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constant__ CombineParams p) {
+static_assert(sizeof(CombineParams) % 4 == 0 && sizeof(CombineParams) <= 256 * 4, "copied by one block");
+template <int ROWS>                    // of a warp
+__global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constant__ CombineParams args) {
+  __shared__ CombineParams p;          // (before the wait: see PagedScalars)
+  if (threadIdx.x < sizeof(CombineParams) / 4) reinterpret_cast<int*>(&p)[threadIdx.x] = reinterpret_cast<const int*>(&args)[threadIdx.x];
+  __syncthreads();
   grid_wait();
   grid_trigger();
   const int first = blockIdx.x, z = blockIdx.z, lane = threadIdx.x & 31;
@@ -583,9 +590,21 @@ __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constan
   const float *part_o = p.part_o[z], *part_lse = p.part_lse[z];
   const long part_rows = p.part_rows[z];
   // its head, and how far it goes: up to the next CTA that does not say that its part goes on (one load for all)
-  const int x0 = blockIdx.y * COMBINE_ROWS + (threadIdx.x >> 5);
+  const int x0 = blockIdx.y * (8 * ROWS) + (threadIdx.x >> 5);
   const int4 d = *reinterpret_cast<const int4*>(desc + first * PA_DESC);
   const int ahead = first + 1 + lane < p.ctas ? desc[(first + 1 + lane) * PA_DESC + 4] : 0;
+  // the slots of its parts: 2 first + 1, then 2 (first + 1), 2 (first + 2) ..
+  auto row_of = [&](int i, int x) -> long { return (i == 0 ? 2 * first + 1 : 2 * (first + i)) * part_rows + x; };
+  auto lse_of = [&](int i, int k) -> float { return part_lse[row_of(i, x0 + 8 * k)]; };
+  auto o_of = [&](int i, int k) -> float4 { return *reinterpret_cast<const float4*>(part_o + row_of(i, x0 + 8 * k) * PD + lane * 4); };
+  constexpr bool at_once = ROWS == 1;
+  float y[ROWS];                       // lane i: lse of part i
+  float4 o0, o1;
+  if (at_once && x0 < part_rows) {     // (in the workspace, written or not)
+    y[0] = first + lane < p.ctas ? lse_of(lane, 0) : 0.f;
+    o0 = o_of(0, 0);
+    o1 = o_of(first + 1 < p.ctas ? 1 : 0, 0);
+  }
   if (d.x == 0 || x0 >= d.w) return;
   unsigned ends = __ballot_sync(0xFFFFFFFFu, ahead != 1);
   int n = 1;
@@ -594,27 +613,27 @@ __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constan
     ends = __ballot_sync(0xFFFFFFFFu, first + n + lane >= p.ctas || desc[(first + n + lane) * PA_DESC + 4] != 1);
   }
   n += __ffs(ends);
-  // the slots of its parts: 2 first + 1, then 2 (first + 1), 2 (first + 2) ..
-  auto row_of = [&](int i, int x) -> long { return (i == 0 ? 2 * first + 1 : 2 * (first + i)) * part_rows + x; };
   // lane i: the lse of part i (and of parts 32 + i ..), then its weight; the parts themselves in one go behind that
-  float mx[4];
-  bool bad[4];                         // a NaN score, in O and lse as in an item that is not cut
+  float mx[ROWS];
+  bool bad[ROWS];                      // a NaN score, in O and lse as in an item that is not cut
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    mx[k] = -INFINITY;
-    bad[k] = false;
+  for (int k = 0; k < ROWS; ++k) {
+    if (lane >= n || x0 + 8 * k >= d.w) y[k] = -INFINITY;
+    else if (!at_once) y[k] = lse_of(lane, k);
+    mx[k] = y[k];
+    bad[k] = y[k] != y[k];
   }
-  for (int i = lane; i < n; i += 32)
+  for (int i = lane + 32; i < n; i += 32)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float y = x0 + 8 * k < d.w ? part_lse[row_of(i, x0 + 8 * k)] : -INFINITY;
-      bad[k] |= y != y;
-      mx[k] = fmaxf(mx[k], y);
+    for (int k = 0; k < ROWS; ++k) {
+      const float t = x0 + 8 * k < d.w ? lse_of(i, k) : -INFINITY;
+      bad[k] |= t != t;
+      mx[k] = fmaxf(mx[k], t);
     }
-  float tot[4];
-  float4 acc[4];
+  float tot[ROWS];
+  float4 acc[ROWS];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < ROWS; ++k) {
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xFFFFFFFFu, mx[k], s));
     bad[k] = __any_sync(0xFFFFFFFFu, bad[k]);
@@ -622,33 +641,43 @@ __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constan
     tot[k] = 0.f;
     acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  auto add = [&](int k, float f, const float4& v) {      // (f = 0 times what is not finite: as P V does with P = 0)
+    acc[k].x += f * v.x;
+    acc[k].y += f * v.y;
+    acc[k].z += f * v.z;
+    acc[k].w += f * v.w;
+  };
   for (int i0 = 0; i0 < n; i0 += 32) {
-    float w[4];
+    float w[ROWS];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      w[k] = i0 + lane < n && mx[k] > -INFINITY ? __expf(part_lse[row_of(i0 + lane, x0 + 8 * k)] - mx[k]) : 0.f;
+    for (int k = 0; k < ROWS; ++k) {
+      w[k] = i0 + lane < n && mx[k] > -INFINITY ? __expf((i0 == 0 ? y[k] : lse_of(i0 + lane, k)) - mx[k]) : 0.f;
       tot[k] += w[k];
+    }
+    int i = 0;
+    if (at_once && i0 == 0) {
+      i = 2;                           // (n > 1)
+      const float f0 = __shfl_sync(0xFFFFFFFFu, w[0], 0), f1 = __shfl_sync(0xFFFFFFFFu, w[0], 1);
+      if (mx[0] > -INFINITY) {
+        add(0, f0, o0);
+        add(0, f1, o1);
+      }
     }
     const int here = min(32, n - i0);
 #pragma unroll 4
-    for (int i = 0; i < here; ++i)
+    for (; i < here; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < ROWS; ++k) {
         const float f = __shfl_sync(0xFFFFFFFFu, w[k], i);
-        if (!(mx[k] > -INFINITY)) continue;
-        const float4 v = *reinterpret_cast<const float4*>(part_o + row_of(i0 + i, x0 + 8 * k) * PD + lane * 4);
-        acc[k].x += f * v.x;           // (f = 0 times what is not finite: as P V does with P = 0)
-        acc[k].y += f * v.y;
-        acc[k].z += f * v.z;
-        acc[k].w += f * v.w;
+        if (mx[k] > -INFINITY) add(k, f, o_of(i0 + i, k));
       }
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
+  for (int k = 0; k < ROWS; ++k)
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) tot[k] += __shfl_xor_sync(0xFFFFFFFFu, tot[k], s);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < ROWS; ++k) {
     const int x = x0 + 8 * k, h = x & ((1 << p.pack_shift) - 1);
     if (x >= d.w || h >= p.group) continue;
     const float inv = bad[k] ? NAN : tot[k] > 0.f ? 1.f / tot[k] : 0.f;
@@ -800,6 +829,7 @@ extern "C" int ua_attn_paged(const UaPagedAttn* a, float softmax_scale, float* w
   c.o_head = p.c.o_head;
   c.lse = p.c.lse;
   c.lse_head = p.c.lse_head;
-  UA_CUDA(launch_kernel(combine_parts_kernel, dim3(ctas, (most_part_rows + COMBINE_ROWS - 1) / COMBINE_ROWS, d.n), 256, 0, stream, true, c));
+  if (most_part_rows <= 32) UA_CUDA(launch_kernel(combine_parts_kernel<1>, dim3(ctas, (most_part_rows + 7) / 8, d.n), 256, 0, stream, true, c));
+  else UA_CUDA(launch_kernel(combine_parts_kernel<4>, dim3(ctas, (most_part_rows + 31) / 32, d.n), 256, 0, stream, true, c));
   return 0;
 }
