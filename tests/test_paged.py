@@ -406,6 +406,57 @@ def test_attention_many_requests(new, heads, page):
     A.check_status(dev)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("graph", [False, True])
+def test_mixed_steps_in_a_row(graph):
+    """Steps of requests of all forms, whose queries, cache and lengths are written right in front of each and whose results are read right
+    behind: two launches that work side by side neither begin too early nor end too late."""
+    dev = _dev("cuda")
+    steps = []
+    for seed in range(3):
+        g = torch.Generator().manual_seed(seed)
+        new = [700, 1, 1, 40, 1, 300, 1, 1, 5, 1, 1, 200] if seed < 2 else [1] * 11 + [900]
+        context = [n + int(x) for n, x in zip(new, torch.randint(0, 5000, (12,), generator=g))]
+        steps.append(_problem(dev, context, new, 32, 8, 32, seed=seed, pad=1300 - sum(new)))
+    pages = max(s[1].shape[0] for s in steps)
+    width = max(s[3].shape[1] for s in steps)
+    q, table = torch.empty_like(steps[0][0]), torch.empty(12, width, dtype=torch.int32, device=dev)
+    kc, vc = (torch.empty(pages, 32, 8, 128, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    ctx, cu = torch.empty_like(steps[0][4]), torch.empty_like(steps[0][5])
+
+    def step(s):
+        q.copy_(s[0]), kc[:s[1].shape[0]].copy_(s[1]), vc[:s[2].shape[0]].copy_(s[2])
+        table[:, :s[3].shape[1]].copy_(s[3]), ctx.copy_(s[4]), cu.copy_(s[5])
+        o, lse = ua.paged_attention(q, kc, vc, table, ctx, cu)
+        kept = o.clone(), lse.clone()
+        o.zero_(), lse.zero_()
+        return kept
+
+    want = []
+    for s in steps:
+        torch.cuda.synchronize()
+        want.append(step(s))
+        torch.cuda.synchronize()
+    order = [0, 1, 2, 1, 0, 2, 2, 0, 1] * 3
+    if graph:
+        captured = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(captured):
+            got = [step(steps[i]) for i in order]
+        captured.replay()
+        captured.replay()
+    else:
+        got = [step(steps[i]) for i in order]
+    torch.cuda.synchronize()
+    A.check_status(dev)
+    for i, (o, lse) in zip(order, got):
+        n = int(steps[i][5][-1])
+        assert torch.equal(o[:n], want[i][0][:n]) and torch.equal(lse[:, :n], want[i][1][:, :n])
+    s, (o, lse) = steps[0], want[0]
+    for r in (0, 1, 3, 8):
+        a, b, c = int(s[5][r]), int(s[5][r + 1]), int(s[4][r])
+        _close(o[a:b], lse[:, a:b], *_exact(s[0][a:b], s[6][r], s[7][r], c, b - a, 128 ** -0.5, -1, 0))
+
+
 @pytest.mark.parametrize("device", ["cpu", CUDA])
 def test_attention_ignores_pages_outside_the_window(device):
     """Pages that no query sees any more may be given back: their entries name no page, or one that holds anything."""

@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __g
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = s.tmem_base;            // S0 | S1 | O0 | O1, N columns each
-  grid_wait();
+  if (!p.beside) grid_wait();
   const int psh = p.pack_shift;
 
   WaitCtx wc{&s.abort_flag, p.status, 4000000000ull};
@@ -391,6 +391,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) attn_paged_few_kernel(const __g
     }
   }
 
+  if (p.beside) grid_wait();
   tc_fence_before_sync();
   __syncthreads();
   if (warp == PF_MMA_WARP) {
