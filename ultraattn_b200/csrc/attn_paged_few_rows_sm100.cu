@@ -5,7 +5,8 @@
 // O^T += V^T P^T (128 head-dim elements x N rows), keys and values being the operands with 128 rows. A lane is a key, four warps
 // take N exponentials each, the maximum of a row is found only when a score is more than 2^8 above the one in use (one
 // vote of the four warps per tile), the row sums stay spread over the lanes until the item's end, and O^T is N columns of tensor
-// memory. Bound by reading the keys and values (64 KB a tile, three tiles in flight).
+// memory. Bound by reading the keys and values (64 KB a tile, three tiles in flight): 48 requests of 20 to 16000 keys, 32 / 8 heads, 92 to 94 us,
+// 5.9 of the 6.5 TB/s that a copy reaches; short steps by what a CTA takes to begin and end (one request of 1500 keys 10.1 us).
 //
 // Two groups of four warps take the key tiles in turn, each with its own S^T, P^T and O^T; one warp loads keys, one values, one
 // issues the products, one walks the share. (A share for each group, so that one goes on while the other ends an item: the products are

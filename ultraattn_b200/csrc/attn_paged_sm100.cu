@@ -10,7 +10,8 @@
 // A row is a query head of a token: row x of an item is token x / G', head x % G' of the group of G heads that shares a key/value head,
 // G' the next power of two (rows of heads behind G are computed and not stored), so that a key is read once for its group.
 //
-// How the work is found and shared out, and the loads: paged_attn.cuh.
+// Bound by the tensor core and what stands between its products, as attn_fwd_sm100.cu: 8192 tokens, 32 / 8 heads, 481 us (1143 TFLOP/s; 462 over
+// contiguous keys there), 512 tokens behind 32256 keys 247 to 261 (245 to 249). How the work is found and shared out, and the loads: paged_attn.cuh.
 #include "paged_attn.cuh"
 
 namespace ua {
