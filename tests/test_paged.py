@@ -304,11 +304,11 @@ def _close(o, lse, want_o, want_lse, weight):
     assert (d <= 2.0 ** -11 + 2.0 ** -22 * want_lse[~dead].abs()).all(), f"lse is off by {d.max():.3g}"
 
 
-def _problem(dev, context, new, H, Hk, page, dtype=torch.bfloat16, layout="tokens first", seed=0, pad=0, scale_q=1.0, D=128, extra=2):
+def _problem(dev, context, new, H, Hk, page, dtype=torch.bfloat16, layout="tokens first", seed=0, pad=0, scale_q=1.0, D=128, extra=2, columns=0):
     """A cache whose every place that no request has written holds NaN, and what its requests have written."""
     g = torch.Generator().manual_seed(seed + sum(context) + 7 * H + page)
     n_pages = [-(-c // page) for c in context]
-    total, width = sum(n_pages) + extra, max(n_pages + [0]) + 1
+    total, width = sum(n_pages) + extra, max(n_pages + [0, columns - 1]) + 1
     order = torch.randperm(total, generator=g).tolist()
     table, at = [], 0
     for n in n_pages:
@@ -404,6 +404,24 @@ def test_attention_many_requests(new, heads, page):
         o2, lse2 = ua.paged_attention(q, kc, vc, table, ctx, cu, most_new=new)
         assert torch.equal(o, o2) and torch.equal(lse, lse2)
     A.check_status(dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", BATCHES)
+@pytest.mark.parametrize("heads,kv,page", [(8, 2, 16), (4, 4, 64), (7, 1, 128), (6, 2, 32), (24, 1, 64), (100, 1, 64), (128, 1, 64)])
+def test_attention_in_large_items(name, heads, kv, page):
+    """A table wide enough for a million keys: small steps take the form of large ones."""
+    context, new = BATCHES[name]
+    _check(_dev("cuda"), context, new, heads, kv, page, columns=(1 << 20) // page)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["chunks", "mixed", "prompts", "more new than context"])
+@pytest.mark.parametrize("left,sink", [(0, 0), (63, 4), (127, 0), (128, 130), (500, 1)])
+def test_attention_window_in_large_items(name, left, sink):
+    """So many heads that there are more items of 256 rows than SMs."""
+    context, new = BATCHES[name]
+    _check(_dev("cuda"), context, new, 64, 64, 32, left=left, sink=sink)
 
 
 @pytest.mark.gpu
@@ -507,17 +525,19 @@ def test_attention_large_scores(device):
     _check(_dev(device), [700, 260], [1, 260], 8, 2, 64, scale_q=4.0)
 
 
-# (context, new, query heads of one key/value head): items of 16, 32, 128 and 256 rows; short ones, and long ones in parts
+# (context, new, query heads of one key/value head): items of 16, 32 and 128 rows, with many columns in the
+# table 256 instead of 128; short ones, and long ones in parts
 NAN_BATCHES = [([40, 9000], [1, 1], 4), ([40, 9000], [1, 1], 16), ([40, 9000], [1, 20], 4), ([100, 9000], [70, 90], 4)]
 
 
 @pytest.mark.parametrize("device", ["cpu", CUDA])
 @pytest.mark.parametrize("value", [NAN, math.inf])
+@pytest.mark.parametrize("columns", [0, 1 << 14])
 @pytest.mark.parametrize("context,new,heads", NAN_BATCHES)
-def test_attention_of_a_nan(device, context, new, heads, value):
+def test_attention_of_a_nan(device, context, new, heads, columns, value):
     """A row with a NaN among the scores that it sees is NaN, not 0; the others are what they are."""
     dev = _dev(device)
-    q, kc, vc, table, ctx, cu, keys, values = _problem(dev, context, new, heads, 1, 64)
+    q, kc, vc, table, ctx, cu, keys, values = _problem(dev, context, new, heads, 1, 64, columns=columns)
     exact = [_exact(x, kk, vv, c, n, 128 ** -0.5, -1, 0) for x, kk, vv, c, n in zip(q.split(new), keys, values, context, new)]
     want, want_lse, weight = torch.cat([x[0] for x in exact]), torch.cat([x[1] for x in exact], 1), torch.cat([x[2] for x in exact])
     # one head of one query of the long request (an infinity: one score of +inf or -inf, a NaN with the next one)
@@ -537,11 +557,12 @@ def test_attention_of_a_nan(device, context, new, heads, value):
 
 
 @pytest.mark.parametrize("device", ["cpu", CUDA])
+@pytest.mark.parametrize("columns", [0, 1 << 14])
 @pytest.mark.parametrize("context,new,heads", NAN_BATCHES)
-def test_attention_far_below_zero(device, context, new, heads):
+def test_attention_far_below_zero(device, context, new, heads, columns):
     """Scores of -1e32 and less: still seen, and the first key (of -1e32, the others -2e32) has all the weight."""
     dev = _dev(device)
-    q, kc, vc, table, ctx, cu, _, _ = _problem(dev, context, new, heads, 1, 64)
+    q, kc, vc, table, ctx, cu, _, _ = _problem(dev, context, new, heads, 1, 64, columns=columns)
     q.fill_(-2.0 ** 50)
     for r, c in enumerate(context):
         j = torch.arange(c, device=dev)

@@ -5,13 +5,15 @@
 //
 // One pass over the keys in tiles of 128 with the running maximum and sum of a row in registers, as in attn_fwd_sm100.cu, whose
 // roles and tensor-memory layouts these are (12 warps: 8 softmax, TMA, two MMA issuers):
-//   FEW    requests of up to 128 rows (decoding, short chunks): both sub-tiles hold the same rows and take the key tiles in turn
-//   !FEW   the others: items of 256 rows, 128 in each sub-tile
+//   FEW    items of 128 rows (short chunks, small steps): both sub-tiles hold the same rows and take the key tiles in turn
+//   !FEW   items of 256 rows, 128 in each sub-tile
 // A row is a query head of a token: row x of an item is token x / G', head x % G' of the group of G heads that shares a key/value head,
 // G' the next power of two (rows of heads behind G are computed and not stored), so that a key is read once for its group.
 //
 // Bound by the tensor core and what stands between its products, as attn_fwd_sm100.cu: 8192 tokens, 32 / 8 heads, 481 us (1143 TFLOP/s; 462 over
 // contiguous keys there), 512 tokens behind 32256 keys 247 to 261 (245 to 249). How the work is found and shared out, and the loads: paged_attn.cuh.
+#include <algorithm>
+
 #include "paged_attn.cuh"
 
 namespace ua {
@@ -125,7 +127,7 @@ __device__ __forceinline__ void paged_epilogue(const PagedScalars& p, PagedSmem<
   }
 }
 
-// Up to 128 rows, of whose key tiles each sub-tile has seen half: sub-tile 0's warps merge both O from tensor memory.
+// 128 rows, of whose key tiles each sub-tile has seen half: sub-tile 0's warps merge both O from tensor memory.
 __device__ __forceinline__ void paged_few_epilogue(const PagedScalars& p, PagedSmem<true>& s, const PagedItem& it, uint32_t tO, float l0, float m0) {
   const int x = threadIdx.x;
   const float2 other = s.stat[x];
@@ -693,6 +695,7 @@ __global__ void __launch_bounds__(256) combine_parts_kernel(const __grid_constan
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
+constexpr long PA_SMALL_TILES = 16;
 // The launches of a call: the form (rows of an item), the requests that each takes by their rows, and the rows of its parts.
 struct PagedPlan {
   int pack_shift, n;
@@ -714,7 +717,16 @@ static PagedPlan plan_paged(const UaPagedAttn* a) {
   // several requests: most of them may bring a token each
   const int below = a->requests > 1 && (1 << d.pack_shift) <= 32 ? (1 << d.pack_shift) <= 16 ? 16 : 32 : 0;
   // (requests of a few tokens beside a long one go with it: a launch of their own took 13 us in a step of 20 requests)
-  add(most <= PT ? PT : 2 * PT, below, most);
+  // 128 rows where 256 leave SMs without an item, or a few tiles to each: half as long an item, half as much to merge (by what the host knows
+  // of the keys, the columns of the table and the window; items of 256 rows x their tiles for an SM at most).
+  //   47 tokens behind 1010, 28 / 4 heads (0.5 tiles) 27 us with 256 rows, 20 with 128; 277 behind 18500, 4 / 1 (5) 43, 36; 17 requests of up to 1196, 4 / 2
+  //   (13) 42, 33; 668 behind 10760, 8 / 2 (13) 50, 51; 993 behind 5346, 12 / 4 (22) 62, 67; 1479 behind 16452, 6 / 2 (45) 98, 136: each key
+  //   tile is loaded twice as often
+  const long item_tokens = 2 * PT >> d.pack_shift, items = (a->tokens / item_tokens + a->requests) * a->kv_heads;
+  long tiles = ((a->columns << a->page_shift) + PT - 1) / PT;
+  if (a->left >= 0 && a->left < 1l << 31) tiles = std::min(tiles, (a->left + item_tokens) / PT + 2 + (a->sink + PT - 1) / PT);
+  const bool small = items <= sm_count() && items * tiles <= PA_SMALL_TILES * sm_count();
+  add(most <= PT || small ? PT : 2 * PT, below, most);
   if (below > 0) add(below, 0, below);
   return d;
 }

@@ -5,7 +5,7 @@
 // the next power of two (rows of heads behind G are computed and not stored), so that a key is read once for its group. An item
 // is ROWS rows of a request and key/value head:
 //   16, 32   decoding and the like   (attn_paged_few_rows_sm100.cu)
-//   128      short chunks            (attn_paged_sm100.cu)
+//   128      short chunks and small steps  (attn_paged_sm100.cu)
 //   256      the others
 // and every launch takes the requests with p.min_rows < rows <= p.max_rows.
 //
@@ -138,7 +138,7 @@ struct PagedRequest {
   // weight of the first m row tiles of a key/value head: their key tiles and PA_ITEM_TILES each (a window: an upper bound that is
   // the same for all; what a share's border means is settled per item, with its own number of tiles)
   __device__ __forceinline__ long weight(const PagedScalars& p, int m) const {
-    if (ROWS < 256) {
+    if (ROWS <= 32) {
       PagedItem it;
       return m == 0 ? 0 : PA_ITEM_TILES<ROWS> + tiles(p, 0, it);
     }
@@ -153,7 +153,7 @@ struct PagedRequest {
     if (past < 0) {                            // (more new tokens than the request has)
       for (int i = 0; i < full; ++i) w += max(0, past + (i + 1) * tpt + PT - 1) / PT;
     } else if (tpt < PT) {                     // sum of ceil((past + i tpt) / 128): tpt divides 128 ...
-      w += ceil_sum((past + tpt - 1) / tpt, full, p.pack_shift - 1);
+      w += ceil_sum((past + tpt - 1) / tpt, full, ROWS == 256 ? p.pack_shift - 1 : p.pack_shift);
     } else {                                   // ... or is 128 or 256
       w += static_cast<long>(full) * ((past + PT - 1) / PT) + (tpt / PT) * (static_cast<long>(full) * (full + 1) / 2);
     }
@@ -205,7 +205,7 @@ struct PagedWalk {
     while (r < p.requests) {
       q = paged_request<ROWS>(p, r, ahead[0], ahead[1], ahead[2], false);
       look_ahead(p);
-      same = ROWS < 256 || p.left < 0 ? 0 : static_cast<int>(q.weight(p, 1));
+      same = ROWS <= 32 || p.left < 0 ? 0 : static_cast<int>(q.weight(p, 1));
       if (q.row_tiles > 0) return;
       ++r;
     }
@@ -292,7 +292,7 @@ struct PagedWalk {
     q.past = __shfl_sync(0xFFFFFFFFu, q.past, from);
     q.q_row = __shfl_sync(0xFFFFFFFFu, q.q_row, from);
     q.row_tiles = __shfl_sync(0xFFFFFFFFu, q.row_tiles, from);
-    same = ROWS < 256 || p.left < 0 ? 0 : static_cast<int>(q.weight(p, 1));
+    same = ROWS <= 32 || p.left < 0 ? 0 : static_cast<int>(q.weight(p, 1));
     look_ahead(p);
     const long per_head = q.weight(p, q.row_tiles);
     head = (y >> 32) == 0 ? static_cast<int>(static_cast<unsigned>(y) / static_cast<unsigned>(per_head)) : static_cast<int>(y / per_head);
