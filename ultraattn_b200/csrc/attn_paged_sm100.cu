@@ -567,7 +567,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_paged_kernel(const __grid_
 // boundary (1.3 us), instructions that are not in the cache, loads one behind the other, the parts' bytes (mostly in L2).
 //   ROWS 1  items of up to 32 rows: little code, and what may be asked for is loaded together with the description. One request of 1500 keys, in all:
 //           11.8 us with ROWS 4, 11.1 with 1, 10.2 with the loads at once; 33 behind a window of 4096 23.4, 23.0, 22.4
-//   ROWS 4  others: a warp has four rows under way, so that all blocks are there at once
+//   ROWS 2  up to 128 rows, ROWS 4 256: a warp has so many rows under way that all blocks are there at once. 277 tokens behind 18500 keys, 4 / 1 heads,
+//           in all: 31.1 us with 2, 35.3 with 4, 31.6 with 1; 100 behind 3900, 32 / 8 heads, 25.4, 26.8, 28.8
 struct CombineParams {
   const float* part_o[2];
   const float* part_lse[2];
@@ -841,6 +842,7 @@ extern "C" int ua_attn_paged(const UaPagedAttn* a, float softmax_scale, float* w
   c.lse = p.c.lse;
   c.lse_head = p.c.lse_head;
   if (most_part_rows <= 32) UA_CUDA(launch_kernel(combine_parts_kernel<1>, dim3(ctas, (most_part_rows + 7) / 8, d.n), 256, 0, stream, true, c));
+  else if (most_part_rows <= PT) UA_CUDA(launch_kernel(combine_parts_kernel<2>, dim3(ctas, (most_part_rows + 15) / 16, d.n), 256, 0, stream, true, c));
   else UA_CUDA(launch_kernel(combine_parts_kernel<4>, dim3(ctas, (most_part_rows + 31) / 32, d.n), 256, 0, stream, true, c));
   return 0;
 }
