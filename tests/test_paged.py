@@ -362,6 +362,8 @@ BATCHES = {
     "more new than context": ([2, 40, 0], [5, 40, 3]),
     "nothing new": ([50, 70], [0, 0]),
     "chunk behind a long context": ([5000], [200]),
+    "one prompt": ([1100], [1100]),
+    "one chunk": ([900], [300]),
 }
 
 
@@ -416,7 +418,7 @@ def test_attention_in_large_items(name, heads, kv, page):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("name", ["chunks", "mixed", "prompts", "more new than context"])
+@pytest.mark.parametrize("name", ["chunks", "mixed", "prompts", "more new than context", "one prompt", "one chunk"])
 @pytest.mark.parametrize("left,sink", [(0, 0), (63, 4), (127, 0), (128, 130), (500, 1)])
 def test_attention_window_in_large_items(name, left, sink):
     """So many heads that there are more items of 256 rows than SMs."""

@@ -77,7 +77,11 @@ static_assert(sizeof(PagedScalars) % 4 == 0 && sizeof(PagedScalars) <= 64 * 4, "
 // rows (1 - 3); 4: the part of one that began before (0 none, 1 goes on, 2 ends)
 constexpr int PA_DESC = 8;
 
-constexpr int PA_DEAL = 8;                    // see PagedWalk::start
+// One request's items are dealt out whole if that costs fewer key tiles of every CTA than this (see PagedWalk::start). 256 rows, 32 / 8 heads, never and
+// always: 1500 tokens (4) 46 and 33 us, 2048 (3) 57 and 43, 1300 behind 600 (9) 53 and 41, 3000 behind 1500 (10) 143 and 135, 1300 behind 1700 (16) 70
+// and 69, 3000 behind 3000 (15) 188 and 188; 8192 behind a window of 2048 (2) 258 and 241. 128 rows: 1000 tokens (7) 33 and 25, 100 behind 900 (9)
+// 20.8 and 19.3, 47 behind 1010, 28 / 4 (11) 19.4 and 20.2, 64 behind 1936, 16 / 8 (18) 20 and 28.
+template <int ROWS> constexpr int PA_DEAL = ROWS == 256 ? 12 : 10;
 constexpr int PA_NO_PAGE = -0x7FFFFFFF;
 constexpr int PA_ITEMS = 3;                   // items in shared memory: the one before may still be written out
 
@@ -246,24 +250,26 @@ struct PagedWalk {
     const long most = total / PA_MIN_SHARE;
     int ctas = static_cast<int>(most < 1 ? 1 : most < all_ctas ? most : all_ctas);
     if (total == 0) return false;
-    if (ROWS == 256 && p.requests == 1) {
-      // One request. A chunk behind a long context: all items have about the same keys, and as many CTAs as give each the same number of equal
-      // parts walk them in step, so that a key tile comes out of DRAM once for all (512 queries behind 32768 keys, 64 items, on the
-      // device: 148 equal shares 265 us, 128 of them 260).
+    if (ROWS >= 128 && p.requests == 1) {
+      // One request. Whole items, dealt out from the longest on, every other round backwards, end about as evenly as equal shares, and nothing has
+      // to be merged, as long as the items of the last round, which some CTAs go without, are short or nearly all there.
       q = paged_request<ROWS>(p, 0, false);
-      const int items = p.kv_heads * q.row_tiles, whole = ctas / items * items;
-      if (5 * whole >= 4 * ctas) ctas = whole;
-      // A prompt: many items, the first of few keys. Whole ones dealt out from the longest on, every other round backwards, end as evenly, and
-      // nothing has to be merged (8192 tokens, 32 / 8 heads: 505 us in equal shares, 487 so).
-      PagedItem first;
-      if (p.left < 0 && items >= 2 * ctas && q.tiles(p, 0, first) <= PA_DEAL) {
+      const int items = p.kv_heads * q.row_tiles, rounds = items / all_ctas, over = items - rounds * all_ctas;
+      PagedItem last;
+      const long idle = over == 0 ? 0 : static_cast<long>(all_ctas - over) * (q.tiles(p, q.row_tiles - 1 - rounds * all_ctas / p.kv_heads, last) + PA_ITEM_TILES<ROWS>);
+      if (idle <= static_cast<long>(PA_DEAL<ROWS>) * all_ctas) {
         deal = items;
         dealt = 0;
         deal_cta = cta;
-        deal_ctas = ctas;
+        deal_ctas = all_ctas;
         r = 0;
         return true;
       }
+      // A chunk behind a long context: all items have about the same keys, and as many CTAs as give each the same number of equal parts walk
+      // them in step, so that a key tile comes out of DRAM once for all (512 queries behind 32768 keys, 64 items, on the device: 148
+      // equal shares 265 us, 128 of them 260).
+      const int whole = ctas / items * items;
+      if (ROWS == 256 && 5 * whole >= 4 * ctas) ctas = whole;
     }
     if (cta >= ctas) return false;
     const auto border = [&](int k) -> long {            // total * k / ctas; (a 64-bit division is a hundred instructions)
@@ -309,7 +315,7 @@ struct PagedWalk {
   }
   // the next piece of this share; false: there is none. `part`: 0 whole item, 1 its beginning, 2 its middle, 3 its end
   __device__ __forceinline__ bool next(const PagedScalars& p, PagedItem& it, int& part) {
-    if (ROWS == 256 && deal > 0) {
+    if (ROWS >= 128 && deal > 0) {
       const int i = dealt * deal_ctas + (dealt & 1 ? deal_ctas - 1 - deal_cta : deal_cta);
       ++dealt;
       if (i >= deal) return false;
