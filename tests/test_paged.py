@@ -580,6 +580,19 @@ def test_attention_far_below_zero(device, context, new, heads, columns):
 
 
 @pytest.mark.parametrize("device", ["cpu", CUDA])
+def test_windows_of_any_size(device):
+    """Windows and sinks behind every length are none."""
+    dev = _dev(device)
+    q, kc, vc, table, ctx, cu, _, _ = _problem(dev, [300, 200], [1, 70], 8, 2, 16)
+    want = ua.paged_attention(q, kc, vc, table, ctx, cu)
+    for left, sink in ((1 << 30, 0), ((1 << 31) - 1, 1 << 31), (1 << 40, 5), ((1 << 62), (1 << 63) - 1)):
+        if device == "cpu" and sink >= 1 << 62:
+            continue
+        o, lse = ua.paged_attention(q, kc, vc, table, ctx, cu, window_size=(left, 0), sink_tokens=sink)
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.parametrize("device", ["cpu", CUDA])
 def test_attention_of_nothing(device):
     """No heads, no tokens, no requests; a bound of no new tokens, which one token may exceed unnoticed and no result is lost."""
     dev = _dev(device)

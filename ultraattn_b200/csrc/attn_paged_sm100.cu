@@ -725,7 +725,7 @@ static PagedPlan plan_paged(const UaPagedAttn* a) {
   //   tile is loaded twice as often
   const long item_tokens = 2 * PT >> d.pack_shift, items = (a->tokens / item_tokens + a->requests) * a->kv_heads;
   long tiles = ((a->columns << a->page_shift) + PT - 1) / PT;
-  if (a->left >= 0 && a->left < 1l << 31) tiles = std::min(tiles, (a->left + item_tokens) / PT + 2 + (a->sink + PT - 1) / PT);
+  if (a->left >= 0 && a->left < 1l << 31) tiles = std::min(tiles, (a->left + item_tokens) / PT + 2 + std::min(a->sink, 1l << 31) / PT + 1);
   const bool small = items <= sm_count() && items * tiles <= PA_SMALL_TILES * sm_count();
   add(most <= PT || small ? PT : 2 * PT, below, most);
   if (below > 0) add(below, 0, below);
